@@ -115,6 +115,27 @@ struct HeadArgs {
 const char* launch_head_loss(HeadArgs a, cudaStream_t st);
 const char* launch_head_score(HeadArgs a, cudaStream_t st);
 
+// layer_norm.cu  (return nullptr or a static error string)
+struct LayerNormArgs {
+  int kind;                             // of x, y, dy and dx: 0 fp32, 1 bf16, 2 fp16; rows behind one another, from 16-byte boundaries
+  long long rows;                       // at least one
+  int C;
+  const void* x;
+  const void* dy;
+  const float* gamma;                   // [C]; null: ones
+  const float* beta;                    // [C]; null: zeros
+  float eps;
+  void* y;
+  float* stats;                         // [2][rows] mean and 1 / sqrt(var + eps): written by fwd unless null, read by bwd
+  void* dx;                             // null: not wanted
+  float* dgamma;                        // [C]; null: not wanted
+  float* dbeta;
+  float* part;                          // workspace of bwd where dgamma or dbeta is wanted: layer_norm_part_rows() x [2][C]
+};
+const char* launch_layer_norm_fwd(const LayerNormArgs& a, cudaStream_t st);
+const char* launch_layer_norm_bwd(const LayerNormArgs& a, cudaStream_t st);
+int layer_norm_part_rows(const LayerNormArgs& a);
+
 // embed_input.cu  (return nullptr or a static error string)
 constexpr int kEmbedInputColumns = 128;
 struct EmbedInput {

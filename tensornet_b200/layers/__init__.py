@@ -1,8 +1,8 @@
 from .embedding_features import EmbeddingFeatures
 from .sequence_embedding_features import SequenceEmbeddingFeatures
-from .normalization_layer import TNBatchNormalizationBase, TNBatchNormalization, PCTRDNNBatchNormalization
+from .normalization_layer import TNBatchNormalizationBase, TNBatchNormalization, PCTRDNNBatchNormalization, LayerNormalization
 from .position_mapping import PositionMappingLayer
 from .dense import MLP, DenseHead, FMLayer, DeepCrossLayer
 
 __all__ = ["EmbeddingFeatures", "SequenceEmbeddingFeatures", "TNBatchNormalizationBase", "TNBatchNormalization",
-           "PCTRDNNBatchNormalization", "PositionMappingLayer", "MLP", "DenseHead", "FMLayer", "DeepCrossLayer"]
+           "PCTRDNNBatchNormalization", "LayerNormalization", "PositionMappingLayer", "MLP", "DenseHead", "FMLayer", "DeepCrossLayer"]

@@ -248,3 +248,25 @@ class PCTRDNNBatchNormalization(TNBatchNormalizationBase):
         if training:
             self._push_counted(self._local_stats(inputs, center=self.moving_mean))
         return self._normalize(inputs)
+
+
+class LayerNormalization(nn.Module):
+    """Normalises each row by its own moments, see :func:`tensornet_b200.ops.functional.layer_norm`: the layer between the blocks
+    of a sequence encoder, where :class:`TNBatchNormalization`'s statistics over examples and positions would mix sequences."""
+
+    def __init__(self, num_features: int, center=True, scale=True, epsilon=1e-5, name=None):
+        super().__init__()
+        self.num_features = int(num_features)
+        self.center, self.scale, self.epsilon = center, scale, epsilon
+        self.layer_name = name or "layer_normalization"
+        self.gamma = nn.Parameter(torch.ones(self.num_features)) if scale else None
+        self.beta = nn.Parameter(torch.zeros(self.num_features)) if center else None
+
+    def forward(self, inputs: torch.Tensor) -> torch.Tensor:
+        if inputs.shape[-1] != self.num_features:
+            raise ValueError(f"{self.layer_name}: rows of {self.num_features} columns, not {tuple(inputs.shape)}")
+        return F.layer_norm(inputs, self.gamma, self.beta, self.epsilon)
+
+    def get_config(self) -> dict:
+        return {"num_features": self.num_features, "center": self.center, "scale": self.scale, "epsilon": self.epsilon,
+                "name": self.layer_name}

@@ -652,6 +652,74 @@ def embed_input(anchor, link, ids, offsets, B, S, D, combiner, labels=None, labe
 
 
 # =========================================================================================
+# layer normalisation
+# =========================================================================================
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """``t`` contiguous from a 16-byte boundary."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gamma, beta, eps, keep):
+        C = x.shape[-1]
+        x2 = _rows16(x.detach()).view(-1, C)
+        rows = x2.shape[0]
+        y = torch.empty_like(x2)
+        stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if keep else None
+        g = None if gamma is None else gamma.detach().contiguous()
+        if rows:
+            _ext().layer_norm_fwd(x2, g, None if beta is None else beta.detach().contiguous(), eps, y, stats)
+        ctx.save_for_backward(x2 if x2.data_ptr() != x.data_ptr() else x, stats, gamma)
+        return y.view(x.shape)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, stats, gamma = ctx.saved_tensors
+        need_x, need_g, need_b = ctx.needs_input_grad[:3]
+        C = dy.shape[-1]
+        x2, dy2 = x.detach().reshape(-1, C), _rows16(dy).view(-1, C)
+        dx = torch.empty_like(dy2) if need_x else None
+        dg, db = [torch.empty(C, dtype=torch.float32, device=dy.device) if need else None for need in (need_g, need_b)]
+        if x2.shape[0]:
+            _ext().layer_norm_bwd(dy2, x2, stats, None if gamma is None else gamma.detach().contiguous(), dx, dg, db)
+        else:
+            for t in (dg, db):
+                if t is not None:
+                    t.zero_()
+        return None if dx is None else dx.view(dy.shape), dg, db, None, None
+
+
+def layer_norm(x: torch.Tensor, gamma: Optional[torch.Tensor] = None, beta: Optional[torch.Tensor] = None, eps: float = 1e-5) -> torch.Tensor:
+    """``(x - mean) / sqrt(var + eps) * gamma + beta`` with the moments of each row, the last dimension of ``x`` (fp32, bf16 or
+    fp16); the result has ``x``'s shape and type.  ``gamma`` and ``beta``: fp32 ``[columns]``, either may be left out.  Moments
+    and sums are fp32, and the gradients of ``gamma`` and ``beta`` are summed in a fixed order.  Differentiable once."""
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"layer_norm: rows of one column or more, not {tuple(x.shape)}")
+    if x.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise ValueError(f"layer_norm: fp32, bf16 or fp16, not {x.dtype}")
+    for name, p in (("gamma", gamma), ("beta", beta)):
+        if p is not None and (p.dtype != torch.float32 or p.shape != (x.shape[-1],) or p.device != x.device):
+            raise ValueError(f"layer_norm: {name} must be fp32 [{x.shape[-1]}] on {x.device}, not {p.dtype} {tuple(p.shape)} on {p.device}")
+    eps = float(eps)
+    if not 0.0 < eps < float("inf"):
+        raise ValueError(f"layer_norm: eps must be above zero, not {eps}")
+    if x.is_cuda:
+        keep = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gamma, beta))
+        return _LayerNorm.apply(x, gamma, beta, eps, keep)
+    f = x.float()
+    c = f - f.mean(dim=-1, keepdim=True)
+    y = c / torch.sqrt((c * c).mean(dim=-1, keepdim=True) + eps)
+    if gamma is not None:
+        y = y * gamma
+    if beta is not None:
+        y = y + beta
+    return y.to(x.dtype)
+
+
+# =========================================================================================
 # head + loss + head backward (GPU only)
 # =========================================================================================
 class _HeadLoss(torch.autograd.Function):
