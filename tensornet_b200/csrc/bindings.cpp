@@ -14,6 +14,7 @@
 
 #include "gemm_tcgen05.h"
 #include "mlp_fused.h"
+#include "sequence_ops.h"
 #include "tn_ops.h"
 #include "tn_types.h"
 
@@ -690,6 +691,9 @@ tn::MlpChainDesc chain_desc(bool backward, const at::Tensor& x, int in_cols, con
 
 }  // namespace
 
+cudaStream_t counted_stream() { return cur_stream(); }
+void count_launches(int n) { g_launches.fetch_add(n, std::memory_order_relaxed); }
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   py::class_<SparseCtx>(m, "SparseCtx")
       .def(py::init<py::dict, py::dict, py::dict>())
@@ -1160,58 +1164,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       if (const char* err = tn::launch_head_score(a, cur_stream())) throw std::runtime_error(err);
     });
   }
-  {
-    auto kind_of = [](const at::Tensor& x) {
-      TORCH_CHECK(x.scalar_type() == at::kFloat || x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf,
-                  "layer_norm: fp32, bf16 or fp16 rows");
-      return x.scalar_type() == at::kFloat ? 0 : x.scalar_type() == at::kBFloat16 ? 1 : 2;
-    };
-    auto rows_like = [](const at::Tensor& t, const at::Tensor& x, const char* what) {
-      TORCH_CHECK(t.is_cuda() && t.device() == x.device() && t.is_contiguous() && t.scalar_type() == x.scalar_type() && t.sizes() == x.sizes() &&
-                      reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, "layer_norm: ", what, " must be contiguous, like the input, on 16 bytes");
-    };
-    auto vec = [](const c10::optional<at::Tensor>& v, const at::Tensor& x, int64_t n, const char* what) -> float* {
-      if (!v) return nullptr;
-      TORCH_CHECK(v->is_cuda() && v->device() == x.device() && v->is_contiguous() && v->scalar_type() == at::kFloat && v->numel() == n,
-                  "layer_norm: ", what, " must be fp32, one value per column");
-      return ptr_of<float>(*v);
-    };
-    auto args_of = [kind_of, rows_like](const at::Tensor& x) {
-      TORCH_CHECK(x.dim() == 2 && x.size(0) >= 1 && x.size(1) >= 1 && x.size(1) < (1LL << 31) - 64, "layer_norm: rows of one column or more");
-      rows_like(x, x, "x");
-      tn::LayerNormArgs a{};
-      a.kind = kind_of(x); a.rows = x.size(0); a.C = (int)x.size(1); a.x = x.data_ptr();
-      return a;
-    };
-    // stats: fp32 [2, rows], what the backward pass needs of the forward one
-    m.def("layer_norm_fwd", [args_of, rows_like, vec](at::Tensor x, c10::optional<at::Tensor> gamma, c10::optional<at::Tensor> beta, double eps,
-                                                      at::Tensor y, c10::optional<at::Tensor> stats) {
-      c10::cuda::CUDAGuard guard(x.device());
-      tn::LayerNormArgs a = args_of(x);
-      rows_like(y, x, "y");
-      a.gamma = vec(gamma, x, a.C, "gamma"); a.beta = vec(beta, x, a.C, "beta"); a.eps = (float)eps;
-      a.y = y.data_ptr(); a.stats = vec(stats, x, 2 * a.rows, "stats");
-      if (const char* err = tn::launch_layer_norm_fwd(a, cur_stream())) throw std::runtime_error(err);
-    });
-    m.def("layer_norm_bwd", [args_of, rows_like, vec](at::Tensor dy, at::Tensor x, at::Tensor stats, c10::optional<at::Tensor> gamma,
-                                                      c10::optional<at::Tensor> dx, c10::optional<at::Tensor> dgamma,
-                                                      c10::optional<at::Tensor> dbeta) {
-      c10::cuda::CUDAGuard guard(x.device());
-      tn::LayerNormArgs a = args_of(x);
-      rows_like(dy, x, "the output's gradient");
-      if (dx) rows_like(*dx, x, "the input's gradient");
-      a.dy = dy.data_ptr(); a.gamma = vec(gamma, x, a.C, "gamma"); a.stats = vec(stats, x, 2 * a.rows, "stats");
-      a.dx = dx ? dx->data_ptr() : nullptr;
-      a.dgamma = vec(dgamma, x, a.C, "gamma's gradient"); a.dbeta = vec(dbeta, x, a.C, "beta's gradient");
-      at::Tensor part;
-      if (a.dgamma || a.dbeta) {
-        part = at::empty({(int64_t)tn::layer_norm_part_rows(a), 2, (int64_t)a.C}, x.options().dtype(at::kFloat));
-        a.part = ptr_of<float>(part);
-        g_launches.fetch_add(1, std::memory_order_relaxed);
-      }
-      if (const char* err = tn::launch_layer_norm_bwd(a, cur_stream())) throw std::runtime_error(err);
-    });
-  }
+  bind_sequence_ops(m);
   m.def("unique_assign", [](at::Tensor ids, c10::optional<at::Tensor> labels, at::Tensor dd_keys, at::Tensor dd_vals, at::Tensor uniq,
                             at::Tensor inverse, c10::optional<at::Tensor> show, c10::optional<at::Tensor> click, at::Tensor count,
                             at::Tensor status) {

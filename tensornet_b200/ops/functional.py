@@ -654,44 +654,6 @@ def embed_input(anchor, link, ids, offsets, B, S, D, combiner, labels=None, labe
 # =========================================================================================
 # layer normalisation
 # =========================================================================================
-def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """``t`` contiguous from a 16-byte boundary."""
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
-
-
-class _LayerNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, gamma, beta, eps, keep):
-        C = x.shape[-1]
-        x2 = _rows16(x.detach()).view(-1, C)
-        rows = x2.shape[0]
-        y = torch.empty_like(x2)
-        stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if keep else None
-        g = None if gamma is None else gamma.detach().contiguous()
-        if rows:
-            _ext().layer_norm_fwd(x2, g, None if beta is None else beta.detach().contiguous(), eps, y, stats)
-        ctx.save_for_backward(x2 if x2.data_ptr() != x.data_ptr() else x, stats, gamma)
-        return y.view(x.shape)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        x, stats, gamma = ctx.saved_tensors
-        need_x, need_g, need_b = ctx.needs_input_grad[:3]
-        C = dy.shape[-1]
-        x2, dy2 = x.detach().reshape(-1, C), _rows16(dy).view(-1, C)
-        dx = torch.empty_like(dy2) if need_x else None
-        dg, db = [torch.empty(C, dtype=torch.float32, device=dy.device) if need else None for need in (need_g, need_b)]
-        if x2.shape[0]:
-            _ext().layer_norm_bwd(dy2, x2, stats, None if gamma is None else gamma.detach().contiguous(), dx, dg, db)
-        else:
-            for t in (dg, db):
-                if t is not None:
-                    t.zero_()
-        return None if dx is None else dx.view(dy.shape), dg, db, None, None
-
-
 def layer_norm(x: torch.Tensor, gamma: Optional[torch.Tensor] = None, beta: Optional[torch.Tensor] = None, eps: float = 1e-5) -> torch.Tensor:
     """``(x - mean) / sqrt(var + eps) * gamma + beta`` with the moments of each row, the last dimension of ``x`` (fp32, bf16 or
     fp16); the result has ``x``'s shape and type.  ``gamma`` and ``beta``: fp32 ``[columns]``, either may be left out.  Moments
@@ -707,8 +669,7 @@ def layer_norm(x: torch.Tensor, gamma: Optional[torch.Tensor] = None, beta: Opti
     if not 0.0 < eps < float("inf"):
         raise ValueError(f"layer_norm: eps must be above zero, not {eps}")
     if x.is_cuda:
-        keep = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gamma, beta))
-        return _LayerNorm.apply(x, gamma, beta, eps, keep)
+        return _ext().layer_norm(x, gamma, beta, eps)
     f = x.float()
     c = f - f.mean(dim=-1, keepdim=True)
     y = c / torch.sqrt((c * c).mean(dim=-1, keepdim=True) + eps)
@@ -717,6 +678,111 @@ def layer_norm(x: torch.Tensor, gamma: Optional[torch.Tensor] = None, beta: Opti
     if beta is not None:
         y = y + beta
     return y.to(x.dtype)
+
+
+# =========================================================================================
+# attention within sequences
+# =========================================================================================
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, lengths: Optional[torch.Tensor] = None,
+              kv_lengths: Optional[torch.Tensor] = None, offsets: Optional[torch.Tensor] = None, kv_offsets: Optional[torch.Tensor] = None,
+              causal: bool = False, prefix: Optional[torch.Tensor] = None, cap: Optional[float] = None,
+              slopes: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> torch.Tensor:
+    """Scaled dot-product attention of each sequence's queries over its own keys; the result has ``q``'s shape.
+
+    Operands are bf16, 8 to 128 columns (a multiple of 8), with sums and softmax in fp32.  Padded ones are ``[B, T, heads,
+    columns]``, of which ``lengths`` / ``kv_lengths`` (int32 ``[B]``, at most ``T``) say how much is there (None: all); packed
+    ones ``[N, heads, columns]`` with the sequences one after another, ``offsets`` / ``kv_offsets`` (int32 ``[B + 1]``,
+    ascending, at most ``N``) saying where.  Queries may be padded and keys packed or the other way round.  Several query heads
+    may share a key head: query head ``h`` reads key head ``h // (heads / kv_heads)``.  Any strides are taken; operands whose rows
+    do not start on 16 bytes are copied first.
+
+    A sequence's queries stand at the end of its keys: query ``i`` of ``nq`` is at place ``i + nk - nq`` of ``nk`` keys, so that one
+    query is the newest token.  Its score with key ``j`` is ``scale * q.k``, with ``cap`` as ``cap * tanh(scale * q.k / cap)``, less
+    ``slopes[h] * |place - j|`` (fp32 ``[heads]``, constants).  ``causal`` hides the keys behind a query's place, but for the first
+    ``prefix[b]`` (int32 ``[B]``) keys of the sequence, which all its queries see.  ``scale`` defaults to ``columns ** -0.5``.
+
+    A query that sees no key has a zero result, and so have rows that belong to no sequence; their gradients are zero, and what
+    such rows hold is not looked at.  What a sequence holds has to be finite.  Differentiable once, in a fixed order of sums."""
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if t.dtype != torch.bfloat16 or t.dim() not in (3, 4) or t.device != q.device:
+            raise ValueError(f"attention: {name} must be bf16 [N, heads, columns] or [B, T, heads, columns] on {q.device}, "
+                             f"not {t.dtype} {tuple(t.shape)} on {t.device}")
+    H, D = q.shape[-2:]
+    G = k.shape[-2]
+    if k.shape != v.shape or k.shape[-1] != D:
+        raise ValueError(f"attention: keys {tuple(k.shape)} and values {tuple(v.shape)} must be alike, with the queries' {D} columns")
+    if D % 8 or not 8 <= D <= 128:
+        raise ValueError(f"attention: 8 to 128 columns, a multiple of 8, not {D}")
+    if H < 1 or G < 1 or H % G:
+        raise ValueError(f"attention: {H} query heads are no multiple of {G} key heads")
+    rows = []
+    for t, off, ln, what in ((q, offsets, lengths, ""), (k, kv_offsets, kv_lengths, "kv_")):
+        packed = t.dim() == 3
+        if packed and (off is None or ln is not None):
+            raise ValueError(f"attention: packed operands go with {what}offsets, not with {what}lengths")
+        if not packed and off is not None:
+            raise ValueError(f"attention: padded operands go with {what}lengths, not with {what}offsets")
+        r = off if packed else ln
+        if r is not None and (r.dtype != torch.int32 or r.dim() != 1 or r.device != q.device or (packed and r.numel() < 1)):
+            raise ValueError(f"attention: {what}{'offsets' if packed else 'lengths'} must be int32 [{'B + 1' if packed else 'B'}] on {q.device}")
+        rows.append(None if r is None else r.contiguous())
+    B = offsets.numel() - 1 if q.dim() == 3 else q.shape[0]
+    if B != (kv_offsets.numel() - 1 if k.dim() == 3 else k.shape[0]) or any(
+            t.dim() == 4 and r is not None and r.numel() != B for t, r in zip((q, k), rows)):
+        raise ValueError("attention: queries, keys and their lengths or offsets have different numbers of sequences")
+    if prefix is not None:
+        if not causal:
+            raise ValueError("attention: a prefix is what causal attention sees of later keys")
+        if prefix.dtype != torch.int32 or prefix.shape != (B,) or prefix.device != q.device:
+            raise ValueError(f"attention: prefix must be int32 [{B}] on {q.device}")
+        prefix = prefix.contiguous()
+    if slopes is not None:
+        if slopes.dtype != torch.float32 or slopes.shape != (H,) or slopes.device != q.device:
+            raise ValueError(f"attention: slopes must be fp32 [{H}] on {q.device}")
+        if slopes.requires_grad:
+            raise ValueError("attention: slopes are constants, they have no gradient")
+        slopes = slopes.contiguous()
+    cap = 0.0 if cap is None else float(cap)
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not 0.0 <= cap < float("inf") or not 0.0 < scale < float("inf"):
+        raise ValueError(f"attention: scale ({scale}) must be above zero, and so must cap ({cap or None})")
+    if q.is_cuda:
+        return _ext().attention(q, k, v, rows[0], rows[1], prefix, slopes, bool(causal), cap, scale, _status())
+    return _attention_cpu(q, k, v, rows, B, bool(causal), prefix, cap, slopes, scale)
+
+
+def _attention_cpu(q, k, v, rows, B, causal, prefix, cap, slopes, scale):
+    R = q.shape[-2] // k.shape[-2]
+    out = torch.zeros(q.shape, dtype=torch.float32)
+
+    def where(t, r, b):
+        if t.dim() == 3:
+            lo = min(max(int(r[b]), 0), t.shape[0])
+            return slice(lo, min(max(int(r[b + 1]), lo), t.shape[0]))
+        return b, slice(0, t.shape[1] if r is None else min(max(int(r[b]), 0), t.shape[1]))
+
+    for b in range(B):
+        wq, wk = where(q, rows[0], b), where(k, rows[1], b)
+        qb = q[wq].float().transpose(0, 1)
+        kb, vb = [t[wk].float().transpose(0, 1).repeat_interleave(R, dim=0) for t in (k, v)]
+        nq, nk = qb.shape[1], kb.shape[1]
+        if not nq or not nk:
+            continue
+        s = qb @ kb.transpose(1, 2) * scale
+        if cap:
+            s = cap * torch.tanh(s / cap)
+        place = torch.arange(nq).unsqueeze(1) + (nk - nq)
+        j = torch.arange(nk)
+        if slopes is not None:
+            s = s - slopes.view(-1, 1, 1) * (place - j).abs()
+        seen = torch.ones((nq, nk), dtype=torch.bool)
+        if causal:
+            seen = j <= place
+            if prefix is not None:
+                seen = seen | (j < int(prefix[b]))
+        p = torch.softmax(s.masked_fill(~seen, -3e38), dim=-1) * seen.any(dim=-1, keepdim=True)
+        out[wq] = (p @ vb).transpose(0, 1)
+    return out.to(q.dtype)
 
 
 # =========================================================================================

@@ -176,6 +176,5 @@ def test_second_derivatives_are_refused(tn_gpu, status_ok):
     from tensornet_b200.ops import functional as F
 
     x = _made(tn_gpu.core.runtime().device, 4, 8).requires_grad_()
-    (g,) = torch.autograd.grad(F.layer_norm(x).square().sum(), x, create_graph=True)
-    with pytest.raises(RuntimeError):
-        g.sum().backward()
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(F.layer_norm(x).square().sum(), x, create_graph=True)
