@@ -1,4 +1,4 @@
-// Attention within sequences: what the launchers of attention.cu take.
+// Attention within sequences: what the launchers of attention_fwd.cu and attention_bwd.cu take.
 #pragma once
 #include <cuda_runtime.h>
 

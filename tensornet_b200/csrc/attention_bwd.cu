@@ -1,6 +1,5 @@
-// Attention within sequences, forward and backward: a warp per row.
+// Attention within sequences, backward: a warp per row.
 //
-//   p = softmax over the visible keys of s;  o = p v
 //   dv = p^T do;  dp = do v^T;  ds = p (dp - sum(do o)) (1 - tanh^2) scale;  dq = ds k;  dk = ds^T q
 //
 // A lane scores one key (or query) of 32, then the 32 weights pass around the warp while the lanes own columns of the result.
@@ -72,39 +71,6 @@ __device__ __forceinline__ Place place_of(const AttnArgs& a, const AttnRows& r, 
     if (p.i >= span_of(r, p.seq).n) p.seq = -1;
   }
   return p;
-}
-
-__global__ void __launch_bounds__(32 * kWarps) attention_fwd_kernel(const AttnArgs a, long long rows) {
-  pdl_sync();
-  __shared__ float s_q[kWarps][128];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h = blockIdx.y;
-  const long long row = (long long)blockIdx.x * kWarps + warp;
-  if (row >= rows) return;
-  const Place p = place_of(a, a.rq, row);
-  float acc[kCols] = {}, m = -CUDART_INF_F, l = 0.f;
-  if (p.seq >= 0) {
-    const int g = h / (a.H / a.G), lim = keys_seen(a, p.seq, p.i, p.nq, p.nk);
-    const float slope2 = a.slopes ? a.slopes[h] * kLog2e : 0.f;
-    load_row(at(a.q, p.b, p.t, h), s_q[warp], a.D, lane);
-    __syncwarp();
-    for (int j0 = 0; j0 < lim; j0 += 32) {
-      const int j = j0 + lane;
-      float s = -CUDART_INF_F, th;
-      if (j < lim) s = score_of(a, dot(at(a.k, p.keys.b, p.keys.first + j, g), s_q[warp], a.D), slope2, p.i + p.nk - p.nq - j, th);
-      float top = s;
-      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      top = fmaxf(top, m);
-      const float old = exp2f(m - top), w = exp2f(s - top);
-      m = top;
-      l = l * old + warp_sum(w);
-#pragma unroll
-      for (int i = 0; i < kCols; ++i) acc[i] *= old;
-      const int n = min(32, lim - j0);
-      for (int k = 0; k < n; ++k) add_row(at(a.v, p.keys.b, p.keys.first + j0 + k, g), __shfl_sync(0xffffffffu, w, k), acc, a.D, lane);
-    }
-  }
-  store_row(at_out(a.o, p.b, p.t, h), acc, l > 0.f ? 1.f / l : 0.f, a.D, lane);
-  if (a.lse != nullptr && lane == 0) a.lse[h * rows + row] = l > 0.f ? m + log2f(l) : CUDART_INF_F;
 }
 
 __global__ void __launch_bounds__(32 * kWarps) attention_dq_kernel(const AttnArgs a, long long rows) {
@@ -185,11 +151,6 @@ const char* told(cudaError_t e) {
 }
 
 }  // namespace
-
-const char* launch_attention_fwd(const AttnArgs& a, cudaStream_t st) {
-  const long long n = rows_of(a.rq, a.B);
-  return told(launch_pdl(attention_fwd_kernel, dim3((unsigned)((n + kWarps - 1) / kWarps), a.H), dim3(32 * kWarps), 0, st, a, n));
-}
 
 const char* launch_attention_bwd(const AttnArgs& a, cudaStream_t st) {
   const long long nq = rows_of(a.rq, a.B), nk = rows_of(a.rk, a.B);

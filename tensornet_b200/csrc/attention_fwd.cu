@@ -1,0 +1,367 @@
+// Attention within sequences, forward, on the tensor cores.
+//
+//   s = scores of 128 queries with 128 keys;  m = the largest so far;  p = 2^(s - m);  l += sum p;  o += p v;  out = o / l
+//
+// One pass over the keys.  A block has one or two tiles of 128 queries: a warp loads tiles of keys and values by TMA into a ring, a
+// warp issues the products, and a warpgroup per tile has a query per thread, so that maxima and sums never leave a thread.  Scores
+// are read from tensor memory into registers, and the weights go back into the columns that the scores had, as the left operand
+// of the product with the values.
+//
+// The order of products is  s0(0) s1(0) | o0(0) s0(1) | o1(0) s1(1) | ...: while one tile's weights are made, the other's products
+// run.  Products of one thread run in the order of their issue, so the next scores may overwrite the weights that the
+// product before them reads, and a barrier behind s(j + 1) also says that o(j) is there.
+//
+// The reference m of a row moves only when its maximum has grown by more than 2^8: weights then stay below 2^8, and what has been
+// added up is brought to the new reference by the thread that owns the row.  Sums are fp32, weights bf16 for the product (their
+// sum takes them unrounded).
+#include <cuda_bf16.h>
+#include <mutex>
+#include "attention_tc.cuh"
+
+namespace tn {
+
+namespace {
+
+using namespace attn;
+
+constexpr int kRows = 128;
+constexpr float kGrowth = 8.f;
+
+template <int kD, int kTiles>
+struct FwdShape {
+  static constexpr int chunks = kD / 64;
+  static constexpr int tile_bytes = kRows * 128 * chunks;
+  static constexpr int slots = kTiles == 2 ? (kD == 128 ? 4 : 6) : (kD == 128 ? 2 : 4);
+  static constexpr int softmax_warps = 4 * kTiles;
+  static constexpr int threads = 32 * (softmax_warps + 2);
+  static constexpr int smem = tile_bytes * (kTiles + slots) + 1024;
+  static constexpr int tmem_cols = kTiles == 2 ? 512 : 256;
+  static constexpr int o_col = 128 * kTiles;
+};
+
+struct FwdMaps {
+  CUtensorMap q, k, v;
+};
+
+template <int kD, int kTiles, bool kCap, bool kBias>
+__global__ void __launch_bounds__(FwdShape<kD, kTiles>::threads, kTiles == 2 ? 1 : 2)
+attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_constant__ AttnArgs a) {
+  using Shape = FwdShape<kD, kTiles>;
+  constexpr int kSlots = Shape::slots;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t s_q, s_full[kSlots], s_empty[kSlots], s_score[kTiles], s_weight[kTiles], s_out[kTiles];
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_abort_i;
+  volatile int* s_abort = &s_abort_i;
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  const int h = blockIdx.y;
+
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  // the last tiles of causal sequences have the most keys: they go first
+  const Tile tile = tile_of(a.rq, a.B, kRows * kTiles, (int)(gridDim.x - 1 - blockIdx.x));
+  if (!tile.any) return;
+  const int tile_rows = min(kRows * kTiles, tile.rows.n - tile.first);      // of the output that are this block's
+  Span qs{tile.rows.b, tile.rows.first, 0}, ks{0, 0, 0};
+  if (tile.seq >= 0) {
+    qs = span_of(a.rq, tile.seq);
+    ks = span_of(a.rk, tile.seq);
+  }
+  // keys that tile t sees, none where it has no queries; keys_seen grows with the query
+  int vis[kTiles], most = 0;
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t) {
+    const int i0 = tile.first + t * kRows;
+    vis[t] = i0 < qs.n ? keys_seen(a, tile.seq, min(i0 + kRows, qs.n) - 1, qs.n, ks.n) : 0;
+    most = max(most, vis[t]);
+  }
+  if (most == 0) {
+    const int per = a.D / 8;
+    for (int i = threadIdx.x; i < tile_rows * per; i += Shape::threads)
+      *reinterpret_cast<uint4*>(at_out(a.o, tile.rows.b, tile.rows.first + tile.first + i / per, h) + i % per * 8) = make_uint4(0, 0, 0, 0);
+    if (a.lse != nullptr && tile.seq >= 0)
+      for (int i = threadIdx.x; i < tile_rows; i += Shape::threads)
+        a.lse[(long long)h * (a.rq.off ? a.rq.T : (long long)a.B * a.rq.T) + (a.rq.off ? 0 : (long long)tile.rows.b * a.rq.T) + tile.rows.first +
+              tile.first + i] = CUDART_INF_F;
+    return;
+  }
+  const int steps = (most + kRows - 1) / kRows;
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem_gen = smem_raw + (base - smem_u32(smem_raw));
+  const uint32_t ring = base + kTiles * Shape::tile_bytes;
+
+  if (threadIdx.x == 0) {
+    *s_abort = 0;
+    mbar_init(smem_u32(&s_q), 1);
+    for (int s = 0; s < kSlots; ++s) { mbar_init(smem_u32(&s_full[s]), 1); mbar_init(smem_u32(&s_empty[s]), 1); }
+    for (int t = 0; t < kTiles; ++t) {
+      mbar_init(smem_u32(&s_score[t]), 1);
+      mbar_init(smem_u32(&s_weight[t]), kRows);
+      mbar_init(smem_u32(&s_out[t]), 1);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 0) tmem_alloc<Shape::tmem_cols>(&s_tmem);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  const int d16 = round16(a.D);
+
+  if (warp == Shape::softmax_warps) {
+    // ---- loads: the queries, then k(0) v(0) k(1) v(1) ... through the ring
+    const int g = h / (a.H / a.G);
+    const bool lead = elect_one();
+    if (lead) {
+      int n = 0;
+      for (int t = 0; t < kTiles; ++t) n += vis[t] > 0;
+      mbar_expect_tx(smem_u32(&s_q), n * Shape::tile_bytes);
+      for (int t = 0; t < kTiles; ++t)
+        if (vis[t] > 0)
+          for (int c = 0; c < Shape::chunks; ++c)
+            tma_load_4d(base + t * Shape::tile_bytes + c * (kRows * 128), &maps.q, 64 * c, qs.first + tile.first + t * kRows, h, qs.b, smem_u32(&s_q));
+    }
+    __syncwarp();
+    for (int i = 0; i < 2 * steps; ++i) {
+      const int s = i % kSlots;
+      if (i >= kSlots && !mbar_wait_warp(smem_u32(&s_empty[s]), ((i / kSlots) & 1) ^ 1, s_abort)) { *s_abort = 1; break; }
+      if (lead) {
+        const uint32_t bar = smem_u32(&s_full[s]);
+        mbar_expect_tx(bar, Shape::tile_bytes);
+        for (int c = 0; c < Shape::chunks; ++c)
+          tma_load_4d(ring + s * Shape::tile_bytes + c * (kRows * 128), (i & 1) ? &maps.v : &maps.k, 64 * c, ks.first + (i >> 1) * kRows, g, ks.b, bar);
+      }
+      __syncwarp();
+    }
+  } else if (warp == Shape::softmax_warps + 1) {
+    // ---- products
+    const bool lead = elect_one();
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    bool ok = mbar_wait_warp(smem_u32(&s_q), 0, s_abort);
+    auto full = [&](int i) {           // load i of the ring has landed
+      ok = ok && mbar_wait_warp(smem_u32(&s_full[i % kSlots]), (i / kSlots) & 1, s_abort);
+      tc_fence_after();
+    };
+    auto scores = [&](int t, int j) {
+      const uint32_t q = base + t * Shape::tile_bytes, k = ring + (2 * j % kSlots) * Shape::tile_bytes;
+      const uint32_t id = idesc_of(round16(min(kRows, vis[t] - j * kRows)), false);
+      if (lead) {
+        for (int s = 0; s < d16 / 16; ++s) umma_f16(tm + t * 128, desc_k<kRows>(q, s), desc_k<kRows>(k, s), id, s > 0);
+        umma_commit(smem_u32(&s_score[t]));
+      }
+      __syncwarp();
+    };
+    auto values = [&](int t, int j) {
+      const uint32_t v = ring + ((2 * j + 1) % kSlots) * Shape::tile_bytes;
+      const int n = round16(min(kRows, vis[t] - j * kRows)) / 16;
+      const uint32_t id = idesc_of(d16, true);
+      if (lead)
+        for (int s = 0; s < n; ++s) umma_f16_ts(tm + Shape::o_col + t * kD, tm + t * 128 + s * 8, desc_mn<kRows>(v, s), id, j > 0 || s > 0);
+      __syncwarp();
+    };
+    auto free_slot = [&](int i) {
+      if (lead && i + kSlots < 2 * steps) umma_commit(smem_u32(&s_empty[i % kSlots]));
+      __syncwarp();
+    };
+    full(0);
+    if (ok) {
+      for (int t = 0; t < kTiles; ++t)
+        if (vis[t] > 0) scores(t, 0);
+      free_slot(0);
+    }
+    for (int j = 0; j < steps && ok; ++j) {
+      full(2 * j + 1);
+      if (!ok) break;
+      const int end = ks.n - j * kRows;            // rows of this tile of values that the sequence has
+      if (end < kRows && (end & 15)) zero_rows<kRows>(smem_gen + (ring - base) + ((2 * j + 1) % kSlots) * Shape::tile_bytes, Shape::chunks, end, round16(end), lane);
+      bool next = false;
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) {
+        if (j * kRows >= vis[t]) continue;
+        ok = ok && mbar_wait_warp(smem_u32(&s_weight[t]), j & 1, s_abort);
+        if (!ok) break;
+        tc_fence_after();
+        values(t, j);
+        if ((j + 1) * kRows < vis[t]) {
+          if (!next) full(2 * j + 2);
+          if (!ok) break;
+          next = true;
+          scores(t, j + 1);
+        } else {
+          if (lead) umma_commit(smem_u32(&s_out[t]));
+          __syncwarp();
+        }
+      }
+      free_slot(2 * j + 1);
+      if (next) free_slot(2 * j + 2);
+    }
+    if (!ok) *s_abort = 1;
+  } else {
+    // ---- softmax: a query per thread
+    const int t = warp >> 2, r = (warp & 3) * 32 + lane;
+    const int i = tile.first + t * kRows + r;
+    const uint32_t tm = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t tm_s = tm + t * 128, tm_o = tm + Shape::o_col + t * kD;
+    const int my_vis = t == 0 ? vis[0] : vis[kTiles - 1];
+    const int lim = i < qs.n ? keys_seen(a, tile.seq, i, qs.n, ks.n) : my_vis;
+    const int least = keys_seen(a, tile.seq, tile.first + t * kRows, qs.n, ks.n);      // of the tile's queries
+    const float c = kCap ? 2.f * kLog2e * a.scale / a.cap : a.scale * kLog2e;
+    const float cap2 = a.cap * kLog2e;
+    const float slope2 = kBias ? a.slopes[h] * kLog2e : 0.f;
+    const int place = i + ks.n - qs.n;
+    float m = kNone, l = 0.f;
+    bool ok = true;
+    for (int j = 0; j * kRows < my_vis; ++j) {
+      if (!mbar_wait_warp(smem_u32(&s_score[t]), j & 1, s_abort)) { *s_abort = 1; ok = false; break; }
+      tc_fence_after();
+      const int wide = min(kRows, my_vis - j * kRows);              // columns of scores
+      const bool masked = (j + 1) * kRows > least;
+      float s[kRows];
+#pragma unroll
+      for (int c0 = 0; c0 < kRows; c0 += 32)
+        if (c0 < wide) tmem_ld32_nowait(tm_s + c0, reinterpret_cast<uint32_t*>(s + c0));
+      tmem_ld_wait();
+      float top = kNone;
+#pragma unroll
+      for (int c0 = 0; c0 < kRows; c0 += 32) {
+        if (c0 >= wide) continue;
+#pragma unroll
+        for (int e = c0; e < c0 + 32; ++e) {
+          float x = s[e];
+          if (kCap) x = cap2 - __fdividef(2.f * cap2, 1.f + ex2(x * c));
+          if (kBias) x = (kCap ? x : x * c) - slope2 * fabsf((float)(place - (j * kRows + e)));
+          if (masked) x = j * kRows + e < lim ? x : kNone;
+          s[e] = x;
+          top = fmaxf(top, x);
+        }
+      }
+      if (!kCap && !kBias) top *= c;
+      const bool grown = top > m + kGrowth;
+      if (__any_sync(0xffffffffu, grown)) {
+        const float to = grown ? top : m;
+        const float by = to == kNone ? 1.f : ex2(m - to);
+        m = to;
+        l *= by;
+        if (j > 0) {
+          for (int c0 = 0; c0 < d16; c0 += 16) {
+            float o[16];
+            tmem_ld16_nowait(tm_o + c0, reinterpret_cast<uint32_t*>(o));
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] *= by;
+            tmem_st16(tm_o + c0, reinterpret_cast<const uint32_t*>(o));
+          }
+        }
+      }
+      const float ref = m == kNone ? 0.f : m;
+#pragma unroll
+      for (int c0 = 0; c0 < kRows; c0 += 32) {
+        if (c0 >= wide) continue;
+        uint32_t w[16];
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          const float p0 = ex2((kCap || kBias) ? s[c0 + e] - ref : fmaf(s[c0 + e], c, -ref));
+          const float p1 = ex2((kCap || kBias) ? s[c0 + e + 1] - ref : fmaf(s[c0 + e + 1], c, -ref));
+          l += p0 + p1;
+          w[e / 2] = pack_bf16(p0, p1);
+        }
+        tmem_st16(tm_s + c0 / 2, w);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(smem_u32(&s_weight[t]));
+    }
+    if (ok && my_vis > 0) {
+      ok = mbar_wait_warp(smem_u32(&s_out[t]), 0, s_abort);
+      if (!ok) *s_abort = 1;
+      tc_fence_after();
+    }
+    if (ok) {
+      const float w = l > 0.f && i < qs.n ? 1.f / l : 0.f;
+      const bool mine = t * kRows + r < tile_rows;
+      const long long row = tile.rows.first + i;
+      __nv_bfloat16* out = at_out(a.o, tile.rows.b, row, h);
+      for (int c0 = 0; c0 < a.D; c0 += 16) {
+        float o[16];
+        if (my_vis > 0) {
+          tmem_ld16_nowait(tm_o + c0, reinterpret_cast<uint32_t*>(o));
+          tmem_ld_wait();
+        }
+        if (!mine) continue;
+        const bool some = w != 0.f;         // (what a row without weights holds may be anything)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[e] = some ? o[e] : 0.f;
+        *reinterpret_cast<uint4*>(out + c0) = pack8(o, w);
+        if (c0 + 8 < a.D) *reinterpret_cast<uint4*>(out + c0 + 8) = pack8(o + 8, w);
+      }
+      if (a.lse != nullptr && mine)
+        a.lse[(long long)h * (a.rq.off ? a.rq.T : (long long)a.B * a.rq.T) + (a.rq.off ? 0 : (long long)tile.rows.b * a.rq.T) + row] =
+            w != 0.f ? m + log2f(l) : CUDART_INF_F;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (*s_abort) {
+    if (threadIdx.x == 0) set_status(a.status, kMbarTimeout, 40, (int)blockIdx.x);
+    for (int i = 0; i < 2000; ++i) __nanosleep(1000);        // copies in flight land
+    __syncthreads();
+  }
+  if (warp == 0) tmem_dealloc<Shape::tmem_cols>(tmem);
+}
+
+template <int kD, int kTiles, bool kCap, bool kBias>
+cudaError_t launch(const FwdMaps& maps, const AttnArgs& a, cudaStream_t st) {
+  using Shape = FwdShape<kD, kTiles>;
+  auto* k = attention_fwd_tc_kernel<kD, kTiles, kCap, kBias>;
+  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::smem);      // of the current device
+  if (e != cudaSuccess) return e;
+  return launch_pdl(k, dim3((unsigned)tile_count(a.rq, a.B, kRows * kTiles), a.H), dim3(Shape::threads), Shape::smem, st, maps, a);
+}
+template <int kD, int kTiles>
+cudaError_t launch(const FwdMaps& maps, const AttnArgs& a, cudaStream_t st) {
+  if (a.cap > 0.f) return a.slopes ? launch<kD, kTiles, true, true>(maps, a, st) : launch<kD, kTiles, true, false>(maps, a, st);
+  return a.slopes ? launch<kD, kTiles, false, true>(maps, a, st) : launch<kD, kTiles, false, false>(maps, a, st);
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &found) == cudaSuccess && found == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(ptr);
+  });
+  return fn;
+}
+
+}  // namespace
+
+namespace attn {
+bool operand_map(const AttnOperand& o, int D, const AttnRows& r, int B, int heads, int box_rows, CUtensorMap* out) {
+  EncodeTiledFn enc = encode_fn();
+  if (!enc) return false;
+  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)r.T, (cuuint64_t)heads, (cuuint64_t)(r.off ? 1 : B)};
+  const cuuint64_t strides[3] = {(cuuint64_t)o.st * 2, (cuuint64_t)o.sh * 2, r.off ? (cuuint64_t)16 : (cuuint64_t)o.sb * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1}, step[4] = {1, 1, 1, 1};
+  return enc(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, o.p, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+}  // namespace attn
+
+const char* launch_attention_fwd(const AttnArgs& a, cudaStream_t st) {
+  FwdMaps maps;
+  if (!operand_map(a.q, a.D, a.rq, a.B, a.H, kRows, &maps.q) || !operand_map(a.k, a.D, a.rk, a.B, a.G, kRows, &maps.k) ||
+      !operand_map(a.v, a.D, a.rk, a.B, a.G, kRows, &maps.v))
+    return "attention: cuTensorMapEncodeTiled failed";
+  const bool two = a.rq.off ? a.rq.T > 256LL * a.B : a.rq.T > kRows;
+  cudaError_t e = a.D > 64 ? (two ? launch<128, 2>(maps, a, st) : launch<128, 1>(maps, a, st))
+                           : (two ? launch<64, 2>(maps, a, st) : launch<64, 1>(maps, a, st));
+  if (e == cudaSuccess) e = cudaGetLastError();
+  return e == cudaSuccess ? nullptr : cudaGetErrorString(e);
+}
+
+}  // namespace tn

@@ -1,0 +1,96 @@
+// Instructions and layouts that the tensor-core attention kernels share.
+//
+// Every operand tile lies in shared memory as chunks of 64 columns, [rows][128 bytes] with the 128-byte swizzle, so that one tile
+// serves as either side of a product: along its columns (K-major) for q k^T, along its rows (MN-major) for p v.
+#pragma once
+#include <cuda.h>
+#include "attention_rows.cuh"
+#include "tc_primitives.cuh"
+
+namespace tn {
+namespace attn {
+
+using namespace tc;
+
+constexpr float kNone = -__builtin_huge_valf();
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int t, int h, int b, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(t), "r"(h), "r"(b)
+      : "memory");
+}
+// A from tensor memory: lane = row, two bf16 along the contraction per column
+__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accum) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accum)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]), "r"(r[1]),
+      "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
+      "r"(r[14]), "r"(r[15]), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+template <int kCols>
+__device__ __forceinline__ uint32_t tmem_alloc(uint32_t* slot) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "n"(kCols) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  return 0;
+}
+template <int kCols>
+__device__ __forceinline__ void tmem_dealloc(uint32_t tmem) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kCols) : "memory");
+}
+
+// fp32 results of bf16 operands, 128 rows, n columns; b_mn: B lies with its output columns behind one another
+__device__ __forceinline__ uint32_t idesc_of(int n, bool b_mn) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+// Step ks of 16 along the columns of a tile of kRows rows
+template <int kRows>
+__device__ __forceinline__ uint64_t desc_k(uint32_t tile, int ks) {
+  return make_smem_desc(tile + (ks >> 2) * (kRows * 128) + (ks & 3) * 32, 16u, 1024u);
+}
+// Step ks of 16 along its rows
+template <int kRows>
+__device__ __forceinline__ uint64_t desc_mn(uint32_t tile, int ks) {
+  return make_smem_desc(tile + ks * 2048, kRows * 128, 1024u);
+}
+
+__device__ __forceinline__ int round16(int n) { return (n + 15) & ~15; }
+
+// Rows [from, to) of a tile set to zero by one warp: rows behind the end of a sequence hold anything, and a weight of zero times a
+// NaN is a NaN.
+template <int kRows>
+__device__ __forceinline__ void zero_rows(uint8_t* tile, int chunks, int from, int to, int lane) {
+  const int per = (to - from) * 8;
+  for (int i = lane; i < per * chunks; i += 32)
+    *reinterpret_cast<uint4*>(tile + (i / per) * (kRows * 128) + from * 128 + (i % per) * 16) = make_uint4(0, 0, 0, 0);
+  fence_proxy_async_smem();
+  __syncwarp();
+}
+
+// Eight bf16 of zero, or of fp32 values times w, to a row
+__device__ __forceinline__ uint4 pack8(const float* f, float w) {
+  return make_uint4(pack_bf16(f[0] * w, f[1] * w), pack_bf16(f[2] * w, f[3] * w), pack_bf16(f[4] * w, f[5] * w), pack_bf16(f[6] * w, f[7] * w));
+}
+
+// [rows, 64 columns] boxes of an operand; columns beyond D and rows beyond T come as zeros
+bool operand_map(const AttnOperand& o, int D, const AttnRows& r, int B, int heads, int box_rows, CUtensorMap* out);
+
+}  // namespace attn
+}  // namespace tn
