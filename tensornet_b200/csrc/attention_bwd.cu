@@ -1,11 +1,20 @@
-// Attention within sequences, backward: a warp per row.
+// Attention within sequences, backward, on the tensor cores.
 //
-//   dv = p^T do;  dp = do v^T;  ds = p (dp - sum(do o)) (1 - tanh^2) scale;  dq = ds k;  dk = ds^T q
+//   p = 2^(s - lse);  dp = do v^T;  ds = p (dp - delta) ds/dx  with delta = sum(do o)
+//   dv = p^T do;  dk = scale ds^T q;  dq = scale ds k
 //
-// A lane scores one key (or query) of 32, then the 32 weights pass around the warp while the lanes own columns of the result.
+// Every result has one owner, so no sums meet in memory and their order is fixed: a block owns 128 keys and walks over the queries
+// of all heads that share them (dk, dv), or owns 128 queries and walks over their keys (dq).  That costs the scores and dp twice,
+// seven products in place of five; sums of dq in memory would need a pass of their own over fp32 rows, and an order.
+//
+// Both kinds of block are one program.  X are the two operands of the 128 rows that it owns, Y those of the 64 rows at a time that
+// it walks over: (K, V) and (Q, dO), or (Q, dO) and (K, V).
+//   s = X1 Y1^T, dp = X2 Y2^T  [128, 64];   acc1 += ds Y1;   acc2 += p Y2 (keys' owners only)
+// A row of the block is a thread's, so p and ds are made in registers and go back into the columns of tensor memory that s and dp
+// had, as left operands; the tiles of Y serve as right operands of both kinds of product.  Where keys own the rows, queries are
+// columns, and their lse and delta come through shared memory.
 #include <cuda_bf16.h>
-#include "attention_rows.cuh"
-#include "tn_device.cuh"
+#include "attention_tc.cuh"
 
 namespace tn {
 
@@ -13,150 +22,377 @@ namespace {
 
 using namespace attn;
 
-constexpr int kWarps = 8;
-constexpr int kCols = 4;      // columns of a row per lane, 128 / 32
+constexpr int kX = 128, kY = 64;
 
-__device__ __forceinline__ float dot(const __nv_bfloat16* a, const float* b, int D) {
-  float s = 0.f;
-  for (int d = 0; d < D; d += 8) {
-    const uint4 v = *reinterpret_cast<const uint4*>(a + d);
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s += __uint_as_float(w[i] << 16) * b[d + 2 * i] + __uint_as_float(w[i] & 0xffff0000u) * b[d + 2 * i + 1];
-  }
-  return s;
-}
-__device__ __forceinline__ void load_row(const __nv_bfloat16* p, float* s, int D, int lane) {
-  for (int d = lane; d < D; d += 32) s[d] = __bfloat162float(p[d]);
-}
-__device__ __forceinline__ void add_row(const __nv_bfloat16* p, float w, float* acc, int D, int lane) {
-#pragma unroll
-  for (int i = 0; i < kCols; ++i)
-    if (lane + 32 * i < D) acc[i] += w * __bfloat162float(p[lane + 32 * i]);
-}
-__device__ __forceinline__ void store_row(__nv_bfloat16* p, const float* acc, float w, int D, int lane) {
-#pragma unroll
-  for (int i = 0; i < kCols; ++i)
-    if (lane + 32 * i < D) p[lane + 32 * i] = __float2bfloat16_rn(acc[i] * w);
-}
-__device__ __forceinline__ float warp_sum(float v) {
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
-struct Place {
-  int seq, b, t, i, nq, nk;     // i: of the row within its sequence; seq -1: in none
-  Span keys, queries;
+// kD 128: two stages of s and dp and a warpgroup for each, a block per SM.  kD 64: one stage, two blocks per SM take turns.
+template <int kD>
+struct BwdShape {
+  static constexpr int chunks = kD / 64;
+  static constexpr int stages = kD == 128 ? 2 : 1;
+  static constexpr int slots = kD == 128 ? 4 : 3;
+  static constexpr int x_bytes = kX * 128 * chunks, y_bytes = kY * 128 * chunks;      // of one operand
+  static constexpr int soft_warps = 4 * stages;
+  static constexpr int threads = 32 * (soft_warps + 2);
+  static constexpr int smem = 2 * x_bytes + slots * 2 * y_bytes + 1024;
+  static constexpr int acc_col = 2 * kY * stages;
+  static constexpr int tmem_cols = kD == 128 ? 512 : 256;
 };
-// The row `at` of an operand's rows, over all sequences
-__device__ __forceinline__ Place place_of(const AttnArgs& a, const AttnRows& r, long long row) {
-  Place p{};
-  const Tile t = tile_of(r, a.B, 1, r.off == nullptr ? (int)row : 0);
-  if (r.off == nullptr) {
-    p.seq = t.seq; p.b = t.seq; p.t = t.first; p.i = t.first;
+
+struct BwdMaps {
+  CUtensorMap q, k, v, go;      // boxes of 64 rows
+};
+
+template <int kD>
+struct BwdShared {
+  uint64_t x, full[BwdShape<kD>::slots], empty[BwdShape<kD>::slots], score[BwdShape<kD>::stages], weight[BwdShape<kD>::stages], acc;
+  uint32_t tmem;
+  int abort;
+  alignas(16) float vec[BwdShape<kD>::stages][2][2 * kY];      // lse and delta of a tile of queries
+};
+
+__device__ __forceinline__ long long flat_rows(const AttnRows& r, int B) { return r.off ? r.T : (long long)B * r.T; }
+
+// The first query of a sequence that sees key j
+__device__ __forceinline__ int first_query(const AttnArgs& a, int seq, int j, int nq, int nk) {
+  if (!a.causal || (a.prefix != nullptr && j < a.prefix[seq])) return 0;
+  return max(0, j + nq - nk);
+}
+
+// A thread's columns [c0, c0 + 16) of an accumulator, times w, to a row of the result; zeros where the row has no terms
+__device__ __forceinline__ void store_acc(uint32_t tm, int from, int to, int D, bool mine, bool some, float w, __nv_bfloat16* row) {
+  for (int c0 = from; c0 < to; c0 += 16) {
+    float o[16];
+    tmem_ld16_nowait(tm + c0, reinterpret_cast<uint32_t*>(o));
+    tmem_ld_wait();
+    if (mine) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[e] = some ? o[e] : 0.f;
+      *reinterpret_cast<uint4*>(row + c0) = pack8(o, w);
+      if (c0 + 8 < D) *reinterpret_cast<uint4*>(row + c0 + 8) = pack8(o + 8, w);
+    }
+    __syncwarp();
+  }
+}
+
+// kKeys: the block owns keys
+template <int kD, bool kKeys, bool kCap, bool kBias>
+__device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a, BwdShared<kD>& sh, uint8_t* smem_raw, int tile_at, int head) {
+  using Shape = BwdShape<kD>;
+  constexpr int kStages = Shape::stages, kSlots = Shape::slots;
+  volatile int* s_abort = &sh.abort;
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  const Tile tile = tile_of(kKeys ? a.rk : a.rq, a.B, kX, tile_at);
+  if (!tile.any) return;
+  const int tile_rows = min(kX, tile.rows.n - tile.first);
+  Span qs{tile.rows.b, tile.rows.first, 0}, ks = qs;
+  if (tile.seq >= 0) {
+    qs = span_of(a.rq, tile.seq);
+    ks = span_of(a.rk, tile.seq);
+  }
+  const Span& xs = kKeys ? ks : qs;
+  const Span& ys = kKeys ? qs : ks;
+  const int last = min(tile.first + kX, xs.n) - 1;            // row of the sequence
+  const int R = a.H / a.G;
+  // rows of Y that rows of X meet: [lo, hi), and where all of them meet all: [all_lo, all_hi)
+  int lo = 0, hi = 0, all_lo = 0, all_hi = 0;
+  if (tile.first < xs.n) {
+    if (kKeys) {
+      lo = first_query(a, tile.seq, tile.first, qs.n, ks.n) & ~(kY - 1);
+      hi = qs.n;
+      all_lo = first_query(a, tile.seq, last, qs.n, ks.n);
+      all_hi = qs.n;
+    } else {
+      hi = keys_seen(a, tile.seq, last, qs.n, ks.n);
+      all_hi = keys_seen(a, tile.seq, tile.first, qs.n, ks.n);
+    }
+  }
+  const int per_head = hi > lo ? (hi - lo + kY - 1) / kY : 0;
+  const int steps = per_head * (kKeys ? R : 1);
+  if (steps == 0) {
+    const int per = a.D / 8;
+    for (int i = threadIdx.x; i < tile_rows * per; i += Shape::threads) {
+      const long long row = tile.rows.first + tile.first + i / per;
+      *reinterpret_cast<uint4*>(at_out(kKeys ? a.gk : a.gq, tile.rows.b, row, head) + i % per * 8) = make_uint4(0, 0, 0, 0);
+      if (kKeys) *reinterpret_cast<uint4*>(at_out(a.gv, tile.rows.b, row, head) + i % per * 8) = make_uint4(0, 0, 0, 0);
+    }
+    return;
+  }
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* ring_gen = smem_raw + (base - smem_u32(smem_raw)) + 2 * Shape::x_bytes;
+  const uint32_t ring = base + 2 * Shape::x_bytes;
+  if (threadIdx.x == 0) {
+    *s_abort = 0;
+    mbar_init(smem_u32(&sh.x), 1);
+    for (int s = 0; s < kSlots; ++s) { mbar_init(smem_u32(&sh.full[s]), 1); mbar_init(smem_u32(&sh.empty[s]), 1); }
+    for (int s = 0; s < kStages; ++s) { mbar_init(smem_u32(&sh.score[s]), 1); mbar_init(smem_u32(&sh.weight[s]), kX); }
+    mbar_init(smem_u32(&sh.acc), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 0) tmem_alloc<Shape::tmem_cols>(&sh.tmem);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+  const int d16 = round16(a.D);
+  auto y_first = [&](int it) { return lo + (kKeys ? it % per_head : it) * kY; };
+  auto y_head = [&](int it) { return kKeys ? head * R + it / per_head : head / R; };
+
+  if (warp == Shape::soft_warps) {
+    // ---- loads
+    const bool lead = elect_one();
+    if (lead) {
+      const uint32_t bar = smem_u32(&sh.x);
+      mbar_expect_tx(bar, 2 * Shape::x_bytes);
+      for (int o = 0; o < 2; ++o)
+        for (int c = 0; c < Shape::chunks; ++c)
+          for (int r = 0; r < kX; r += kY)
+            tma_load_4d(base + o * Shape::x_bytes + c * (kX * 128) + r * 128, kKeys ? (o ? &maps.v : &maps.k) : (o ? &maps.go : &maps.q), 64 * c,
+                        xs.first + tile.first + r, head, xs.b, bar);
+    }
+    __syncwarp();
+    for (int it = 0; it < steps; ++it) {
+      const int s = it % kSlots;
+      if (it >= kSlots && !mbar_wait_warp(smem_u32(&sh.empty[s]), ((it / kSlots) & 1) ^ 1, s_abort)) { *s_abort = 1; break; }
+      if (lead) {
+        const uint32_t bar = smem_u32(&sh.full[s]), to = ring + s * 2 * Shape::y_bytes;
+        mbar_expect_tx(bar, 2 * Shape::y_bytes);
+        for (int o = 0; o < 2; ++o)
+          for (int c = 0; c < Shape::chunks; ++c)
+            tma_load_4d(to + o * Shape::y_bytes + c * (kY * 128), kKeys ? (o ? &maps.go : &maps.q) : (o ? &maps.v : &maps.k), 64 * c,
+                        ys.first + y_first(it), y_head(it), ys.b, bar);
+      }
+      __syncwarp();
+    }
+  } else if (warp == Shape::soft_warps + 1) {
+    // ---- products
+    const bool lead = elect_one();
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    bool ok = mbar_wait_warp(smem_u32(&sh.x), 0, s_abort);
+    auto scores = [&](int it) {
+      const int s = it % kSlots;
+      ok = ok && mbar_wait_warp(smem_u32(&sh.full[s]), (it / kSlots) & 1, s_abort);
+      if (!ok) return;
+      tc_fence_after();
+      const int end = ys.n - y_first(it);
+      if (end < kY && (end & 15)) {      // rows behind the sequence's end
+        zero_rows<kY>(ring_gen + s * 2 * Shape::y_bytes, Shape::chunks, end, round16(end), lane);
+        zero_rows<kY>(ring_gen + s * 2 * Shape::y_bytes + Shape::y_bytes, Shape::chunks, end, round16(end), lane);
+      }
+      const uint32_t y1 = ring + s * 2 * Shape::y_bytes, y2 = y1 + Shape::y_bytes;
+      const uint32_t to = tm + (it % kStages) * 2 * kY;
+      const uint32_t id = idesc_of(round16(min(kY, hi - y_first(it))), false);
+      if (lead) {
+        for (int k = 0; k < d16 / 16; ++k) umma_f16(to, desc_k<kX>(base, k), desc_k<kY>(y1, k), id, k > 0);
+        for (int k = 0; k < d16 / 16; ++k) umma_f16(to + kY, desc_k<kX>(base + Shape::x_bytes, k), desc_k<kY>(y2, k), id, k > 0);
+        umma_commit(smem_u32(&sh.score[it % kStages]));
+      }
+      __syncwarp();
+    };
+    for (int it = 0; it < kStages && it < steps; ++it) scores(it);
+    for (int it = 0; it < steps && ok; ++it) {
+      const int st = it % kStages, s = it % kSlots;
+      ok = mbar_wait_warp(smem_u32(&sh.weight[st]), (it / kStages) & 1, s_abort);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t y1 = ring + s * 2 * Shape::y_bytes, y2 = y1 + Shape::y_bytes;
+      const uint32_t from = tm + st * 2 * kY;
+      const int n = round16(min(kY, hi - y_first(it))) / 16;
+      const uint32_t id = idesc_of(d16, true);
+      if (lead) {
+        for (int k = 0; k < n; ++k) umma_f16_ts(tm + Shape::acc_col, from + kY + k * 8, desc_mn<kY>(y1, k), id, it > 0 || k > 0);
+        if (kKeys)
+          for (int k = 0; k < n; ++k) umma_f16_ts(tm + Shape::acc_col + kD, from + k * 8, desc_mn<kY>(y2, k), id, it > 0 || k > 0);
+        umma_commit(it + 1 == steps ? smem_u32(&sh.acc) : smem_u32(&sh.empty[s]));
+      }
+      __syncwarp();
+      if (it + kStages < steps) scores(it + kStages);
+    }
+    if (!ok) *s_abort = 1;
   } else {
-    int lo = 0, hi = a.B;       // the first offset beyond the row
-    while (lo < hi) {
-      const int mid = (lo + hi) / 2;
-      if (r.off[mid] <= row) lo = mid + 1; else hi = mid;
+    // ---- p and ds: a row of X per thread, stages in turn
+    const int st = warp >> 2, r = (warp & 3) * 32 + lane;
+    const int x = tile.first + r;
+    const uint32_t tm_row = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t tm = tm_row + st * 2 * kY;
+    const float c = kCap ? 2.f * kLog2e * a.scale / a.cap : a.scale * kLog2e;
+    const float cap2 = a.cap * kLog2e;
+    const long long q_rows = flat_rows(a.rq, a.B), q_flat = (a.rq.off ? 0 : (long long)qs.b * a.rq.T) + qs.first;
+    // keys: the queries [meet, qs.n) see this one; queries: keys [0, meet) are seen
+    const int meet = x < xs.n ? (kKeys ? first_query(a, tile.seq, x, qs.n, ks.n) : keys_seen(a, tile.seq, x, qs.n, ks.n)) : (kKeys ? lo : hi);
+    const int shift = ks.n - qs.n;
+    float lse = 0.f, delta = 0.f, next = 0.f;
+    auto fetch = [&](int it) {           // lse (threads 0 to 63) or delta of a query of step `it`
+      const int i = y_first(it) + (r & (kY - 1));
+      return i < qs.n ? (r < kY ? a.lse : a.delta)[y_head(it) * q_rows + q_flat + i] : 0.f;
+    };
+    if (kKeys) {
+      if (st < steps) next = fetch(st);
+    } else if (x < xs.n) {
+      lse = a.lse[head * q_rows + q_flat + x];
+      delta = a.delta[head * q_rows + q_flat + x];
     }
-    p.seq = lo >= 1 && lo <= a.B && row < r.off[a.B] ? lo - 1 : -1;
-    p.b = 0; p.t = (int)row;
-    if (p.seq >= 0) p.i = (int)row - span_of(r, p.seq).first;
-  }
-  if (p.seq >= 0) {
-    p.queries = span_of(a.rq, p.seq);
-    p.keys = span_of(a.rk, p.seq);
-    p.nq = p.queries.n; p.nk = p.keys.n;
-    if (p.i >= span_of(r, p.seq).n) p.seq = -1;
-  }
-  return p;
-}
-
-__global__ void __launch_bounds__(32 * kWarps) attention_dq_kernel(const AttnArgs a, long long rows) {
-  pdl_sync();
-  __shared__ float s_q[kWarps][128], s_g[kWarps][128];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h = blockIdx.y;
-  const long long row = (long long)blockIdx.x * kWarps + warp;
-  if (row >= rows) return;
-  const Place p = place_of(a, a.rq, row);
-  float acc[kCols] = {};
-  if (p.seq >= 0) {
-    const int g = h / (a.H / a.G), lim = keys_seen(a, p.seq, p.i, p.nq, p.nk);
-    const float slope2 = a.slopes ? a.slopes[h] * kLog2e : 0.f;
-    load_row(at(a.q, p.b, p.t, h), s_q[warp], a.D, lane);
-    load_row(at(a.go, p.b, p.t, h), s_g[warp], a.D, lane);
-    __syncwarp();
-    float delta = 0.f;
-    for (int d = lane; d < a.D; d += 32) delta += s_g[warp][d] * __bfloat162float(at(a.o, p.b, p.t, h)[d]);
-    delta = warp_sum(delta);
-    if (lane == 0) a.delta[h * rows + row] = delta;
-    const float lse = a.lse[h * rows + row];
-    for (int j0 = 0; j0 < lim; j0 += 32) {
-      const int j = j0 + lane;
-      float ds = 0.f, th = 0.f;
-      if (j < lim) {
-        const float s = score_of(a, dot(at(a.k, p.keys.b, p.keys.first + j, g), s_q[warp], a.D), slope2, p.i + p.nk - p.nq - j, th);
-        const float dp = dot(at(a.v, p.keys.b, p.keys.first + j, g), s_g[warp], a.D);
-        ds = exp2f(s - lse) * (dp - delta) * (1.f - th * th) * a.scale;
+    bool ok = true;
+    for (int it = st; it < steps; it += kStages) {
+      const int y0 = y_first(it);
+      float* vec = sh.vec[st][(it / kStages) & 1];
+      const float slope2 = kBias ? a.slopes[kKeys ? y_head(it) : head] * kLog2e : 0.f;
+      if (kKeys) {
+        vec[r] = next;
+        if (it + kStages < steps) next = fetch(it + kStages);
+        asm volatile("bar.sync %0, 128;" ::"r"(st + 1) : "memory");
       }
-      const int n = min(32, lim - j0);
-      for (int k = 0; k < n; ++k) add_row(at(a.k, p.keys.b, p.keys.first + j0 + k, g), __shfl_sync(0xffffffffu, ds, k), acc, a.D, lane);
+      ok = ok && mbar_wait_warp(smem_u32(&sh.score[st]), (it / kStages) & 1, s_abort);
+      if (!ok) {         // the other warps of the stage still count on this one at its barrier
+        *s_abort = 1;
+        continue;
+      }
+      tc_fence_after();
+      const int wide = min(kY, hi - y0);
+      const bool masked = kKeys ? y0 < all_lo || y0 + kY > all_hi : y0 + kY > all_hi;
+#pragma unroll
+      for (int c0 = 0; c0 < kY; c0 += 32) {
+        if (c0 >= wide) continue;
+        float s[32], d[32];
+        tmem_ld32_nowait(tm + c0, reinterpret_cast<uint32_t*>(s));
+        tmem_ld32_nowait(tm + kY + c0, reinterpret_cast<uint32_t*>(d));
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          float ls[4], de[4];
+          if (kKeys) {
+            *reinterpret_cast<float4*>(ls) = *reinterpret_cast<const float4*>(vec + c0 + e);
+            *reinterpret_cast<float4*>(de) = *reinterpret_cast<const float4*>(vec + kY + c0 + e);
+          }
+#pragma unroll
+          for (int f = 0; f < 4; ++f) {
+            const int y = y0 + c0 + e + f;
+            const float lg = kKeys ? ls[f] : lse, dl = kKeys ? de[f] : delta;
+            float arg, slope = 1.f;
+            if (kCap) {
+              const float t = __fdividef(1.f, 1.f + ex2(s[e + f] * c));       // tanh = 1 - 2 t
+              arg = cap2 - 2.f * cap2 * t - lg;
+              slope = 4.f * t * (1.f - t);
+            } else {
+              arg = fmaf(s[e + f], c, -lg);
+            }
+            if (kBias) arg -= slope2 * fabsf((float)(kKeys ? y + shift - x : x + shift - y));
+            float p = ex2(arg);
+            float ds = p * (d[e + f] - dl);
+            if (kCap) ds *= slope;
+            if (masked && !(kKeys ? y >= meet && y < qs.n : y < meet)) p = ds = 0.f;
+            s[e + f] = p;
+            d[e + f] = ds;
+          }
+        }
+        uint32_t w[16];
+        if (kKeys) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) w[e] = pack_bf16(s[2 * e], s[2 * e + 1]);
+          tmem_st16(tm + c0 / 2, w);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) w[e] = pack_bf16(d[2 * e], d[2 * e + 1]);
+        tmem_st16(tm + kY + c0 / 2, w);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(smem_u32(&sh.weight[st]));
     }
-  }
-  store_row(at_out(a.gq, p.b, p.t, h), acc, 1.f, a.D, lane);
-}
-
-__global__ void __launch_bounds__(32 * kWarps) attention_dkv_kernel(const AttnArgs a, long long rows, long long q_rows) {
-  pdl_sync();
-  __shared__ float s_k[kWarps][128], s_v[kWarps][128];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = blockIdx.y;
-  const long long row = (long long)blockIdx.x * kWarps + warp;
-  if (row >= rows) return;
-  const Place p = place_of(a, a.rk, row);
-  float dk[kCols] = {}, dv[kCols] = {};
-  if (p.seq >= 0) {
-    load_row(at(a.k, p.b, p.t, g), s_k[warp], a.D, lane);
-    load_row(at(a.v, p.b, p.t, g), s_v[warp], a.D, lane);
-    __syncwarp();
-    const long long flat = (a.rq.off ? 0 : (long long)p.queries.b * a.rq.T) + p.queries.first;
-    for (int h = g * (a.H / a.G); h < (g + 1) * (a.H / a.G); ++h) {
-      const float slope2 = a.slopes ? a.slopes[h] * kLog2e : 0.f;
-      for (int i0 = 0; i0 < p.nq; i0 += 32) {
-        const int i = i0 + lane;
-        float w = 0.f, ds = 0.f, th = 0.f;
-        if (i < p.nq && p.i < keys_seen(a, p.seq, i, p.nq, p.nk)) {
-          const float s = score_of(a, dot(at(a.q, p.queries.b, p.queries.first + i, h), s_k[warp], a.D), slope2, i + p.nk - p.nq - p.i, th);
-          w = exp2f(s - a.lse[h * q_rows + flat + i]);
-          ds = w * (dot(at(a.go, p.queries.b, p.queries.first + i, h), s_v[warp], a.D) - a.delta[h * q_rows + flat + i]) * (1.f - th * th) * a.scale;
-        }
-        const int n = min(32, p.nq - i0);
-        for (int k = 0; k < n; ++k) {
-          const float wk = __shfl_sync(0xffffffffu, w, k), dk_w = __shfl_sync(0xffffffffu, ds, k);
-          if (wk == 0.f && dk_w == 0.f) continue;
-          add_row(at(a.go, p.queries.b, p.queries.first + i0 + k, h), wk, dv, a.D, lane);
-          add_row(at(a.q, p.queries.b, p.queries.first + i0 + k, h), dk_w, dk, a.D, lane);
-        }
+    if (ok) {
+      ok = mbar_wait_warp(smem_u32(&sh.acc), 0, s_abort);
+      if (!ok) *s_abort = 1;
+      tc_fence_after();
+    }
+    if (ok) {
+      const bool mine = r < tile_rows, some = x < xs.n;
+      const long long row = tile.rows.first + x;
+      const uint32_t acc = tm_row + Shape::acc_col;
+      if (kKeys) {
+        if (st == 0) store_acc(acc, 0, a.D, a.D, mine, some, a.scale, at_out(a.gk, tile.rows.b, row, head));
+        if (st == kStages - 1) store_acc(acc + kD, 0, a.D, a.D, mine, some, 1.f, at_out(a.gv, tile.rows.b, row, head));
+      } else {
+        const int half = kStages == 1 ? a.D : min(a.D, kD / 2);
+        store_acc(acc, st == 0 ? 0 : half, st == 0 ? half : a.D, a.D, mine, some, a.scale, at_out(a.gq, tile.rows.b, row, head));
       }
     }
   }
-  store_row(at_out(a.gk, p.b, p.t, g), dk, 1.f, a.D, lane);
-  store_row(at_out(a.gv, p.b, p.t, g), dv, 1.f, a.D, lane);
+
+  tc_fence_before();
+  __syncthreads();
+  if (*s_abort) {
+    if (threadIdx.x == 0) set_status(a.status, kMbarTimeout, kKeys ? 41 : 42, (int)blockIdx.x);
+    for (int i = 0; i < 2000; ++i) __nanosleep(1000);        // copies in flight land
+    __syncthreads();
+  }
+  if (warp == 0) tmem_dealloc<Shape::tmem_cols>(tmem);
 }
 
-long long rows_of(const AttnRows& r, int B) { return r.off ? r.T : (long long)B * r.T; }
-const char* told(cudaError_t e) {
-  if (e == cudaSuccess) e = cudaGetLastError();
-  return e == cudaSuccess ? nullptr : cudaGetErrorString(e);
+// The first key_tiles * G blocks own keys, the others queries.  Early keys are seen by the most queries and late queries see the most
+// keys: those go first.
+template <int kD, bool kCap, bool kBias>
+__global__ void __launch_bounds__(BwdShape<kD>::threads, kD == 128 ? 1 : 2)
+attention_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, const __grid_constant__ AttnArgs a, int key_tiles, int query_tiles) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ BwdShared<kD> sh;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int at = blockIdx.x;
+  if (at < key_tiles * a.G)
+    bwd_block<kD, true, kCap, kBias>(maps, a, sh, smem_raw, at / a.G, at % a.G);
+  else
+    bwd_block<kD, false, kCap, kBias>(maps, a, sh, smem_raw, query_tiles - 1 - (at - key_tiles * a.G) / a.H, (at - key_tiles * a.G) % a.H);
+}
+
+// delta[h][row] = sum over the columns of do o; `lanes` threads, a power of two, per row of a head
+__global__ void __launch_bounds__(256) attention_delta_kernel(const AttnArgs a, long long rows, int lanes) {
+  pdl_sync();
+  const long long at_row = ((long long)blockIdx.x * 256 + threadIdx.x) / lanes;
+  const int lane = threadIdx.x % lanes;
+  float v = 0.f;
+  const long long row = at_row / a.H;
+  const int h = (int)(at_row % a.H);
+  if (row < rows && lane * 8 < a.D) {
+    const int b = a.rq.off ? 0 : (int)(row / a.rq.T);
+    const long long t = a.rq.off ? row : row % a.rq.T;
+    const uint4 x = *reinterpret_cast<const uint4*>(at(a.go, b, t, h) + lane * 8), y = *reinterpret_cast<const uint4*>(at(a.o, b, t, h) + lane * 8);
+    const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      v += __uint_as_float(xw[i] << 16) * __uint_as_float(yw[i] << 16) + __uint_as_float(xw[i] & 0xffff0000u) * __uint_as_float(yw[i] & 0xffff0000u);
+  }
+  for (int o = lanes / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (row < rows && lane == 0) a.delta[h * rows + row] = v;
+}
+
+template <int kD, bool kCap, bool kBias>
+cudaError_t launch(const BwdMaps& maps, const AttnArgs& a, cudaStream_t st) {
+  auto* k = attention_bwd_tc_kernel<kD, kCap, kBias>;
+  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, BwdShape<kD>::smem);      // of the current device
+  if (e != cudaSuccess) return e;
+  const long long kt = tile_count(a.rk, a.B, kX), qt = tile_count(a.rq, a.B, kX);
+  if (kt * a.G + qt * a.H >= (1LL << 31)) return cudaErrorInvalidConfiguration;
+  return launch_pdl(k, dim3((unsigned)(kt * a.G + qt * a.H)), dim3(BwdShape<kD>::threads), BwdShape<kD>::smem, st, maps, a, (int)kt, (int)qt);
+}
+template <int kD>
+cudaError_t launch(const BwdMaps& maps, const AttnArgs& a, cudaStream_t st) {
+  if (a.cap > 0.f) return a.slopes ? launch<kD, true, true>(maps, a, st) : launch<kD, true, false>(maps, a, st);
+  return a.slopes ? launch<kD, false, true>(maps, a, st) : launch<kD, false, false>(maps, a, st);
 }
 
 }  // namespace
 
 const char* launch_attention_bwd(const AttnArgs& a, cudaStream_t st) {
-  const long long nq = rows_of(a.rq, a.B), nk = rows_of(a.rk, a.B);
-  if (const char* e = told(launch_pdl(attention_dq_kernel, dim3((unsigned)((nq + kWarps - 1) / kWarps), a.H), dim3(32 * kWarps), 0, st, a, nq)))
-    return e;
-  return told(launch_pdl(attention_dkv_kernel, dim3((unsigned)((nk + kWarps - 1) / kWarps), a.G), dim3(32 * kWarps), 0, st, a, nk, nq));
+  BwdMaps maps;
+  if (!operand_map(a.q, a.D, a.rq, a.B, a.H, kY, &maps.q) || !operand_map(a.k, a.D, a.rk, a.B, a.G, kY, &maps.k) ||
+      !operand_map(a.v, a.D, a.rk, a.B, a.G, kY, &maps.v) || !operand_map(a.go, a.D, a.rq, a.B, a.H, kY, &maps.go))
+    return "attention: cuTensorMapEncodeTiled failed";
+  const long long rows = a.rq.off ? a.rq.T : (long long)a.B * a.rq.T;
+  int lanes = 1;
+  while (lanes * 8 < a.D) lanes <<= 1;
+  cudaError_t e = launch_pdl(attention_delta_kernel, dim3((unsigned)((rows * a.H * lanes + 255) / 256)), dim3(256), 0, st, a, rows, lanes);
+  if (e == cudaSuccess) e = a.D > 64 ? launch<128>(maps, a, st) : launch<64>(maps, a, st);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  return e == cudaSuccess ? nullptr : cudaGetErrorString(e);
 }
 
 }  // namespace tn

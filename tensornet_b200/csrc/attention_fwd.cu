@@ -287,12 +287,14 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
           tmem_ld16_nowait(tm_o + c0, reinterpret_cast<uint32_t*>(o));
           tmem_ld_wait();
         }
-        if (!mine) continue;
-        const bool some = w != 0.f;         // (what a row without weights holds may be anything)
+        if (mine) {
+          const bool some = w != 0.f;         // (what a row without weights holds may be anything)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) o[e] = some ? o[e] : 0.f;
-        *reinterpret_cast<uint4*>(out + c0) = pack8(o, w);
-        if (c0 + 8 < a.D) *reinterpret_cast<uint4*>(out + c0 + 8) = pack8(o + 8, w);
+          for (int e = 0; e < 16; ++e) o[e] = some ? o[e] : 0.f;
+          *reinterpret_cast<uint4*>(out + c0) = pack8(o, w);
+          if (c0 + 8 < a.D) *reinterpret_cast<uint4*>(out + c0 + 8) = pack8(o + 8, w);
+        }
+        __syncwarp();
       }
       if (a.lse != nullptr && mine)
         a.lse[(long long)h * (a.rq.off ? a.rq.T : (long long)a.B * a.rq.T) + (a.rq.off ? 0 : (long long)tile.rows.b * a.rq.T) + row] =
@@ -344,6 +346,14 @@ namespace attn {
 bool operand_map(const AttnOperand& o, int D, const AttnRows& r, int B, int heads, int box_rows, CUtensorMap* out) {
   EncodeTiledFn enc = encode_fn();
   if (!enc) return false;
+  // A thread that has made no call of the runtime yet, as one of torch's graph, has no context for the driver's call.
+  thread_local int bound = -1;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  if (bound != dev) {
+    if (cudaSetDevice(dev) != cudaSuccess) return false;
+    bound = dev;
+  }
   const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)r.T, (cuuint64_t)heads, (cuuint64_t)(r.off ? 1 : B)};
   const cuuint64_t strides[3] = {(cuuint64_t)o.st * 2, (cuuint64_t)o.sh * 2, r.off ? (cuuint64_t)16 : (cuuint64_t)o.sb * 2};
   const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1}, step[4] = {1, 1, 1, 1};
