@@ -35,6 +35,10 @@ struct AttnArgs {
 };
 
 const char* launch_attention_fwd(const AttnArgs& a, cudaStream_t st);
+// Few queries, padded: whether launch_attention_few takes the call, and the fp32 values of workspace that it wants then.
+bool attention_few_takes(const AttnArgs& a);
+long long attention_few_floats(const AttnArgs& a);
+const char* launch_attention_few(const AttnArgs& a, float* work, cudaStream_t st);
 const char* launch_attention_bwd(const AttnArgs& a, cudaStream_t st);
 
 }  // namespace tn

@@ -181,7 +181,16 @@ struct Attention : torch::autograd::Function<Attention> {
         lse = at::empty({a.H, q.numel() / (a.H * a.D)}, q.options().dtype(at::kFloat));
         a.lse = lse.data_ptr<float>();
       }
-      told(tn::launch_attention_fwd(a, counted_stream()));
+      if (tn::attention_few_takes(a)) {
+        at::Tensor work;
+        if (const long long n = tn::attention_few_floats(a)) {
+          work = at::empty({n}, q.options().dtype(at::kFloat));
+          count_launches(1);
+        }
+        told(tn::launch_attention_few(a, work.defined() ? work.data_ptr<float>() : nullptr, counted_stream()));
+      } else {
+        told(tn::launch_attention_fwd(a, counted_stream()));
+      }
     }
     if (keep) {
       auto opt = [](const OptTensor& t) { return t ? *t : at::Tensor(); };
