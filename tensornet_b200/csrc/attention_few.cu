@@ -1,13 +1,16 @@
 // Attention of a few queries against many keys, forward: up to 16 rows, a query head's query each, that share a key head.
 //
-// What bounds it is reading keys and values once.  A warp takes 16 or 32 keys at a time with a softmax of its own and no shared
-// memory: products are mma.sync of 16 rows (at these rates far from what bounds it), and both operands come from memory in the
-// layout that the instruction wants.
+// What bounds it is reading keys and values once.  A warp takes 16 or 32 keys at a time with a softmax and a ring of its own: one
+// lane asks for tiles of keys and values by TMA, three steps ahead, so that a GPU's worth of warps has 28 MB on the way; products
+// are mma.sync of 16 rows (at these rates far from what bounds it).  Tiles lie in rows of 128 bytes, swizzled, and are read
+// 16 bytes at a time in the layout that the instruction wants, without conflicts:
 //   * scores: the contraction may go over the columns in any order that both sides share.  A lane of group g = lane / 4, t = lane % 4
-//     loads the 16 bytes of key g at column 8 t of 32: four words, the right operand of two products whose k are those columns.
-//   * values: lane (g, t) loads the 16 bytes of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9 at column 8 g of 64.  Words of two keys,
-//     interleaved by byte permutation, are the right operand of eight products; product i has columns 8 g + i.
-// Rows of 16 or 32 columns take pieces of 4 or 8 bytes in the same way.
+//     reads key spread(g) at column 8 t of 32: four words, the right operand of two products whose k are those columns.
+//   * values: lane (g, t) reads keys t, t + 4, t + 8 and t + 12, which is where spread() has put the keys of its weights, at column
+//     8 spread(g) of 64.  Words of two keys, interleaved by byte permutation, are the right operand of eight products; product i has
+//     columns 8 spread(g) + i.
+// spread() puts neighbouring groups four rows (or four pieces) apart, where the swizzle has the other half of the banks.
+// Rows of 16 or 32 columns take pieces of 4 or 8 bytes of values in the same way.
 // A sequence's keys are split over warps, blocks or both; what the blocks have of a row is brought to one reference and added by a
 // second kernel, in a fixed order.
 #include <cuda_bf16.h>
@@ -35,38 +38,64 @@ __device__ __forceinline__ void mma16(float* c, const uint32_t* a, uint32_t b0, 
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// kWords 32-bit words at p, or zeros
-template <int kWords>
-__device__ __forceinline__ void load_words(const __nv_bfloat16* p, bool there, uint32_t* w) {
+// kWords 32-bit words at p
+template <int kWords, typename P>
+__device__ __forceinline__ void load_words(const P* p, uint32_t* w) {
   if constexpr (kWords == 4) {
-    const uint4 v = there ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
     w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
   } else if constexpr (kWords == 2) {
-    const uint2 v = there ? __ldg(reinterpret_cast<const uint2*>(p)) : make_uint2(0, 0);
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
     w[0] = v.x; w[1] = v.y;
   } else {
-    w[0] = there ? __ldg(reinterpret_cast<const uint32_t*>(p)) : 0u;
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
   }
 }
+template <int kWords>
+__device__ __forceinline__ void store_words(__nv_bfloat16* p, const uint32_t* w) {
+  if constexpr (kWords == 4) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  else if constexpr (kWords == 2) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+  else *reinterpret_cast<uint32_t*>(p) = w[0];
+}
+__device__ __forceinline__ int spread(int g) { return (g & 1) * 4 + (g >> 1); }
 
 template <int kD>
 struct FewShape {
   static constexpr int keys = kD == 128 ? 16 : 32;                    // of a step
+  static constexpr int chunks = kD == 128 ? 2 : 1;                    // of 64 columns
+  static constexpr int chunk_bytes = keys * 128;
+  static constexpr int stage_bytes = 2 * chunks * chunk_bytes;        // keys, then values: 8 KiB
+  static constexpr int stages = 3;
+  static constexpr int smem = kWarps * stages * stage_bytes + 1024;
   static constexpr int k_words = kD == 16 ? 2 : 4, k_pieces = kD == 16 ? 1 : kD / 32;
   static constexpr int v_words = kD >= 64 ? 4 : kD / 16, v_pieces = kD >= 64 ? kD / 64 : 1;
   static constexpr int v_cols = 2 * v_words;                          // columns of a piece
 };
 
-// part: [unit][split][16][kD] sums and [unit][split][2][16] references and sums of weights, where there are several splits
+struct FewMaps {
+  CUtensorMap k, v;      // boxes of a step's keys
+};
+
+// part: [unit][split][16][kD] sums and [unit][split][16][2] references and sums of weights, where there are several splits
 template <int kD>
-__global__ void __launch_bounds__(32 * kWarps) attention_few_kernel(const __grid_constant__ AttnArgs a, const FewPlan plan, float* __restrict__ part,
-                                                                    float* __restrict__ part_ml) {
+__global__ void __launch_bounds__(32 * kWarps, 2)
+attention_few_kernel(const __grid_constant__ FewMaps maps, const __grid_constant__ AttnArgs a, const FewPlan plan, float* __restrict__ part,
+                     float* __restrict__ part_ml) {
   using S = FewShape<kD>;
   constexpr int kTilesN = S::keys / 8;
-  pdl_sync();
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t s_full[kWarps][S::stages];
   __shared__ float s_m[kWarps][kRowsM], s_l[kWarps][kRowsM];
-  __shared__ __align__(16) float s_o[kWarps][kRowsM][kD];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  __shared__ int s_abort_i;
+  volatile int* s_abort = &s_abort_i;
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  if (lane == 0) {
+    for (int s = 0; s < S::stages; ++s) mbar_init(smem_u32(&s_full[warp][s]), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    s_abort_i = 0;
+  }
+  __syncthreads();
+  pdl_sync();
   const int R = a.H / a.G, rows = a.rq.T * R;
   const long long units = (long long)a.B * a.G * plan.row_blocks;
   const bool alone = plan.per_unit == 1;
@@ -75,92 +104,100 @@ __global__ void __launch_bounds__(32 * kWarps) attention_few_kernel(const __grid
   const int rb = (int)(unit % plan.row_blocks), kh = (int)(unit / plan.row_blocks % a.G), seq = (int)(unit / plan.row_blocks / a.G);
   const Span qs = span_of(a.rq, seq), ks = span_of(a.rk, seq);
   const int row0 = rb * kRowsM;
+  // keys that the unit's last query sees; keys_seen grows with the query
+  const int last = min((min(rows, row0 + kRowsM) - 1) / R, qs.n - 1);
+  const int vis = row0 / R <= last ? keys_seen(a, seq, last, qs.n, ks.n) : 0;
+  const int from = blockIdx.y * plan.chunk, to = min(vis, from + plan.chunk);
+  const bool whole = vis <= plan.chunk;              // the first split has all there is to the unit's rows
+  if (blockIdx.y > 0 && from >= to) return;          // the second kernel knows as much
+
+  const uint32_t ring = ((smem_u32(smem_raw) + 1023u) & ~1023u) + warp * S::stages * S::stage_bytes;
+  const uint8_t* ring_gen = smem_raw + (ring - smem_u32(smem_raw));
+  const int stride = S::keys * plan.per_unit;
+  const int j_first = from + (alone ? 0 : warp * S::keys);
+  const int steps = j_first < to ? (to - j_first + stride - 1) / stride : 0;
+  const bool lead = elect_one();
+  auto ask = [&](int n) {
+    const uint32_t bar = smem_u32(&s_full[warp][n % S::stages]), dst = ring + (n % S::stages) * S::stage_bytes;
+    const int row = ks.first + j_first + n * stride;
+    if (lead) {
+      mbar_expect_tx(bar, S::stage_bytes);
+#pragma unroll
+      for (int c = 0; c < S::chunks; ++c) {
+        tma_load_4d(dst + c * S::chunk_bytes, &maps.k, 64 * c, row, kh, ks.b, bar);
+        tma_load_4d(dst + (S::chunks + c) * S::chunk_bytes, &maps.v, 64 * c, row, kh, ks.b, bar);
+      }
+    }
+    __syncwarp();
+  };
+  for (int n = 0; n < S::stages && n < steps; ++n) ask(n);
+
   // row r of the unit: query (row0 + r) / R, query head kh * R + (row0 + r) % R
-  int lim[2], place[2];
+  int lim[2], place[2], least = vis;
   float slope2[2];
-  const __nv_bfloat16* q_at[2];
+  uint32_t q[S::k_pieces * S::k_words][2];      // words of rows g and g + 8
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     const int r = row0 + g + 8 * e, i = r / R, h = kh * R + r % R;
     const bool there = r < rows && i < qs.n;
     lim[e] = there ? keys_seen(a, seq, i, qs.n, ks.n) : 0;
+    if (there) least = min(least, lim[e]);
     place[e] = i + ks.n - qs.n;
     slope2[e] = there && a.slopes ? a.slopes[h] * kLog2e : 0.f;
-    q_at[e] = there ? at(a.q, qs.b, i, h) : nullptr;
-  }
-  int vis = max(lim[0], lim[1]);
-  for (int o = 16; o > 0; o >>= 1) vis = max(vis, __shfl_xor_sync(0xffffffffu, vis, o));
-  const int from = blockIdx.y * plan.chunk, to = min(vis, from + plan.chunk);
-
-  uint32_t q[S::k_pieces * S::k_words][2];      // words of rows g and g + 8
 #pragma unroll
-  for (int p = 0; p < S::k_pieces; ++p)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
+    for (int p = 0; p < S::k_pieces; ++p) {
       const int d = (p * 4 + t) * 2 * S::k_words;
-      uint32_t w[S::k_words];
-      load_words<S::k_words>(q_at[e] + d, q_at[e] != nullptr && d < a.D, w);
+      uint32_t w[S::k_words] = {};
+      if (there && d < a.D) load_words<S::k_words>(at(a.q, qs.b, i, h) + d, w);
 #pragma unroll
-      for (int i = 0; i < S::k_words; ++i) q[p * S::k_words + i][e] = w[i];
+      for (int i2 = 0; i2 < S::k_words; ++i2) q[p * S::k_words + i2][e] = w[i2];
     }
-
-  uint32_t kw[kTilesN][S::k_pieces * S::k_words];
-  uint32_t vw[S::keys / 16][4][S::v_pieces * S::v_words];
-  const __nv_bfloat16* k_base = at(a.k, ks.b, ks.first, kh);
-  const __nv_bfloat16* v_base = at(a.v, ks.b, ks.first, kh);
-  auto load_k = [&](int j0) {
-#pragma unroll
-    for (int n = 0; n < kTilesN; ++n)
-#pragma unroll
-      for (int p = 0; p < S::k_pieces; ++p) {
-        const int j = j0 + n * 8 + g, d = (p * 4 + t) * 2 * S::k_words;
-        load_words<S::k_words>(k_base + j * a.k.st + d, j < to && d < a.D, &kw[n][p * S::k_words]);
-      }
-  };
-  auto load_v = [&](int j0) {
-#pragma unroll
-    for (int n = 0; n < S::keys / 16; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-#pragma unroll
-        for (int p = 0; p < S::v_pieces; ++p) {
-          const int j = j0 + n * 16 + 2 * t + (e & 1) + (e >> 1) * 8, d = (p * 8 + g) * S::v_cols;
-          load_words<S::v_words>(v_base + j * a.v.st + d, j < to && d < a.D, &vw[n][e][p * S::v_words]);
-        }
-  };
+  }
+  for (int o = 16; o > 0; o >>= 1) least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
 
   float o[S::v_pieces * S::v_cols][4];
 #pragma unroll
   for (int i = 0; i < S::v_pieces * S::v_cols; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
   float m[2] = {kNone, kNone}, l[2] = {0.f, 0.f};
-  const int stride = S::keys * plan.per_unit;
-  const int j_first = from + (alone ? 0 : warp * S::keys);
   const float cs = a.cap > 0.f ? 2.f * kLog2e * a.scale / a.cap : a.scale * kLog2e;
   const float cap2 = a.cap * kLog2e;
-  if (j_first < to) { load_k(j_first); load_v(j_first); }
-  for (int j0 = j_first; j0 < to; j0 += stride) {
+  // where a lane reads: row spread(g) of eight for keys, rows t and t + 4 for values; the swizzle takes the row's number off the piece's
+  const int k_row = spread(g), v_piece = kD >= 64 ? spread(g) : g;
+  bool ok = true;
+  for (int n = 0; n < steps; ++n) {
+    const int j0 = j_first + n * stride;
+    if (!mbar_wait_warp(smem_u32(&s_full[warp][n % S::stages]), (n / S::stages) & 1, s_abort)) { *s_abort = 1; ok = false; break; }
+    const uint8_t* kt = ring_gen + (n % S::stages) * S::stage_bytes;
+    const uint8_t* vt = kt + S::chunks * S::chunk_bytes;
+    const bool masked = j0 + S::keys > min(least, to);
     float s[kTilesN][4];
 #pragma unroll
-    for (int n = 0; n < kTilesN; ++n) {
-      s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+    for (int c = 0; c < kTilesN; ++c) {
+      s[c][0] = s[c][1] = s[c][2] = s[c][3] = 0.f;
 #pragma unroll
-      for (int w = 0; w < S::k_pieces * S::k_words; w += 2) {
-        const uint32_t aw[4] = {q[w][0], q[w][1], q[w + 1][0], q[w + 1][1]};
-        mma16(s[n], aw, kw[n][w], kw[n][w + 1]);
+      for (int p = 0; p < S::k_pieces; ++p) {
+        uint32_t w[S::k_words];
+        const int byte = (p * 4 + t) * 4 * S::k_words;          // of the row
+        load_words<S::k_words>(kt + (byte >> 7) * S::chunk_bytes + (c * 8 + k_row) * 128 + ((byte & 127) ^ (k_row << 4)), w);
+#pragma unroll
+        for (int i = 0; i < S::k_words; i += 2) {
+          const uint32_t aw[4] = {q[p * S::k_words + i][0], q[p * S::k_words + i][1], q[p * S::k_words + i + 1][0], q[p * S::k_words + i + 1][1]};
+          mma16(s[c], aw, w[i], w[i + 1]);
+        }
       }
     }
-    if (j0 + stride < to) load_k(j0 + stride);
+    // score e of product c: key j0 + 8 c + spread(2 t + (e & 1)) = j0 + 8 c + t + 4 (e & 1), row g + 8 (e >> 1)
     float top[2] = {kNone, kNone};
 #pragma unroll
-    for (int n = 0; n < kTilesN; ++n)
+    for (int c = 0; c < kTilesN; ++c)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int j = j0 + n * 8 + 2 * t + (e & 1), r = e >> 1;
-        float x = s[n][e] * cs;
+        const int j = j0 + c * 8 + t + 4 * (e & 1), r = e >> 1;
+        float x = s[c][e] * cs;
         if (a.cap > 0.f) x = cap2 - __fdividef(2.f * cap2, 1.f + ex2(x));
         if (a.slopes != nullptr) x -= slope2[r] * fabsf((float)(place[r] - j));
-        x = j < min(lim[r], to) ? x : kNone;
-        s[n][e] = x;
+        if (masked) x = j < min(lim[r], to) ? x : kNone;
+        s[c][e] = x;
         top[r] = fmaxf(top[r], x);
       }
 #pragma unroll
@@ -178,36 +215,55 @@ __global__ void __launch_bounds__(32 * kWarps) attention_few_kernel(const __grid
         for (int i = 0; i < S::v_pieces * S::v_cols; ++i) { o[i][2 * r] *= by; o[i][2 * r + 1] *= by; }
       }
     }
+    const float ref[2] = {m[0] == kNone ? 0.f : m[0], m[1] == kNone ? 0.f : m[1]};
 #pragma unroll
-    for (int n = 0; n < kTilesN; ++n)
+    for (int c = 0; c < kTilesN; ++c)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int r = e >> 1;
-        s[n][e] = ex2(s[n][e] - (m[r] == kNone ? 0.f : m[r]));
-        l[r] += s[n][e];
+        s[c][e] = ex2(s[c][e] - ref[e >> 1]);
+        l[e >> 1] += s[c][e];
       }
 #pragma unroll
-    for (int n = 0; n < S::keys / 16; ++n) {
-      const uint32_t p[4] = {pack_bf16(s[2 * n][0], s[2 * n][1]), pack_bf16(s[2 * n][2], s[2 * n][3]), pack_bf16(s[2 * n + 1][0], s[2 * n + 1][1]),
-                             pack_bf16(s[2 * n + 1][2], s[2 * n + 1][3])};
+    for (int c = 0; c < S::keys / 16; ++c) {
+      const uint32_t p[4] = {pack_bf16(s[2 * c][0], s[2 * c][1]), pack_bf16(s[2 * c][2], s[2 * c][3]), pack_bf16(s[2 * c + 1][0], s[2 * c + 1][1]),
+                             pack_bf16(s[2 * c + 1][2], s[2 * c + 1][3])};
 #pragma unroll
-      for (int i = 0; i < S::v_pieces * S::v_words; ++i) {
-        const uint32_t lo0 = __byte_perm(vw[n][0][i], vw[n][1][i], 0x5410), hi0 = __byte_perm(vw[n][0][i], vw[n][1][i], 0x7632);
-        const uint32_t lo1 = __byte_perm(vw[n][2][i], vw[n][3][i], 0x5410), hi1 = __byte_perm(vw[n][2][i], vw[n][3][i], 0x7632);
-        mma16(o[2 * i], p, lo0, lo1);
-        mma16(o[2 * i + 1], p, hi0, hi1);
+      for (int pc = 0; pc < S::v_pieces; ++pc) {
+        uint32_t w[4][S::v_words];
+        const int byte = v_piece * 4 * S::v_words;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int row = t + 4 * (e & 1);                      // of eight
+          load_words<S::v_words>(vt + pc * S::chunk_bytes + (c * 16 + (e >> 1) * 8 + row) * 128 + (byte ^ (row << 4)), w[e]);
+          if (masked && j0 + c * 16 + (e >> 1) * 8 + row >= to)      // what lies behind the sequence may be anything
+#pragma unroll
+            for (int i = 0; i < S::v_words; ++i) w[e][i] = 0u;
+        }
+#pragma unroll
+        for (int i = 0; i < S::v_words; ++i) {
+          mma16(o[pc * S::v_cols + 2 * i], p, __byte_perm(w[0][i], w[1][i], 0x5410), __byte_perm(w[2][i], w[3][i], 0x5410));
+          mma16(o[pc * S::v_cols + 2 * i + 1], p, __byte_perm(w[0][i], w[1][i], 0x7632), __byte_perm(w[2][i], w[3][i], 0x7632));
+        }
       }
     }
-    if (j0 + stride < to) load_v(j0 + stride);
+    __syncwarp();
+    if (n + S::stages < steps) ask(n + S::stages);
   }
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
     l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+    if (lim[r] <= 0) { l[r] = 0.f; m[r] = kNone; }
+  }
+  if (!ok) {
+    if (lane == 0) set_status(a.status, kMbarTimeout, 43, (int)blockIdx.x);
+    for (int i = 0; i < 2000; ++i) __nanosleep(1000);        // copies in flight land
   }
 
-  // Lane (g, t) has of row g + 8 r the columns (p 8 + 2 t + f) v_cols + i, f < 2, i < v_cols: value o[p v_cols + i][2 r + f].
+  // Lane (g, t) has of row g + 8 r the columns (8 p + piece(2 t + f)) v_cols + i, f < 2, i < v_cols: value o[p v_cols + i][2 r + f],
+  // where piece() is spread() as for the values read.
   const long long q_rows = (long long)a.B * a.rq.T;
+  auto column = [&](int p, int f) { return (p * 8 + (kD >= 64 ? t + 4 * f : 2 * t + f)) * S::v_cols; };
   if (alone) {
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
@@ -220,15 +276,13 @@ __global__ void __launch_bounds__(32 * kWarps) attention_few_kernel(const __grid
       for (int p = 0; p < S::v_pieces; ++p)
 #pragma unroll
         for (int f = 0; f < 2; ++f) {
-          const int d = (p * 8 + 2 * t + f) * S::v_cols;
+          const int d = column(p, f);
           if (d >= a.D) continue;
           uint32_t v[S::v_words];
 #pragma unroll
           for (int k = 0; k < S::v_words; ++k)
             v[k] = pack_bf16(o[p * S::v_cols + 2 * k][2 * r + f] * w, o[p * S::v_cols + 2 * k + 1][2 * r + f] * w);
-          if constexpr (S::v_words == 4) *reinterpret_cast<uint4*>(out + d) = make_uint4(v[0], v[1], v[2], v[3]);
-          else if constexpr (S::v_words == 2) *reinterpret_cast<uint2*>(out + d) = make_uint2(v[0], v[1]);
-          else *reinterpret_cast<uint32_t*>(out + d) = v[0];
+          store_words<S::v_words>(out + d, v);
         }
       if (a.lse != nullptr && t == 0) a.lse[h * q_rows + (long long)seq * a.rq.T + i] = l[r] > 0.f ? m[r] + log2f(l[r]) : CUDART_INF_F;
     }
@@ -237,7 +291,9 @@ __global__ void __launch_bounds__(32 * kWarps) attention_few_kernel(const __grid
   if (t == 0)
 #pragma unroll
     for (int r = 0; r < 2; ++r) { s_m[warp][g + 8 * r] = m[r]; s_l[warp][g + 8 * r] = l[r]; }
-  __syncthreads();
+  __syncthreads();              // and every warp is through with its ring
+  float* s_o = reinterpret_cast<float*>(smem_raw);                    // [warp][16][kD + 4]
+  constexpr int kPitch = kD + 4;
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     float all = kNone;
@@ -248,26 +304,24 @@ __global__ void __launch_bounds__(32 * kWarps) attention_few_kernel(const __grid
 #pragma unroll
       for (int f = 0; f < 2; ++f)
 #pragma unroll
-        for (int i = 0; i < S::v_cols; ++i) s_o[warp][g + 8 * r][(p * 8 + 2 * t + f) * S::v_cols + i] = o[p * S::v_cols + i][2 * r + f] * by;
+        for (int i = 0; i < S::v_cols; ++i)
+          s_o[(warp * kRowsM + g + 8 * r) * kPitch + column(p, f) + i] = by == 0.f ? 0.f : o[p * S::v_cols + i][2 * r + f] * by;
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < kRowsM * kD / 2; e += 32 * kWarps) {
+  for (int e = threadIdx.x; e < min(kRowsM, rows - row0) * (kD / 2); e += 32 * kWarps) {
     const int r = e / (kD / 2), d = e % (kD / 2) * 2, row = row0 + r;
-    if (row >= rows || d >= a.D) continue;
+    if (d >= a.D) continue;
     float all = kNone, sum = 0.f, x = 0.f, y = 0.f;
     for (int w = 0; w < kWarps; ++w) all = fmaxf(all, s_m[w][r]);
     for (int w = 0; w < kWarps; ++w) {
       sum += s_m[w][r] == kNone ? 0.f : s_l[w][r] * ex2(s_m[w][r] - all);
-      x += s_o[w][r][d];
-      y += s_o[w][r][d + 1];
+      x += s_o[(w * kRowsM + r) * kPitch + d];
+      y += s_o[(w * kRowsM + r) * kPitch + d + 1];
     }
-    if (plan.splits > 1) {
+    if (!whole) {
       const long long at_part = (unit * plan.splits + blockIdx.y) * kRowsM + r;
       *reinterpret_cast<float2*>(part + at_part * kD + d) = make_float2(x, y);
-      if (d == 0) {
-        part_ml[2 * at_part] = all;
-        part_ml[2 * at_part + 1] = sum;
-      }
+      if (d == 0) *reinterpret_cast<float2*>(part_ml + 2 * at_part) = make_float2(all, sum);
       continue;
     }
     const int i = row / R, h = kh * R + row % R;
@@ -277,33 +331,53 @@ __global__ void __launch_bounds__(32 * kWarps) attention_few_kernel(const __grid
   }
 }
 
-// Splits of one row, in order.  A block of kD / 2 threads per row.
+// Adds a row's splits where the first had not all of it: a block per row, the threads of a column pair take splits in turn and their
+// sums are added in order.
+constexpr int kJoin = 256;
 template <int kD>
-__global__ void __launch_bounds__(kD / 2) attention_few_join_kernel(const __grid_constant__ AttnArgs a, const FewPlan plan, const float* __restrict__ part,
-                                                                    const float* __restrict__ part_ml) {
+__global__ void __launch_bounds__(kJoin) attention_few_join_kernel(const __grid_constant__ AttnArgs a, const FewPlan plan,
+                                                                   const float* __restrict__ part, const float* __restrict__ part_ml) {
   pdl_sync();
+  constexpr int kPairs = kD / 2, kTurns = kJoin / kPairs;
+  __shared__ float s_x[kTurns][kPairs], s_y[kTurns][kPairs], s_sum[kTurns];
   const int R = a.H / a.G, rows = a.rq.T * R;
-  const long long unit = blockIdx.x / kRowsM;
-  const int r = blockIdx.x % kRowsM, row = (int)(unit % plan.row_blocks) * kRowsM + r, d = threadIdx.x * 2;
-  if (row >= rows || d >= a.D) return;
+  const int r = blockIdx.y, row0 = (int)(blockIdx.x % plan.row_blocks) * kRowsM, row = row0 + r;
+  const long long unit = blockIdx.x;
+  if (row >= rows) return;
   const int kh = (int)(unit / plan.row_blocks % a.G), seq = (int)(unit / plan.row_blocks / a.G);
+  const Span qs = span_of(a.rq, seq), ks = span_of(a.rk, seq);
+  const int last = min((min(rows, row0 + kRowsM) - 1) / R, qs.n - 1);
+  const int vis = row0 / R <= last ? keys_seen(a, seq, last, qs.n, ks.n) : 0;
+  if (vis <= plan.chunk) return;
+  const int n = (vis + plan.chunk - 1) / plan.chunk;
+  const int pair = threadIdx.x % kPairs, turn = threadIdx.x / kPairs;
   const long long first = unit * plan.splits * kRowsM + r;
   float all = kNone, sum = 0.f, x = 0.f, y = 0.f;
-  for (int s = 0; s < plan.splits; ++s) all = fmaxf(all, part_ml[2 * (first + (long long)s * kRowsM)]);
-  for (int s = 0; s < plan.splits; ++s) {
+  for (int s = 0; s < n; ++s) all = fmaxf(all, part_ml[2 * (first + (long long)s * kRowsM)]);
+  for (int s = turn; s < n; s += kTurns) {
     const long long at_part = first + (long long)s * kRowsM;
-    const float m = part_ml[2 * at_part];
-    const float by = m == kNone ? 0.f : ex2(m - all);
-    if (by == 0.f) continue;
-    const float2 v = *reinterpret_cast<const float2*>(part + at_part * kD + d);
-    sum += part_ml[2 * at_part + 1] * by;
+    const float2 ml = *reinterpret_cast<const float2*>(part_ml + 2 * at_part);
+    const float by = ml.x == kNone ? 0.f : ex2(ml.x - all);
+    const float2 v = pair * 2 < a.D ? *reinterpret_cast<const float2*>(part + at_part * kD + pair * 2) : make_float2(0.f, 0.f);
+    sum += ml.y * by;
     x += v.x * by;
     y += v.y * by;
   }
+  s_x[turn][pair] = x;
+  s_y[turn][pair] = y;
+  if (pair == 0) s_sum[turn] = sum;
+  __syncthreads();
+  if (turn != 0 || pair * 2 >= a.D) return;
+  for (int k = 1; k < kTurns; ++k) {
+    x += s_x[k][pair];
+    y += s_y[k][pair];
+  }
+  sum = 0.f;
+  for (int k = 0; k < kTurns; ++k) sum += s_sum[k];
   const int i = row / R, h = kh * R + row % R;
   const float w = sum > 0.f ? 1.f / sum : 0.f;
-  *reinterpret_cast<uint32_t*>(at_out(a.o, seq, i, h) + d) = pack_bf16(x * w, y * w);
-  if (a.lse != nullptr && d == 0) a.lse[h * ((long long)a.B * a.rq.T) + (long long)seq * a.rq.T + i] = sum > 0.f ? all + log2f(sum) : CUDART_INF_F;
+  *reinterpret_cast<uint32_t*>(at_out(a.o, seq, i, h) + pair * 2) = pack_bf16(x * w, y * w);
+  if (a.lse != nullptr && pair == 0) a.lse[h * ((long long)a.B * a.rq.T) + (long long)seq * a.rq.T + i] = sum > 0.f ? all + log2f(sum) : CUDART_INF_F;
 }
 
 int few_columns(const AttnArgs& a) { return a.D <= 16 ? 16 : a.D <= 32 ? 32 : a.D <= 64 ? 64 : 128; }
@@ -317,7 +391,7 @@ FewPlan plan_of(const AttnArgs& a) {
   p.splits = 1;
   p.chunk = keys;
   if (p.per_unit > 1) {
-    const long long want = (148 * 4 + units - 1) / units;           // blocks that fill the GPU
+    const long long want = (148 * 2 + units - 1) / units;           // blocks that fill the GPU
     const long long most = (keys + 255) / 256;
     long long s = want < most ? want : most;
     if (s < (keys + 1023) / 1024 && a.rk.len != nullptr) s = (keys + 1023) / 1024;      // lengths may be anything: long ones are shared
@@ -329,14 +403,21 @@ FewPlan plan_of(const AttnArgs& a) {
 }
 
 template <int kD>
-cudaError_t launch(const AttnArgs& a, const FewPlan& p, float* work, cudaStream_t st) {
+cudaError_t launch(const FewMaps& maps, const AttnArgs& a, const FewPlan& p, float* work, cudaStream_t st) {
+  using S = FewShape<kD>;
+  static_assert(kWarps * kRowsM * (kD + 4) * 4 <= S::smem, "the warps' results take the place of the rings");
+  auto* k = attention_few_kernel<kD>;
+  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::smem);      // of the current device
+  if (e != cudaSuccess) return e;
   const long long units = (long long)a.B * a.G * p.row_blocks;
   float* ml = work == nullptr ? nullptr : work + units * p.splits * kRowsM * kD;
   const long long blocks = p.per_unit == 1 ? (units + kWarps - 1) / kWarps : units;
-  if (units * kRowsM >= (1LL << 31)) return cudaErrorInvalidConfiguration;
-  cudaError_t e = launch_pdl(attention_few_kernel<kD>, dim3((unsigned)blocks, p.splits), dim3(32 * kWarps), 0, st, a, p, work, ml);
+  if (units >= (1LL << 31)) return cudaErrorInvalidConfiguration;
+  e = launch_pdl(k, dim3((unsigned)blocks, p.splits), dim3(32 * kWarps), S::smem, st, maps, a, p, work, ml);
   if (e != cudaSuccess || p.splits == 1) return e;
-  return launch_pdl(attention_few_join_kernel<kD>, dim3((unsigned)(units * kRowsM)), dim3(kD / 2), 0, st, a, p, (const float*)work, (const float*)ml);
+  const int rows = a.rq.T * (a.H / a.G);
+  return launch_pdl(attention_few_join_kernel<kD>, dim3((unsigned)units, rows < kRowsM ? rows : kRowsM), dim3(kJoin), 0, st, a, p, (const float*)work,
+                    (const float*)ml);
 }
 
 }  // namespace
@@ -350,8 +431,14 @@ long long attention_few_floats(const AttnArgs& a) {
 
 const char* launch_attention_few(const AttnArgs& a, float* work, cudaStream_t st) {
   const FewPlan p = plan_of(a);
-  const int D = few_columns(a);
-  cudaError_t e = D == 16 ? launch<16>(a, p, work, st) : D == 32 ? launch<32>(a, p, work, st) : D == 64 ? launch<64>(a, p, work, st) : launch<128>(a, p, work, st);
+  const int D = few_columns(a), keys = D == 128 ? FewShape<128>::keys : FewShape<64>::keys;
+  FewMaps maps;
+  if (!operand_map(a.k, a.D, a.rk, a.B, a.G, keys, &maps.k) || !operand_map(a.v, a.D, a.rk, a.B, a.G, keys, &maps.v))
+    return "attention: cuTensorMapEncodeTiled failed";
+  cudaError_t e = D == 16   ? launch<16>(maps, a, p, work, st)
+                  : D == 32 ? launch<32>(maps, a, p, work, st)
+                  : D == 64 ? launch<64>(maps, a, p, work, st)
+                            : launch<128>(maps, a, p, work, st);
   if (e == cudaSuccess) e = cudaGetLastError();
   return e == cudaSuccess ? nullptr : cudaGetErrorString(e);
 }
