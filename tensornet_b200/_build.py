@@ -42,7 +42,7 @@ CUDA_SOURCES = [
     "mlp_fused.cu", "gemm_2sm.cu", "gemm_splitk.cu",
     "dense_fused.cu",
     "elementwise.cu",
-    "layer_norm.cu", "attention_fwd.cu", "attention_bwd.cu", "attention_few.cu", "sequence_ops.cpp",
+    "layer_norm.cu", "attention_fwd.cu", "attention_bwd.cu", "attention_few.cu", "attention_short.cu", "sequence_ops.cpp",
     "head.cu",
     "stage.cu",
     "serving.cu",

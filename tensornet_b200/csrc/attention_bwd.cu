@@ -50,14 +50,6 @@ struct BwdShared {
   alignas(16) float vec[BwdShape<kD>::stages][2][2 * kY];      // lse and delta of a tile of queries
 };
 
-__device__ __forceinline__ long long flat_rows(const AttnRows& r, int B) { return r.off ? r.T : (long long)B * r.T; }
-
-// The first query of a sequence that sees key j
-__device__ __forceinline__ int first_query(const AttnArgs& a, int seq, int j, int nq, int nk) {
-  if (!a.causal || (a.prefix != nullptr && j < a.prefix[seq])) return 0;
-  return max(0, j + nq - nk);
-}
-
 // A thread's columns [c0, c0 + 16) of an accumulator, times w, to a row of the result; zeros where the row has no terms
 __device__ __forceinline__ void store_acc(uint32_t tm, int from, int to, int D, bool mine, bool some, float w, __nv_bfloat16* row) {
   for (int c0 = from; c0 < to; c0 += 16) {
@@ -382,14 +374,15 @@ cudaError_t launch(const BwdMaps& maps, const AttnArgs& a, cudaStream_t st) {
 }  // namespace
 
 const char* launch_attention_bwd(const AttnArgs& a, cudaStream_t st) {
-  BwdMaps maps;
-  if (!operand_map(a.q, a.D, a.rq, a.B, a.H, kY, &maps.q) || !operand_map(a.k, a.D, a.rk, a.B, a.G, kY, &maps.k) ||
-      !operand_map(a.v, a.D, a.rk, a.B, a.G, kY, &maps.v) || !operand_map(a.go, a.D, a.rq, a.B, a.H, kY, &maps.go))
-    return "attention: cuTensorMapEncodeTiled failed";
   const long long rows = a.rq.off ? a.rq.T : (long long)a.B * a.rq.T;
   int lanes = 1;
   while (lanes * 8 < a.D) lanes <<= 1;
   cudaError_t e = launch_pdl(attention_delta_kernel, dim3((unsigned)((rows * a.H * lanes + 255) / 256)), dim3(256), 0, st, a, rows, lanes);
+  if (e == cudaSuccess && attention_short_takes(a)) return launch_attention_short_bwd(a, st);
+  BwdMaps maps;
+  if (!operand_map(a.q, a.D, a.rq, a.B, a.H, kY, &maps.q) || !operand_map(a.k, a.D, a.rk, a.B, a.G, kY, &maps.k) ||
+      !operand_map(a.v, a.D, a.rk, a.B, a.G, kY, &maps.v) || !operand_map(a.go, a.D, a.rq, a.B, a.H, kY, &maps.go))
+    return "attention: cuTensorMapEncodeTiled failed";
   if (e == cudaSuccess) e = a.D > 64 ? launch<128>(maps, a, st) : launch<64>(maps, a, st);
   if (e == cudaSuccess) e = cudaGetLastError();
   return e == cudaSuccess ? nullptr : cudaGetErrorString(e);

@@ -14,7 +14,7 @@
 // A sequence's keys are split over warps, blocks or both; what the blocks have of a row is brought to one reference and added by a
 // second kernel, in a fixed order.
 #include <cuda_bf16.h>
-#include "attention_tc.cuh"
+#include "attention_mma.cuh"
 
 namespace tn {
 
@@ -32,44 +32,16 @@ struct FewPlan {
   int per_unit;        // warps that share a split: 1 or kWarps
 };
 
-__device__ __forceinline__ void mma16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// kWords 32-bit words at p
-template <int kWords, typename P>
-__device__ __forceinline__ void load_words(const P* p, uint32_t* w) {
-  if constexpr (kWords == 4) {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
-    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-  } else if constexpr (kWords == 2) {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
-    w[0] = v.x; w[1] = v.y;
-  } else {
-    w[0] = *reinterpret_cast<const uint32_t*>(p);
-  }
-}
-template <int kWords>
-__device__ __forceinline__ void store_words(__nv_bfloat16* p, const uint32_t* w) {
-  if constexpr (kWords == 4) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-  else if constexpr (kWords == 2) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
-  else *reinterpret_cast<uint32_t*>(p) = w[0];
-}
 __device__ __forceinline__ int spread(int g) { return (g & 1) * 4 + (g >> 1); }
 
 template <int kD>
-struct FewShape {
+struct FewShape : Pieces<kD> {
   static constexpr int keys = kD == 128 ? 16 : 32;                    // of a step
   static constexpr int chunks = kD == 128 ? 2 : 1;                    // of 64 columns
   static constexpr int chunk_bytes = keys * 128;
   static constexpr int stage_bytes = 2 * chunks * chunk_bytes;        // keys, then values: 8 KiB
   static constexpr int stages = 3;
   static constexpr int smem = kWarps * stages * stage_bytes + 1024;
-  static constexpr int k_words = kD == 16 ? 2 : 4, k_pieces = kD == 16 ? 1 : kD / 32;
-  static constexpr int v_words = kD >= 64 ? 4 : kD / 16, v_pieces = kD >= 64 ? kD / 64 : 1;
-  static constexpr int v_cols = 2 * v_words;                          // columns of a piece
 };
 
 struct FewMaps {
@@ -239,11 +211,7 @@ attention_few_kernel(const __grid_constant__ FewMaps maps, const __grid_constant
 #pragma unroll
             for (int i = 0; i < S::v_words; ++i) w[e][i] = 0u;
         }
-#pragma unroll
-        for (int i = 0; i < S::v_words; ++i) {
-          mma16(o[pc * S::v_cols + 2 * i], p, __byte_perm(w[0][i], w[1][i], 0x5410), __byte_perm(w[2][i], w[3][i], 0x5410));
-          mma16(o[pc * S::v_cols + 2 * i + 1], p, __byte_perm(w[0][i], w[1][i], 0x7632), __byte_perm(w[2][i], w[3][i], 0x7632));
-        }
+        mma_values<S::v_words>(o + pc * S::v_cols, p, w);
       }
     }
     __syncwarp();

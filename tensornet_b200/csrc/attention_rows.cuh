@@ -2,7 +2,8 @@
 //
 // Queries stand at the end of their keys: query i of a sequence with nq queries and nk keys stands at place i + nk - nq.  Key j is
 // visible if j < nk and, where causal, j <= place or j < prefix: every mask is a limit per query, the number of keys it sees.
-// Scores are kept in units of log2:  s = c q.k,  or cap tanh(scale q.k / cap) with a cap, less slope |place - j|.
+// Scores are kept in units of log2:  s = c q.k,  or cap tanh(scale q.k / cap) with a cap, less slope |place - j|.  The tanh is
+// 1 - 2 / (1 + e^2x), one exponential: off by 2^-23 of its range, not of its value, which is what a score needs.
 #pragma once
 #include <cuda_bf16.h>
 #include <math_constants.h>
@@ -36,6 +37,7 @@ struct Tile {
 __host__ __device__ __forceinline__ long long tile_count(const AttnRows& r, int B, int m) {
   return r.off == nullptr ? (long long)B * ((r.T + m - 1) / m) : (long long)r.T / m + B + 2;
 }
+// By a converged warp, all of whose lanes look at a segment each: three rounds of loads find one of 32768 sequences.
 __device__ __forceinline__ Tile tile_of(const AttnRows& r, int B, int m, int at) {
   if (r.off == nullptr) {
     const int per = (r.T + m - 1) / m;
@@ -43,10 +45,12 @@ __device__ __forceinline__ Tile tile_of(const AttnRows& r, int B, int m, int at)
     return {seq, {seq, 0, r.T}, (at - seq * per) * m, true};
   }
   auto start = [&](int s) { return s == 0 ? 0 : (s > B + 1 ? r.T : cut(r.off[s - 1], 0, r.T)); };
-  int lo = 0, hi = B + 1;                                  // the last segment that starts at or before tile `at`
+  int lo = 0, hi = B + 1;                                  // between them lies the last segment that starts at or before tile `at`
   while (lo < hi) {
-    const int mid = (lo + hi + 1) / 2;
-    if (start(mid) / m + mid <= at) lo = mid; else hi = mid - 1;
+    const int step = (hi - lo + 31) / 32, s = lo + ((int)(threadIdx.x & 31) + 1) * step;
+    const bool before = s <= hi && start(s) / m + s <= at;
+    lo += __popc(__ballot_sync(0xffffffffu, before)) * step;
+    hi = min(hi, lo + step - 1);
   }
   const int s0 = start(lo), s1 = max(s0, start(lo + 1));
   const int first = (at - (s0 / m + lo)) * m;
@@ -61,20 +65,13 @@ __device__ __forceinline__ int keys_seen(const AttnArgs& a, int seq, int i, int 
   return cut(lim, 0, nk);
 }
 
-// tanh through one exponential: off by 2^-23 of its range, not of its value, which is what a score needs
-__device__ __forceinline__ float tanh_of(float x) { return 1.f - __fdividef(2.f, 1.f + exp2f(2.f * kLog2e * x)); }
-
-// score of a product; th: the tanh of a capped one
-__device__ __forceinline__ float score_of(const AttnArgs& a, float dot, float slope2, int away, float& th) {
-  float s;
-  if (a.cap > 0.f) {
-    th = tanh_of(dot * a.scale / a.cap);
-    s = a.cap * kLog2e * th;
-  } else {
-    s = dot * (a.scale * kLog2e);
-  }
-  return s - slope2 * (float)abs(away);
+// the first query of a sequence that sees key j
+__device__ __forceinline__ int first_query(const AttnArgs& a, int seq, int j, int nq, int nk) {
+  if (!a.causal || (a.prefix != nullptr && j < a.prefix[seq])) return 0;
+  return max(0, j + nq - nk);
 }
+
+__device__ __forceinline__ long long flat_rows(const AttnRows& r, int B) { return r.off ? r.T : (long long)B * r.T; }
 
 __device__ __forceinline__ const __nv_bfloat16* at(const AttnOperand& o, int b, long long t, int h) {
   return reinterpret_cast<const __nv_bfloat16*>(o.p) + b * o.sb + t * o.st + h * o.sh;

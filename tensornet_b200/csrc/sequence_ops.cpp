@@ -181,7 +181,9 @@ struct Attention : torch::autograd::Function<Attention> {
         lse = at::empty({a.H, q.numel() / (a.H * a.D)}, q.options().dtype(at::kFloat));
         a.lse = lse.data_ptr<float>();
       }
-      if (tn::attention_few_takes(a)) {
+      if (tn::attention_short_takes(a)) {
+        told(tn::launch_attention_short_fwd(a, counted_stream()));
+      } else if (tn::attention_few_takes(a)) {
         at::Tensor work;
         if (const long long n = tn::attention_few_floats(a)) {
           work = at::empty({n}, q.options().dtype(at::kFloat));
