@@ -205,9 +205,10 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
     const int my_vis = t == 0 ? vis[0] : vis[kTiles - 1];
     const int lim = i < qs.n ? keys_seen(a, tile.seq, i, qs.n, ks.n) : my_vis;
     const int least = keys_seen(a, tile.seq, tile.first + t * kRows, qs.n, ks.n);      // of the tile's queries
-    const float c = kCap ? 2.f * kLog2e * a.scale / a.cap : a.scale * kLog2e;
+    const float c = kCap ? a.scale / a.cap : a.scale * kLog2e;
     const float cap2 = a.cap * kLog2e;
     const float slope2 = kBias ? a.slopes[h] * kLog2e : 0.f;
+    const int place0 = tile.first + t * kRows + ks.n - qs.n;          // of the tile's first query
     const int place = i + ks.n - qs.n;
     float m = kNone, l = 0.f;
     bool ok = true;
@@ -216,25 +217,66 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
       tc_fence_after();
       const int wide = min(kRows, my_vis - j * kRows);              // columns of scores
       const bool masked = (j + 1) * kRows > least;
-      float s[kRows];
+      float2 s[kRows / 2];
 #pragma unroll
       for (int c0 = 0; c0 < kRows; c0 += 32)
-        if (c0 < wide) tmem_ld32_nowait(tm_s + c0, reinterpret_cast<uint32_t*>(s + c0));
+        if (c0 < wide) tmem_ld32_nowait(tm_s + c0, reinterpret_cast<uint32_t*>(s + c0 / 2));
       tmem_ld_wait();
-      float top = kNone;
+      const int j0 = j * kRows;
+      // all keys on one side of all queries: the distance is linear in the key
+      const float side = kBias ? (j0 + kRows <= place0 ? 1.f : (j0 >= place0 + kRows ? -1.f : 0.f)) : 0.f;
+      float tops[4] = {kNone, kNone, kNone, kNone};
 #pragma unroll
       for (int c0 = 0; c0 < kRows; c0 += 32) {
         if (c0 >= wide) continue;
+        float2* x = s + c0 / 2;
+        if (kCap) {
+          float far[2] = {0.f, 0.f};
 #pragma unroll
-        for (int e = c0; e < c0 + 32; ++e) {
-          float x = s[e];
-          if (kCap) x = cap2 - __fdividef(2.f * cap2, 1.f + ex2(x * c));
-          if (kBias) x = (kCap ? x : x * c) - slope2 * fabsf((float)(place - (j * kRows + e)));
-          if (masked) x = j * kRows + e < lim ? x : kNone;
-          s[e] = x;
-          top = fmaxf(top, x);
+          for (int e = 0; e < 16; ++e) {
+            x[e] = mul2(x[e], both(c));
+            far[e & 1] = max3(far[e & 1], fabsf(x[e].x), fabsf(x[e].y));
+          }
+          if (__all_sync(0xffffffffu, fmaxf(far[0], far[1]) <= 1.f)) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[e] = mul2(tanh_small(x[e]), both(cap2));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[e] = make_float2(cap2 * tanh_any(x[e].x), cap2 * tanh_any(x[e].y));
+          }
         }
+        if (kBias) {
+          if (side != 0.f) {
+            const float2 from = both(slope2 * side * (float)(j0 + c0 - place)), by = both(slope2 * side);
+            float2 n = make_float2(0.f, 1.f);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float2 bias = fma2(n, by, from);
+              x[e] = kCap ? add2(x[e], bias) : fma2(x[e], both(c), bias);
+              n = add2(n, both(2.f));
+            }
+          } else {
+            const float away = (float)(place - j0 - c0);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              if (!kCap) x[e] = mul2(x[e], both(c));
+              x[e].x = fmaf(-slope2, fabsf(away - (float)(2 * e)), x[e].x);
+              x[e].y = fmaf(-slope2, fabsf(away - (float)(2 * e + 1)), x[e].y);
+            }
+          }
+        }
+        if (masked) {
+          const int there = lim - j0 - c0;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            x[e].x = 2 * e < there ? x[e].x : kNone;
+            x[e].y = 2 * e + 1 < there ? x[e].y : kNone;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) tops[e & 3] = max3(tops[e & 3], x[e].x, x[e].y);
       }
+      float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
       if (!kCap && !kBias) top *= c;
       const bool grown = top > m + kGrowth;
       if (__any_sync(0xffffffffu, grown)) {
@@ -253,20 +295,24 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
           }
         }
       }
-      const float ref = m == kNone ? 0.f : m;
+      const float2 ref = both(m == kNone ? 0.f : -m);
+      float2 sums[2] = {make_float2(l, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
       for (int c0 = 0; c0 < kRows; c0 += 32) {
         if (c0 >= wide) continue;
         uint32_t w[16];
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          const float p0 = ex2((kCap || kBias) ? s[c0 + e] - ref : fmaf(s[c0 + e], c, -ref));
-          const float p1 = ex2((kCap || kBias) ? s[c0 + e + 1] - ref : fmaf(s[c0 + e + 1], c, -ref));
-          l += p0 + p1;
-          w[e / 2] = pack_bf16(p0, p1);
+        for (int e = 0; e < 16; ++e) {
+          float2 x = s[c0 / 2 + e];
+          x = (kCap || kBias) ? add2(x, ref) : fma2(x, both(c), ref);
+          x = make_float2(ex2(x.x), ex2(x.y));
+          sums[e & 1] = add2(sums[e & 1], x);
+          w[e] = pack_bf16(x.x, x.y);
         }
         tmem_st16(tm_s + c0 / 2, w);
       }
+      sums[0] = add2(sums[0], sums[1]);
+      l = sums[0].x + sums[0].y;
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(smem_u32(&s_weight[t]));
