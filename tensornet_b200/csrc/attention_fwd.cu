@@ -3,16 +3,17 @@
 //   s = scores of 128 queries with 128 keys;  m = the largest so far;  p = 2^(s - m);  l += sum p;  o += p v;  out = o / l
 //
 // One pass over the keys.  A block has one or two tiles of 128 queries: a warp loads tiles of keys and values by TMA into a ring, a
-// warp issues the products, and a warpgroup per tile has a query per thread, so that maxima and sums never leave a thread.  Scores
-// are read from tensor memory into registers, and the weights go back into the columns that the scores had, as the left operand
-// of the product with the values.
+// warp issues the products, and two warpgroups per tile have half of a query's keys per thread: with one, a tile's softmax took
+// twice as long as its products, most of it latency.  Scores are read from tensor memory into registers, and the weights go back
+// into the columns that the scores had, as the left operand of the product with the values.
 //
 // The order of products is  s0(0) s1(0) | o0(0) s0(1) | o1(0) s1(1) | ...: while one tile's weights are made, the other's products
 // run.  Products of one thread run in the order of their issue, so the next scores may overwrite the weights that the
 // product before them reads, and a barrier behind s(j + 1) also says that o(j) is there.
 //
 // The reference m of a row moves only when its maximum has grown by more than 2^8: weights then stay below 2^8, and what has been
-// added up is brought to the new reference by the thread that owns the row.  Sums are fp32, weights bf16 for the product (their
+// added up is brought to the new reference by the threads that own the row.  So the two have to tell each other no more than
+// whether any row of theirs has grown that much, which rarely happens behind the first tile.  Sums are fp32, weights bf16 for the product (their
 // sum takes them unrounded).
 #include <cuda_bf16.h>
 #include <mutex>
@@ -24,7 +25,7 @@ namespace {
 
 using namespace attn;
 
-constexpr int kRows = 128;
+constexpr int kRows = 128, kHalf = 64;
 constexpr float kGrowth = 8.f;
 
 template <int kD, int kTiles>
@@ -32,12 +33,27 @@ struct FwdShape {
   static constexpr int chunks = kD / 64;
   static constexpr int tile_bytes = kRows * 128 * chunks;
   static constexpr int slots = kTiles == 2 ? (kD == 128 ? 4 : 6) : (kD == 128 ? 2 : 4);
-  static constexpr int softmax_warps = 4 * kTiles;
+  static constexpr int softmax_warps = 8 * kTiles;
   static constexpr int threads = 32 * (softmax_warps + 2);
   static constexpr int smem = tile_bytes * (kTiles + slots) + 1024;
   static constexpr int tmem_cols = kTiles == 2 ? 512 : 256;
   static constexpr int o_col = 128 * kTiles;
 };
+
+// The two warps that have half of the same queries' keys each
+__device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ bool any_of_pair(int id, bool p) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %2, 0;\n\t"
+      "bar.red.or.pred q, %1, 64, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(any)
+      : "r"(id), "r"((uint32_t)p)
+      : "memory");
+  return any != 0;
+}
 
 struct FwdMaps {
   CUtensorMap q, k, v;
@@ -50,6 +66,7 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
   constexpr int kSlots = Shape::slots;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t s_q, s_full[kSlots], s_empty[kSlots], s_score[kTiles], s_weight[kTiles], s_out[kTiles];
+  __shared__ float s_pass[kTiles][2][kRows];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort_i;
   volatile int* s_abort = &s_abort_i;
@@ -96,7 +113,7 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
     for (int s = 0; s < kSlots; ++s) { mbar_init(smem_u32(&s_full[s]), 1); mbar_init(smem_u32(&s_empty[s]), 1); }
     for (int t = 0; t < kTiles; ++t) {
       mbar_init(smem_u32(&s_score[t]), 1);
-      mbar_init(smem_u32(&s_weight[t]), kRows);
+      mbar_init(smem_u32(&s_weight[t]), 2 * kRows);
       mbar_init(smem_u32(&s_out[t]), 1);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -197,11 +214,12 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
     }
     if (!ok) *s_abort = 1;
   } else {
-    // ---- softmax: a query per thread
-    const int t = warp >> 2, r = (warp & 3) * 32 + lane;
+    // ---- softmax: half of a query's keys per thread
+    const int t = warp >> 3, half = (warp >> 2) & 1, r = (warp & 3) * 32 + lane;
+    const int pair = 1 + t * 4 + (warp & 3);           // the barrier of the two warps that share 32 queries
     const int i = tile.first + t * kRows + r;
     const uint32_t tm = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t tm_s = tm + t * 128, tm_o = tm + Shape::o_col + t * kD;
+    const uint32_t tm_s = tm + t * 128 + half * kHalf, tm_p = tm + t * 128 + half * (kHalf / 2), tm_o = tm + Shape::o_col + t * kD;
     const int my_vis = t == 0 ? vis[0] : vis[kTiles - 1];
     const int lim = i < qs.n ? keys_seen(a, tile.seq, i, qs.n, ks.n) : my_vis;
     const int least = keys_seen(a, tile.seq, tile.first + t * kRows, qs.n, ks.n);      // of the tile's queries
@@ -211,23 +229,24 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
     const int place0 = tile.first + t * kRows + ks.n - qs.n;          // of the tile's first query
     const int place = i + ks.n - qs.n;
     float m = kNone, l = 0.f;
+    const int d_half = round16(d16 / 2);
     bool ok = true;
     for (int j = 0; j * kRows < my_vis; ++j) {
-      if (!mbar_wait_warp(smem_u32(&s_score[t]), j & 1, s_abort)) { *s_abort = 1; ok = false; break; }
+      ok = ok && mbar_wait_warp(smem_u32(&s_score[t]), j & 1, s_abort);
+      if (!ok) *s_abort = 1;         // (the pair's barriers are passed all the same)
       tc_fence_after();
-      const int wide = min(kRows, my_vis - j * kRows);              // columns of scores
-      const bool masked = (j + 1) * kRows > least;
-      float2 s[kRows / 2];
+      const int j0 = j * kRows + half * kHalf, wide = min(kHalf, my_vis - j0);              // columns of scores
+      const bool masked = j0 + kHalf > least;
+      float2 s[kHalf / 2];
 #pragma unroll
-      for (int c0 = 0; c0 < kRows; c0 += 32)
-        if (c0 < wide) tmem_ld32_nowait(tm_s + c0, reinterpret_cast<uint32_t*>(s + c0 / 2));
+      for (int c0 = 0; c0 < kHalf; c0 += 32)
+        if (ok && c0 < wide) tmem_ld32_nowait(tm_s + c0, reinterpret_cast<uint32_t*>(s + c0 / 2));
       tmem_ld_wait();
-      const int j0 = j * kRows;
       // all keys on one side of all queries: the distance is linear in the key
-      const float side = kBias ? (j0 + kRows <= place0 ? 1.f : (j0 >= place0 + kRows ? -1.f : 0.f)) : 0.f;
+      const float side = kBias ? (j0 + kHalf <= place0 ? 1.f : (j0 >= place0 + kRows ? -1.f : 0.f)) : 0.f;
       float tops[4] = {kNone, kNone, kNone, kNone};
 #pragma unroll
-      for (int c0 = 0; c0 < kRows; c0 += 32) {
+      for (int c0 = 0; c0 < kHalf; c0 += 32) {
         if (c0 >= wide) continue;
         float2* x = s + c0 / 2;
         if (kCap) {
@@ -278,14 +297,17 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
       }
       float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
       if (!kCap && !kBias) top *= c;
-      const bool grown = top > m + kGrowth;
-      if (__any_sync(0xffffffffu, grown)) {
-        const float to = grown ? top : m;
+      // (behind the barrier both warps have their scores in registers, and weights may take their place)
+      if (any_of_pair(pair, top > m + kGrowth)) {
+        s_pass[t][half][r] = top;
+        pair_sync(pair);
+        top = fmaxf(top, s_pass[t][half ^ 1][r]);
+        const float to = top > m + kGrowth ? top : m;
         const float by = to == kNone ? 1.f : ex2(m - to);
         m = to;
         l *= by;
         if (j > 0) {
-          for (int c0 = 0; c0 < d16; c0 += 16) {
+          for (int c0 = half * d_half; c0 < (half ? d16 : d_half); c0 += 16) {
             float o[16];
             tmem_ld16_nowait(tm_o + c0, reinterpret_cast<uint32_t*>(o));
             tmem_ld_wait();
@@ -294,11 +316,12 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
             tmem_st16(tm_o + c0, reinterpret_cast<const uint32_t*>(o));
           }
         }
+        pair_sync(pair);                               // s_pass is free again
       }
       const float2 ref = both(m == kNone ? 0.f : -m);
       float2 sums[2] = {make_float2(l, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-      for (int c0 = 0; c0 < kRows; c0 += 32) {
+      for (int c0 = 0; c0 < kHalf; c0 += 32) {
         if (c0 >= wide) continue;
         uint32_t w[16];
 #pragma unroll
@@ -309,7 +332,7 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
           sums[e & 1] = add2(sums[e & 1], x);
           w[e] = pack_bf16(x.x, x.y);
         }
-        tmem_st16(tm_s + c0 / 2, w);
+        tmem_st16(tm_p + c0 / 2, w);
       }
       sums[0] = add2(sums[0], sums[1]);
       l = sums[0].x + sums[0].y;
@@ -317,6 +340,9 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
       tc_fence_before();
       mbar_arrive(smem_u32(&s_weight[t]));
     }
+    s_pass[t][half][r] = l;
+    pair_sync(pair);
+    l += s_pass[t][half ^ 1][r];
     if (ok && my_vis > 0) {
       ok = mbar_wait_warp(smem_u32(&s_out[t]), 0, s_abort);
       if (!ok) *s_abort = 1;
@@ -327,7 +353,7 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
       const bool mine = t * kRows + r < tile_rows;
       const long long row = tile.rows.first + i;
       __nv_bfloat16* out = at_out(a.o, tile.rows.b, row, h);
-      for (int c0 = 0; c0 < a.D; c0 += 16) {
+      for (int c0 = half * d_half; c0 < (half ? a.D : min(a.D, d_half)); c0 += 16) {
         float o[16];
         if (my_vis > 0) {
           tmem_ld16_nowait(tm_o + c0, reinterpret_cast<uint32_t*>(o));
@@ -342,7 +368,7 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
         }
         __syncwarp();
       }
-      if (a.lse != nullptr && mine)
+      if (a.lse != nullptr && mine && half == 0)
         a.lse[(long long)h * (a.rq.off ? a.rq.T : (long long)a.B * a.rq.T) + (a.rq.off ? 0 : (long long)tile.rows.b * a.rq.T) + row] =
             w != 0.f ? m + log2f(l) : CUDART_INF_F;
     }
