@@ -98,9 +98,9 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
       all_hi = keys_seen(a, tile.seq, tile.first, qs.n, ks.n);
     }
   }
-  const int per_head = hi > lo ? (hi - lo + kY - 1) / kY : 0;
-  const int steps = per_head * (kKeys ? R : 1);
-  if (steps == 0) {
+  const int per_head_ = hi > lo ? (hi - lo + kY - 1) / kY : 0;
+  const int steps_ = per_head_ * (kKeys ? R : 1);
+  if (steps_ == 0) {
     const int per = a.D / 8;
     for (int i = threadIdx.x; i < tile_rows * per; i += Shape::threads) {
       const long long row = tile.rows.first + tile.first + i / per;
@@ -109,6 +109,12 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
     }
     return;
   }
+  // what one lane's loads and products are addressed with is known to be the same for the warp
+  const int steps = one_of_warp(steps_), per_head = one_of_warp(per_head_);
+  lo = one_of_warp(lo);
+  hi = one_of_warp(hi);
+  const int y_end = one_of_warp(ys.n), y_begin = one_of_warp(ys.first), y_b = one_of_warp(ys.b), x_begin = one_of_warp(xs.first + tile.first);
+  head = one_of_warp(head);
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* ring_gen = smem_raw + (base - smem_u32(smem_raw)) + 2 * Shape::x_bytes;
   const uint32_t ring = base + 2 * Shape::x_bytes;
@@ -139,7 +145,7 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
         for (int c = 0; c < Shape::chunks; ++c)
           for (int r = 0; r < kX; r += kY)
             tma_load_4d(base + o * Shape::x_bytes + c * (kX * 128) + r * 128, kKeys ? (o ? &maps.v : &maps.k) : (o ? &maps.go : &maps.q), 64 * c,
-                        xs.first + tile.first + r, head, xs.b, bar);
+                        x_begin + r, head, xs.b, bar);
     }
     __syncwarp();
     for (int it = 0; it < steps; ++it) {
@@ -151,7 +157,7 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
         for (int o = 0; o < 2; ++o)
           for (int c = 0; c < Shape::chunks; ++c)
             tma_load_4d(to + o * Shape::y_bytes + c * (kY * 128), kKeys ? (o ? &maps.go : &maps.q) : (o ? &maps.v : &maps.k), 64 * c,
-                        ys.first + y_first(it), y_head(it), ys.b, bar);
+                        y_begin + y_first(it), y_head(it), y_b, bar);
       }
       __syncwarp();
     }
@@ -165,7 +171,7 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
       ok = ok && mbar_wait_warp(smem_u32(&sh.full[s]), (it / kSlots) & 1, s_abort);
       if (!ok) return;
       tc_fence_after();
-      const int end = ys.n - y_first(it);
+      const int end = y_end - y_first(it);
       if (end < kY && (end & 15)) {      // rows behind the sequence's end
         zero_rows<kY>(ring_gen + s * 2 * Shape::y_bytes, Shape::chunks, end, round16(end), lane);
         zero_rows<kY>(ring_gen + s * 2 * Shape::y_bytes + Shape::y_bytes, Shape::chunks, end, round16(end), lane);
@@ -174,8 +180,14 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
       const uint32_t to = tm + (it % kStages) * 2 * kY;
       const uint32_t id = idesc_of(round16(min(kY, hi - y_first(it))), false);
       if (lead) {
-        for (int k = 0; k < d16 / 16; ++k) umma_f16(to, desc_k<kX>(base, k), desc_k<kY>(y1, k), id, k > 0);
-        for (int k = 0; k < d16 / 16; ++k) umma_f16(to + kY, desc_k<kX>(base + Shape::x_bytes, k), desc_k<kY>(y2, k), id, k > 0);
+        const uint64_t x1 = make_smem_desc(base, 16u, 1024u), x2 = make_smem_desc(base + Shape::x_bytes, 16u, 1024u);
+        const uint64_t d1 = make_smem_desc(y1, 16u, 1024u), d2 = make_smem_desc(y2, 16u, 1024u);
+#pragma unroll
+        for (int k = 0; k < kD / 16; ++k)
+          if (k * 16 < d16) umma_f16(to, x1 + step_k<kX>(k), d1 + step_k<kY>(k), id, k > 0);
+#pragma unroll
+        for (int k = 0; k < kD / 16; ++k)
+          if (k * 16 < d16) umma_f16(to + kY, x2 + step_k<kX>(k), d2 + step_k<kY>(k), id, k > 0);
         umma_commit(smem_u32(&sh.score[it % kStages]));
       }
       __syncwarp();
@@ -191,9 +203,14 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
       const int n = round16(min(kY, hi - y_first(it))) / 16;
       const uint32_t id = idesc_of(d16, true);
       if (lead) {
-        for (int k = 0; k < n; ++k) umma_f16_ts(tm + Shape::acc_col, from + kY + k * 8, desc_mn<kY>(y1, k), id, it > 0 || k > 0);
+        const uint64_t d1 = make_smem_desc(y1, kY * 128, 1024u), d2 = make_smem_desc(y2, kY * 128, 1024u);
+#pragma unroll
+        for (int k = 0; k < kY / 16; ++k)
+          if (k < n) umma_f16_ts(tm + Shape::acc_col, from + kY + k * 8, d1 + step_mn(k), id, it > 0 || k > 0);
         if (kKeys)
-          for (int k = 0; k < n; ++k) umma_f16_ts(tm + Shape::acc_col + kD, from + k * 8, desc_mn<kY>(y2, k), id, it > 0 || k > 0);
+#pragma unroll
+          for (int k = 0; k < kY / 16; ++k)
+            if (k < n) umma_f16_ts(tm + Shape::acc_col + kD, from + k * 8, d2 + step_mn(k), id, it > 0 || k > 0);
         umma_commit(it + 1 == steps ? smem_u32(&sh.acc) : smem_u32(&sh.empty[s]));
       }
       __syncwarp();

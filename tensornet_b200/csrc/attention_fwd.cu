@@ -102,7 +102,10 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
               tile.first + i] = CUDART_INF_F;
     return;
   }
-  const int steps = (most + kRows - 1) / kRows;
+  // what one lane's loads and products are addressed with is known to be the same for the warp
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t) vis[t] = one_of_warp(vis[t]);
+  const int steps = one_of_warp((most + kRows - 1) / kRows);
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_gen = smem_raw + (base - smem_u32(smem_raw));
   const uint32_t ring = base + kTiles * Shape::tile_bytes;
@@ -127,7 +130,7 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
 
   if (warp == Shape::softmax_warps) {
     // ---- loads: the queries, then k(0) v(0) k(1) v(1) ... through the ring
-    const int g = h / (a.H / a.G);
+    const int g = h / (a.H / a.G), k_first = one_of_warp(ks.first), k_b = one_of_warp(ks.b), q_first = one_of_warp(qs.first + tile.first);
     const bool lead = elect_one();
     if (lead) {
       int n = 0;
@@ -136,7 +139,7 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
       for (int t = 0; t < kTiles; ++t)
         if (vis[t] > 0)
           for (int c = 0; c < Shape::chunks; ++c)
-            tma_load_4d(base + t * Shape::tile_bytes + c * (kRows * 128), &maps.q, 64 * c, qs.first + tile.first + t * kRows, h, qs.b, smem_u32(&s_q));
+            tma_load_4d(base + t * Shape::tile_bytes + c * (kRows * 128), &maps.q, 64 * c, q_first + t * kRows, h, qs.b, smem_u32(&s_q));
     }
     __syncwarp();
     for (int i = 0; i < 2 * steps; ++i) {
@@ -146,7 +149,7 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
         const uint32_t bar = smem_u32(&s_full[s]);
         mbar_expect_tx(bar, Shape::tile_bytes);
         for (int c = 0; c < Shape::chunks; ++c)
-          tma_load_4d(ring + s * Shape::tile_bytes + c * (kRows * 128), (i & 1) ? &maps.v : &maps.k, 64 * c, ks.first + (i >> 1) * kRows, g, ks.b, bar);
+          tma_load_4d(ring + s * Shape::tile_bytes + c * (kRows * 128), (i & 1) ? &maps.v : &maps.k, 64 * c, k_first + (i >> 1) * kRows, g, k_b, bar);
       }
       __syncwarp();
     }
@@ -163,7 +166,10 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
       const uint32_t q = base + t * Shape::tile_bytes, k = ring + (2 * j % kSlots) * Shape::tile_bytes;
       const uint32_t id = idesc_of(round16(min(kRows, vis[t] - j * kRows)), false);
       if (lead) {
-        for (int s = 0; s < d16 / 16; ++s) umma_f16(tm + t * 128, desc_k<kRows>(q, s), desc_k<kRows>(k, s), id, s > 0);
+        const uint64_t qd = make_smem_desc(q, 16u, 1024u), kd = make_smem_desc(k, 16u, 1024u);
+#pragma unroll
+        for (int s = 0; s < kD / 16; ++s)
+          if (s * 16 < d16) umma_f16(tm + t * 128, qd + step_k<kRows>(s), kd + step_k<kRows>(s), id, s > 0);
         umma_commit(smem_u32(&s_score[t]));
       }
       __syncwarp();
@@ -172,8 +178,12 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
       const uint32_t v = ring + ((2 * j + 1) % kSlots) * Shape::tile_bytes;
       const int n = round16(min(kRows, vis[t] - j * kRows)) / 16;
       const uint32_t id = idesc_of(d16, true);
-      if (lead)
-        for (int s = 0; s < n; ++s) umma_f16_ts(tm + Shape::o_col + t * kD, tm + t * 128 + s * 8, desc_mn<kRows>(v, s), id, j > 0 || s > 0);
+      if (lead) {
+        const uint64_t vd = make_smem_desc(v, kRows * 128, 1024u);
+#pragma unroll
+        for (int s = 0; s < kRows / 16; ++s)
+          if (s < n) umma_f16_ts(tm + Shape::o_col + t * kD, tm + t * 128 + s * 8, vd + step_mn(s), id, j > 0 || s > 0);
+      }
       __syncwarp();
     };
     auto free_slot = [&](int i) {

@@ -98,16 +98,14 @@ __device__ __forceinline__ void tmem_dealloc(uint32_t tmem) {
 __device__ __forceinline__ uint32_t idesc_of(int n, bool b_mn) {
   return (1u << 4) | (1u << 7) | (1u << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
 }
-// Step ks of 16 along the columns of a tile of kRows rows
+// What a descriptor grows by for step s of 16: along the columns of a tile of kRows rows (K-major), along its rows (MN-major)
 template <int kRows>
-__device__ __forceinline__ uint64_t desc_k(uint32_t tile, int ks) {
-  return make_smem_desc(tile + (ks >> 2) * (kRows * 128) + (ks & 3) * 32, 16u, 1024u);
-}
-// Step ks of 16 along its rows
-template <int kRows>
-__device__ __forceinline__ uint64_t desc_mn(uint32_t tile, int ks) {
-  return make_smem_desc(tile + ks * 2048, kRows * 128, 1024u);
-}
+__device__ constexpr uint64_t step_k(int s) { return (uint64_t)(((s >> 2) * (kRows * 128) + (s & 3) * 32) >> 4); }
+__device__ constexpr uint64_t step_mn(int s) { return (uint64_t)((s * 2048) >> 4); }
+
+// `v`, the same for all lanes, in a form that the compiler knows to be: descriptors and coordinates made of it need not be collected
+// from a lane's registers for each instruction
+__device__ __forceinline__ int one_of_warp(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 
 __device__ __forceinline__ int round16(int n) { return (n + 15) & ~15; }
 
