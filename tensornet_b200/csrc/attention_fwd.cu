@@ -3,18 +3,25 @@
 //   s = scores of 128 queries with 128 keys;  m = the largest so far;  p = 2^(s - m);  l += sum p;  o += p v;  out = o / l
 //
 // One pass over the keys.  A block has one or two tiles of 128 queries: a warp loads tiles of keys and values by TMA into a ring, a
-// warp issues the products, and two warpgroups per tile have half of a query's keys per thread: with one, a tile's softmax took
-// twice as long as its products, most of it latency.  Scores are read from tensor memory into registers, and the weights go back
-// into the columns that the scores had, as the left operand of the product with the values.
+// warp issues the products, and a warpgroup per tile has a query per thread, or two, where scores are capped, half of a query's keys
+// per thread.  Scores are read from tensor memory into registers, and the weights go back into the columns that the scores had, as
+// the left operand of the product with the values.
 //
 // The order of products is  s0(0) s1(0) | o0(0) s0(1) | o1(0) s1(1) | ...: while one tile's weights are made, the other's products
 // run.  Products of one thread run in the order of their issue, so the next scores may overwrite the weights that the
 // product before them reads, and a barrier behind s(j + 1) also says that o(j) is there.
 //
 // The reference m of a row moves only when its maximum has grown by more than 2^8: weights then stay below 2^8, and what has been
-// added up is brought to the new reference by the threads that own the row.  So the two have to tell each other no more than
-// whether any row of theirs has grown that much, which rarely happens behind the first tile.  Sums are fp32, weights bf16 for the product (their
-// sum takes them unrounded).
+// added up is brought to the new reference by the threads that own the row.  Sums are fp32, weights bf16 for the product (their sum
+// takes them unrounded).
+//
+// What bounds it is the exponentials, 2048 cycles of the special function unit per step of two tiles, and the latency around them:
+// a step takes 3300 at 64 columns and 3700 at 128, where its products take 1024 and 2048.  A quarter of the exponentials is a
+// polynomial (ex2_poly); with a third the instructions cost more than that saves.  2 x 4096 x 16 heads, us at 64 and 128 columns:
+//   a query per thread 261, 281; and a quarter polynomial 238, 270; a third 256, 274
+//   half a query per thread 244, 283; and a quarter polynomial 248, 286 (capped, 8192 causal: 498; a query per thread 550)
+//   weights in columns of their own, scores ahead, a warp of products per tile: 246, 297; weights ahead of the maximum: 250, 322
+//   steps of 64 keys with two buffers of scores: 283, 356
 #include <cuda_bf16.h>
 #include <mutex>
 #include "attention_tc.cuh"
@@ -25,15 +32,15 @@ namespace {
 
 using namespace attn;
 
-constexpr int kRows = 128, kHalf = 64;
+constexpr int kRows = 128;
 constexpr float kGrowth = 8.f;
 
-template <int kD, int kTiles>
+template <int kD, int kTiles, int kHalves>
 struct FwdShape {
   static constexpr int chunks = kD / 64;
   static constexpr int tile_bytes = kRows * 128 * chunks;
   static constexpr int slots = kTiles == 2 ? (kD == 128 ? 4 : 6) : (kD == 128 ? 2 : 4);
-  static constexpr int softmax_warps = 8 * kTiles;
+  static constexpr int softmax_warps = 4 * kHalves * kTiles;
   static constexpr int threads = 32 * (softmax_warps + 2);
   static constexpr int smem = tile_bytes * (kTiles + slots) + 1024;
   static constexpr int tmem_cols = kTiles == 2 ? 512 : 256;
@@ -60,9 +67,10 @@ struct FwdMaps {
 };
 
 template <int kD, int kTiles, bool kCap, bool kBias>
-__global__ void __launch_bounds__(FwdShape<kD, kTiles>::threads, kTiles == 2 ? 1 : 2)
+__global__ void __launch_bounds__(FwdShape<kD, kTiles, kCap ? 2 : 1>::threads, kTiles == 2 ? 1 : 2)
 attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_constant__ AttnArgs a) {
-  using Shape = FwdShape<kD, kTiles>;
+  constexpr int kHalves = kCap ? 2 : 1, kHalf = kRows / kHalves;      // threads per query, keys of a step per thread
+  using Shape = FwdShape<kD, kTiles, kHalves>;
   constexpr int kSlots = Shape::slots;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t s_q, s_full[kSlots], s_empty[kSlots], s_score[kTiles], s_weight[kTiles], s_out[kTiles];
@@ -116,7 +124,7 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
     for (int s = 0; s < kSlots; ++s) { mbar_init(smem_u32(&s_full[s]), 1); mbar_init(smem_u32(&s_empty[s]), 1); }
     for (int t = 0; t < kTiles; ++t) {
       mbar_init(smem_u32(&s_score[t]), 1);
-      mbar_init(smem_u32(&s_weight[t]), 2 * kRows);
+      mbar_init(smem_u32(&s_weight[t]), kHalves * kRows);
       mbar_init(smem_u32(&s_out[t]), 1);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -224,8 +232,8 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
     }
     if (!ok) *s_abort = 1;
   } else {
-    // ---- softmax: half of a query's keys per thread
-    const int t = warp >> 3, half = (warp >> 2) & 1, r = (warp & 3) * 32 + lane;
+    // ---- softmax
+    const int t = warp / (4 * kHalves), half = kHalves == 2 ? (warp >> 2) & 1 : 0, r = (warp & 3) * 32 + lane;
     const int pair = 1 + t * 4 + (warp & 3);           // the barrier of the two warps that share 32 queries
     const int i = tile.first + t * kRows + r;
     const uint32_t tm = tmem + ((uint32_t)((warp & 3) * 32) << 16);
@@ -239,7 +247,7 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
     const int place0 = tile.first + t * kRows + ks.n - qs.n;          // of the tile's first query
     const int place = i + ks.n - qs.n;
     float m = kNone, l = 0.f;
-    const int d_half = round16(d16 / 2);
+    const int d_half = kHalves == 2 ? round16(d16 / 2) : d16;
     bool ok = true;
     for (int j = 0; j * kRows < my_vis; ++j) {
       ok = ok && mbar_wait_warp(smem_u32(&s_score[t]), j & 1, s_abort);
@@ -308,10 +316,12 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
       float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
       if (!kCap && !kBias) top *= c;
       // (behind the barrier both warps have their scores in registers, and weights may take their place)
-      if (any_of_pair(pair, top > m + kGrowth)) {
-        s_pass[t][half][r] = top;
-        pair_sync(pair);
-        top = fmaxf(top, s_pass[t][half ^ 1][r]);
+      if (kHalves == 2 ? any_of_pair(pair, top > m + kGrowth) : __any_sync(0xffffffffu, top > m + kGrowth) != 0) {
+        if (kHalves == 2) {
+          s_pass[t][half][r] = top;
+          pair_sync(pair);
+          top = fmaxf(top, s_pass[t][half ^ 1][r]);
+        }
         const float to = top > m + kGrowth ? top : m;
         const float by = to == kNone ? 1.f : ex2(m - to);
         m = to;
@@ -326,7 +336,7 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
             tmem_st16(tm_o + c0, reinterpret_cast<const uint32_t*>(o));
           }
         }
-        pair_sync(pair);                               // s_pass is free again
+        if (kHalves == 2) pair_sync(pair);             // s_pass is free again
       }
       const float2 ref = both(m == kNone ? 0.f : -m);
       float2 sums[2] = {make_float2(l, 0.f), make_float2(0.f, 0.f)};
@@ -338,7 +348,7 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
         for (int e = 0; e < 16; ++e) {
           float2 x = s[c0 / 2 + e];
           x = (kCap || kBias) ? add2(x, ref) : fma2(x, both(c), ref);
-          x = make_float2(ex2(x.x), ex2(x.y));
+          x = !kCap && e % 4 == 3 ? ex2_poly(x) : make_float2(ex2(x.x), ex2(x.y));
           sums[e & 1] = add2(sums[e & 1], x);
           w[e] = pack_bf16(x.x, x.y);
         }
@@ -350,9 +360,11 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
       tc_fence_before();
       mbar_arrive(smem_u32(&s_weight[t]));
     }
-    s_pass[t][half][r] = l;
-    pair_sync(pair);
-    l += s_pass[t][half ^ 1][r];
+    if (kHalves == 2) {
+      s_pass[t][half][r] = l;
+      pair_sync(pair);
+      l += s_pass[t][half ^ 1][r];
+    }
     if (ok && my_vis > 0) {
       ok = mbar_wait_warp(smem_u32(&s_out[t]), 0, s_abort);
       if (!ok) *s_abort = 1;
@@ -396,7 +408,7 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
 
 template <int kD, int kTiles, bool kCap, bool kBias>
 cudaError_t launch(const FwdMaps& maps, const AttnArgs& a, cudaStream_t st) {
-  using Shape = FwdShape<kD, kTiles>;
+  using Shape = FwdShape<kD, kTiles, kCap ? 2 : 1>;
   auto* k = attention_fwd_tc_kernel<kD, kTiles, kCap, kBias>;
   cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::smem);      // of the current device
   if (e != cudaSuccess) return e;

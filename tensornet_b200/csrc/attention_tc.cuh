@@ -43,6 +43,23 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 }
 __device__ __forceinline__ float2 both(float a) { return make_float2(a, a); }
 
+// 2^x for two at a time without the special function unit, which makes 16 a cycle and SM: x = n + f, a polynomial for 2^f on
+// [-1/2, 1/2] (least squares reweighted towards the smallest largest relative error: 2.7e-6 in fp32), n added to the exponent.  What
+// comes of -125 is taken off in the end, so that all below, minus infinity too, comes as zero.
+__device__ __forceinline__ float2 ex2_poly(float2 x) {
+  constexpr float c0 = 0.9999992847442627f;
+  x = make_float2(fmaxf(x.x, -125.f), fmaxf(x.y, -125.f));
+  const float2 r = add2(x, both(12582912.f));                     // 1.5 2^23: the integer is in the low bits
+  const float2 f = fma2(add2(r, both(-12582912.f)), both(-1.f), x);
+  float2 p = fma2(f, both(0.009570101276040077f), both(0.05591785907745361f));
+  p = fma2(f, p, both(0.240247443318367f));
+  p = fma2(f, p, both(0.6931217908859253f));
+  p = fma2(f, p, both(c0));
+  p.x = __int_as_float(__float_as_int(p.x) + (__float_as_int(r.x) << 23));
+  p.y = __int_as_float(__float_as_int(p.y) + (__float_as_int(r.y) << 23));
+  return add2(p, both(-c0 * 2.3509887016445750e-38f));           // 2^-125
+}
+
 // tanh for |y| <= 1: y times a polynomial in y^2, least squares reweighted towards the smallest largest error of tanh itself
 // (2.4e-7, 3.2e-7 in fp32).  No exponential, and two at a time.
 __device__ __forceinline__ float2 tanh_small(float2 y) {
