@@ -47,7 +47,7 @@ struct BwdShared {
   uint64_t x, full[BwdShape<kD>::slots], empty[BwdShape<kD>::slots], score[BwdShape<kD>::stages], weight[BwdShape<kD>::stages], acc;
   uint32_t tmem;
   int abort;
-  alignas(16) float vec[BwdShape<kD>::stages][2][2 * kY];      // lse and delta of a tile of queries
+  alignas(16) float vec[BwdShape<kD>::stages][2][2 * kY];      // less lse and delta of a tile of queries
 };
 
 // A thread's columns [c0, c0 + 16) of an accumulator, times w, to a row of the result; zeros where the row has no terms
@@ -223,22 +223,22 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
     const int x = tile.first + r;
     const uint32_t tm_row = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t tm = tm_row + st * 2 * kY;
-    const float c = kCap ? 2.f * kLog2e * a.scale / a.cap : a.scale * kLog2e;
+    const float c = kCap ? a.scale / a.cap : a.scale * kLog2e;
     const float cap2 = a.cap * kLog2e;
     const long long q_rows = flat_rows(a.rq, a.B), q_flat = (a.rq.off ? 0 : (long long)qs.b * a.rq.T) + qs.first;
     // keys: the queries [meet, qs.n) see this one; queries: keys [0, meet) are seen
     const int meet = x < xs.n ? (kKeys ? first_query(a, tile.seq, x, qs.n, ks.n) : keys_seen(a, tile.seq, x, qs.n, ks.n)) : (kKeys ? lo : hi);
     const int shift = ks.n - qs.n;
-    float lse = 0.f, delta = 0.f, next = 0.f;
-    auto fetch = [&](int it) {           // lse (threads 0 to 63) or delta of a query of step `it`
+    float lse = 0.f, delta = 0.f, next = 0.f;      // negative
+    auto fetch = [&](int it) {           // less lse (threads 0 to 63) or delta of a query of step `it`
       const int i = y_first(it) + (r & (kY - 1));
-      return i < qs.n ? (r < kY ? a.lse : a.delta)[y_head(it) * q_rows + q_flat + i] : 0.f;
+      return i < qs.n ? -(r < kY ? a.lse : a.delta)[y_head(it) * q_rows + q_flat + i] : 0.f;
     };
     if (kKeys) {
       if (st < steps) next = fetch(st);
     } else if (x < xs.n) {
-      lse = a.lse[head * q_rows + q_flat + x];
-      delta = a.delta[head * q_rows + q_flat + x];
+      lse = -a.lse[head * q_rows + q_flat + x];
+      delta = -a.delta[head * q_rows + q_flat + x];
     }
     bool ok = true;
     for (int it = st; it < steps; it += kStages) {
@@ -261,47 +261,71 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
 #pragma unroll
       for (int c0 = 0; c0 < kY; c0 += 32) {
         if (c0 >= wide) continue;
-        float s[32], d[32];
+        float2 s[16], d[16];
         tmem_ld32_nowait(tm + c0, reinterpret_cast<uint32_t*>(s));
         tmem_ld32_nowait(tm + kY + c0, reinterpret_cast<uint32_t*>(d));
         tmem_ld_wait();
+        bool near = true;
+        if (kCap) {
+          float far[2] = {0.f, 0.f};
 #pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-          float ls[4], de[4];
+          for (int e = 0; e < 16; ++e) {
+            s[e] = mul2(s[e], both(c));
+            far[e & 1] = max3(far[e & 1], fabsf(s[e].x), fabsf(s[e].y));
+          }
+          near = __all_sync(0xffffffffu, fmaxf(far[0], far[1]) <= 1.f);
+        }
+        // the distance of columns from a row is linear where all lie on one side
+        const float from = (float)(kKeys ? y0 + c0 + shift - x : x + shift - y0 - c0), per = kKeys ? 1.f : -1.f;
+        const bool one_side = kBias && (kKeys ? y0 + c0 + shift >= tile.first + kX || y0 + c0 + 32 + shift <= tile.first
+                                              : tile.first + shift >= y0 + c0 + 32 || tile.first + kX + shift <= y0 + c0);
+        const float2 tilt = both(from + per > 0.f ? -slope2 : slope2);
+        const int meets = meet - y0 - c0, ends = (kKeys ? qs.n : meet) - y0 - c0;
+        uint32_t w[16];
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+          float2 ls[2], de[2];
           if (kKeys) {
-            *reinterpret_cast<float4*>(ls) = *reinterpret_cast<const float4*>(vec + c0 + e);
-            *reinterpret_cast<float4*>(de) = *reinterpret_cast<const float4*>(vec + kY + c0 + e);
+            const float4 l4 = *reinterpret_cast<const float4*>(vec + c0 + 2 * e), d4 = *reinterpret_cast<const float4*>(vec + kY + c0 + 2 * e);
+            ls[0] = make_float2(l4.x, l4.y); ls[1] = make_float2(l4.z, l4.w);
+            de[0] = make_float2(d4.x, d4.y); de[1] = make_float2(d4.z, d4.w);
+          } else {
+            ls[0] = ls[1] = both(lse);
+            de[0] = de[1] = both(delta);
           }
 #pragma unroll
-          for (int f = 0; f < 4; ++f) {
-            const int y = y0 + c0 + e + f;
-            const float lg = kKeys ? ls[f] : lse, dl = kKeys ? de[f] : delta;
-            float arg, slope = 1.f;
+          for (int f = 0; f < 2; ++f) {
+            const int i = e + f;
+            float2 arg, slope;
             if (kCap) {
-              const float t = __fdividef(1.f, 1.f + ex2(s[e + f] * c));       // tanh = 1 - 2 t
-              arg = cap2 - 2.f * cap2 * t - lg;
-              slope = 4.f * t * (1.f - t);
+              const float2 th = near ? tanh_small(s[i]) : make_float2(tanh_any(s[i].x), tanh_any(s[i].y));
+              arg = fma2(th, both(cap2), ls[f]);
+              slope = fma2(mul2(th, both(-1.f)), th, both(1.f));
             } else {
-              arg = fmaf(s[e + f], c, -lg);
+              arg = fma2(s[i], both(c), ls[f]);
             }
-            if (kBias) arg -= slope2 * fabsf((float)(kKeys ? y + shift - x : x + shift - y));
-            float p = ex2(arg);
-            float ds = p * (d[e + f] - dl);
-            if (kCap) ds *= slope;
-            if (masked && !(kKeys ? y >= meet && y < qs.n : y < meet)) p = ds = 0.f;
-            s[e + f] = p;
-            d[e + f] = ds;
+            if (kBias) {
+              const float2 away = make_float2(from + per * (float)(2 * i), from + per * (float)(2 * i + 1));
+              if (one_side) arg = fma2(away, tilt, arg);
+              else arg = make_float2(fmaf(-slope2, fabsf(away.x), arg.x), fmaf(-slope2, fabsf(away.y), arg.y));
+            }
+            float2 p = make_float2(ex2(arg.x), ex2(arg.y));
+            float2 ds = mul2(p, add2(d[i], de[f]));
+            if (kCap) ds = mul2(ds, slope);
+            if (masked) {
+              if (kKeys ? 2 * i < meets || 2 * i >= ends : 2 * i >= ends) p.x = ds.x = 0.f;
+              if (kKeys ? 2 * i + 1 < meets || 2 * i + 1 >= ends : 2 * i + 1 >= ends) p.y = ds.y = 0.f;
+            }
+            s[i] = p;
+            w[i] = pack_bf16(ds.x, ds.y);
           }
         }
-        uint32_t w[16];
+        tmem_st16(tm + kY + c0 / 2, w);
         if (kKeys) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) w[e] = pack_bf16(s[2 * e], s[2 * e + 1]);
+          for (int e = 0; e < 16; ++e) w[e] = pack_bf16(s[e].x, s[e].y);
           tmem_st16(tm + c0 / 2, w);
         }
-#pragma unroll
-        for (int e = 0; e < 16; ++e) w[e] = pack_bf16(d[2 * e], d[2 * e + 1]);
-        tmem_st16(tm + kY + c0 / 2, w);
       }
       tmem_st_wait();
       tc_fence_before();
