@@ -22,7 +22,7 @@ namespace {
 
 using namespace attn;
 
-constexpr int kX = 128, kY = 64;
+constexpr int kX = 128, kY = 64, kHalf = 32;
 
 // kD 128: two stages of s and dp and a warpgroup for each, a block per SM.  kD 64: one stage, two blocks per SM take turns.
 template <int kD>
@@ -31,7 +31,7 @@ struct BwdShape {
   static constexpr int stages = kD == 128 ? 2 : 1;
   static constexpr int slots = kD == 128 ? 4 : 3;
   static constexpr int x_bytes = kX * 128 * chunks, y_bytes = kY * 128 * chunks;      // of one operand
-  static constexpr int soft_warps = 4 * stages;
+  static constexpr int soft_warps = 8 * stages;      // two threads have half of a row's columns each
   static constexpr int threads = 32 * (soft_warps + 2);
   static constexpr int smem = 2 * x_bytes + slots * 2 * y_bytes + 1024;
   static constexpr int acc_col = 2 * kY * stages;
@@ -122,7 +122,7 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
     *s_abort = 0;
     mbar_init(smem_u32(&sh.x), 1);
     for (int s = 0; s < kSlots; ++s) { mbar_init(smem_u32(&sh.full[s]), 1); mbar_init(smem_u32(&sh.empty[s]), 1); }
-    for (int s = 0; s < kStages; ++s) { mbar_init(smem_u32(&sh.score[s]), 1); mbar_init(smem_u32(&sh.weight[s]), kX); }
+    for (int s = 0; s < kStages; ++s) { mbar_init(smem_u32(&sh.score[s]), 1); mbar_init(smem_u32(&sh.weight[s]), 2 * kX); }
     mbar_init(smem_u32(&sh.acc), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -219,7 +219,7 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
     if (!ok) *s_abort = 1;
   } else {
     // ---- p and ds: a row of X per thread, stages in turn
-    const int st = warp >> 2, r = (warp & 3) * 32 + lane;
+    const int st = warp >> 3, c0 = (warp >> 2 & 1) * kHalf, r = (warp & 3) * 32 + lane;
     const int x = tile.first + r;
     const uint32_t tm_row = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t tm = tm_row + st * 2 * kY;
@@ -235,7 +235,7 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
       return i < qs.n ? -(r < kY ? a.lse : a.delta)[y_head(it) * q_rows + q_flat + i] : 0.f;
     };
     if (kKeys) {
-      if (st < steps) next = fetch(st);
+      if (st < steps && c0 == 0) next = fetch(st);
     } else if (x < xs.n) {
       lse = -a.lse[head * q_rows + q_flat + x];
       delta = -a.delta[head * q_rows + q_flat + x];
@@ -246,9 +246,11 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
       float* vec = sh.vec[st][(it / kStages) & 1];
       const float slope2 = kBias ? a.slopes[kKeys ? y_head(it) : head] * kLog2e : 0.f;
       if (kKeys) {
-        vec[r] = next;
-        if (it + kStages < steps) next = fetch(it + kStages);
-        asm volatile("bar.sync %0, 128;" ::"r"(st + 1) : "memory");
+        if (c0 == 0) {
+          vec[r] = next;
+          if (it + kStages < steps) next = fetch(it + kStages);
+        }
+        asm volatile("bar.sync %0, 256;" ::"r"(st + 1) : "memory");
       }
       ok = ok && mbar_wait_warp(smem_u32(&sh.score[st]), (it / kStages) & 1, s_abort);
       if (!ok) {         // the other warps of the stage still count on this one at its barrier
@@ -258,9 +260,7 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
       tc_fence_after();
       const int wide = min(kY, hi - y0);
       const bool masked = kKeys ? y0 < all_lo || y0 + kY > all_hi : y0 + kY > all_hi;
-#pragma unroll
-      for (int c0 = 0; c0 < kY; c0 += 32) {
-        if (c0 >= wide) continue;
+      if (c0 < wide) {
         float2 s[16], d[16];
         tmem_ld32_nowait(tm + c0, reinterpret_cast<uint32_t*>(s));
         tmem_ld32_nowait(tm + kY + c0, reinterpret_cast<uint32_t*>(d));
@@ -340,13 +340,16 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
       const bool mine = r < tile_rows, some = x < xs.n;
       const long long row = tile.rows.first + x;
       const uint32_t acc = tm_row + Shape::acc_col;
-      if (kKeys) {
-        if (st == 0) store_acc(acc, 0, a.D, a.D, mine, some, a.scale, at_out(a.gk, tile.rows.b, row, head));
-        if (st == kStages - 1) store_acc(acc + kD, 0, a.D, a.D, mine, some, 1.f, at_out(a.gv, tile.rows.b, row, head));
-      } else {
-        const int half = kStages == 1 ? a.D : min(a.D, kD / 2);
-        store_acc(acc, st == 0 ? 0 : half, st == 0 ? half : a.D, a.D, mine, some, a.scale, at_out(a.gq, tile.rows.b, row, head));
-      }
+      // each warpgroup stores some columns of a result
+      constexpr int kGroups = 2 * kStages;
+      const int group = warp >> 2;
+      auto store = [&](uint32_t tm_acc, float w, const AttnOperand& to, int of, int n) {
+        const int per = (d16 / 16 + n - 1) / n * 16;
+        store_acc(tm_acc, of * per, min(a.D, (of + 1) * per), a.D, mine, some, w, at_out(to, tile.rows.b, row, head));
+      };
+      if (!kKeys) store(acc, a.scale, a.gq, group, kGroups);
+      else if (group < kStages) store(acc, a.scale, a.gk, group, kStages);
+      else store(acc + kD, 1.f, a.gv, group - kStages, kStages);
     }
   }
 
