@@ -7,12 +7,16 @@
 // of all heads that share them (dk, dv), or owns 128 queries and walks over their keys (dq).  That costs the scores and dp twice,
 // seven products in place of five; sums of dq in memory would need a pass of their own over fp32 rows, and an order.
 //
-// Both kinds of block are one program.  X are the two operands of the 128 rows that it owns, Y those of the 64 rows at a time that
+// Both kinds of block are one program.  X are the two operands of the 128 rows that it owns, Y those of the 128 rows at a time that
 // it walks over: (K, V) and (Q, dO), or (Q, dO) and (K, V).
-//   s = X1 Y1^T, dp = X2 Y2^T  [128, 64];   acc1 += ds Y1;   acc2 += p Y2 (keys' owners only)
-// A row of the block is a thread's, so p and ds are made in registers and go back into the columns of tensor memory that s and dp
-// had, as left operands; the tiles of Y serve as right operands of both kinds of product.  Where keys own the rows, queries are
-// columns, and their lse and delta come through shared memory.
+//   s = X1 Y1^T, dp = X2 Y2^T  [128, 128];   acc1 += ds Y1;   acc2 += p Y2 (keys' owners only)
+// Four threads have a quarter of a row's columns each.  p and ds are made in registers and go back into the columns of tensor memory
+// that each thread's s and dp had, as left operands; the tiles of Y serve as right operands of both kinds of product.  Where keys
+// own the rows, queries are columns, and a warp brings their lse and delta to shared memory.
+//
+// The products of a step are issued in the order  acc2(i) s(i + 1) | acc1(i) dp(i + 1):  p(i) is made while dp(i) is, ds(i) while acc2
+// and the next scores are.  A product of 128 x 64 x 16 takes 62 cycles, one of 128 x 128 x 16 72, so that steps of 64 rows with two
+// buffers of s and dp were bound by their products: 2700 cycles a step at 128 columns (this kind: see the figures below).
 #include <cuda_bf16.h>
 #include "attention_tc.cuh"
 
@@ -22,32 +26,30 @@ namespace {
 
 using namespace attn;
 
-constexpr int kX = 128, kY = 64, kHalf = 32;
+constexpr int kX = 128, kY = 128, kPart = 32, kParts = kY / kPart;      // rows, columns of a step, columns of a thread
 
-// kD 128: two stages of s and dp and a warpgroup for each, a block per SM.  kD 64: one stage, two blocks per SM take turns.
 template <int kD>
 struct BwdShape {
   static constexpr int chunks = kD / 64;
-  static constexpr int stages = kD == 128 ? 2 : 1;
-  static constexpr int slots = kD == 128 ? 4 : 3;
-  static constexpr int x_bytes = kX * 128 * chunks, y_bytes = kY * 128 * chunks;      // of one operand
-  static constexpr int soft_warps = 8 * stages;      // two threads have half of a row's columns each
-  static constexpr int threads = 32 * (soft_warps + 2);
-  static constexpr int smem = 2 * x_bytes + slots * 2 * y_bytes + 1024;
-  static constexpr int acc_col = 2 * kY * stages;
-  static constexpr int tmem_cols = kD == 128 ? 512 : 256;
+  static constexpr int slots = 2;
+  static constexpr int bytes = kX * 128 * chunks;      // of one operand's tile
+  static constexpr int soft_warps = 4 * kParts;
+  static constexpr int threads = 32 * (soft_warps + 3);      // and one each for loads, products, lse and delta
+  static constexpr int smem = 2 * bytes * (1 + slots) + 1024;
+  static constexpr int dp_col = kY, acc_col = 2 * kY;
+  static constexpr int tmem_cols = 512;
 };
 
 struct BwdMaps {
-  CUtensorMap q, k, v, go;      // boxes of 64 rows
+  CUtensorMap q, k, v, go;      // boxes of 128 rows
 };
 
 template <int kD>
 struct BwdShared {
-  uint64_t x, full[BwdShape<kD>::slots], empty[BwdShape<kD>::slots], score[BwdShape<kD>::stages], weight[BwdShape<kD>::stages], acc;
+  uint64_t x, full[2][BwdShape<kD>::slots], empty[2][BwdShape<kD>::slots], score, weight, dp, ds[2], acc, vec_full[2];      // ds by turns: two warps wait for it
   uint32_t tmem;
   int abort;
-  alignas(16) float vec[BwdShape<kD>::stages][2][2 * kY];      // less lse and delta of a tile of queries
+  alignas(16) float vec[2][2][kY];      // of a tile of queries less lse, less delta; two tiles take turns
 };
 
 // A thread's columns [c0, c0 + 16) of an accumulator, times w, to a row of the result; zeros where the row has no terms
@@ -70,7 +72,7 @@ __device__ __forceinline__ void store_acc(uint32_t tm, int from, int to, int D, 
 template <int kD, bool kKeys, bool kCap, bool kBias>
 __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a, BwdShared<kD>& sh, uint8_t* smem_raw, int tile_at, int head) {
   using Shape = BwdShape<kD>;
-  constexpr int kStages = Shape::stages, kSlots = Shape::slots;
+  constexpr int kSlots = Shape::slots;
   volatile int* s_abort = &sh.abort;
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const Tile tile = tile_of(kKeys ? a.rk : a.rq, a.B, kX, tile_at);
@@ -89,7 +91,7 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
   int lo = 0, hi = 0, all_lo = 0, all_hi = 0;
   if (tile.first < xs.n) {
     if (kKeys) {
-      lo = first_query(a, tile.seq, tile.first, qs.n, ks.n) & ~(kY - 1);
+      lo = first_query(a, tile.seq, tile.first, qs.n, ks.n) & ~15;
       hi = qs.n;
       all_lo = first_query(a, tile.seq, last, qs.n, ks.n);
       all_hi = qs.n;
@@ -98,8 +100,7 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
       all_hi = keys_seen(a, tile.seq, tile.first, qs.n, ks.n);
     }
   }
-  const int per_head_ = hi > lo ? (hi - lo + kY - 1) / kY : 0;
-  const int steps_ = per_head_ * (kKeys ? R : 1);
+  const int steps_ = hi > lo ? (hi - lo + kY - 1) / kY * (kKeys ? R : 1) : 0;
   if (steps_ == 0) {
     const int per = a.D / 8;
     for (int i = threadIdx.x; i < tile_rows * per; i += Shape::threads) {
@@ -110,20 +111,21 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
     return;
   }
   // what one lane's loads and products are addressed with is known to be the same for the warp
-  const int steps = one_of_warp(steps_), per_head = one_of_warp(per_head_);
+  const int steps = one_of_warp(steps_);
   lo = one_of_warp(lo);
   hi = one_of_warp(hi);
   const int y_end = one_of_warp(ys.n), y_begin = one_of_warp(ys.first), y_b = one_of_warp(ys.b), x_begin = one_of_warp(xs.first + tile.first);
   head = one_of_warp(head);
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  uint8_t* ring_gen = smem_raw + (base - smem_u32(smem_raw)) + 2 * Shape::x_bytes;
-  const uint32_t ring = base + 2 * Shape::x_bytes;
+  uint8_t* ring_gen = smem_raw + (base - smem_u32(smem_raw)) + 2 * Shape::bytes;
+  const uint32_t ring = base + 2 * Shape::bytes;      // tiles of Y1, then of Y2
   if (threadIdx.x == 0) {
     *s_abort = 0;
     mbar_init(smem_u32(&sh.x), 1);
-    for (int s = 0; s < kSlots; ++s) { mbar_init(smem_u32(&sh.full[s]), 1); mbar_init(smem_u32(&sh.empty[s]), 1); }
-    for (int s = 0; s < kStages; ++s) { mbar_init(smem_u32(&sh.score[s]), 1); mbar_init(smem_u32(&sh.weight[s]), 2 * kX); }
-    mbar_init(smem_u32(&sh.acc), 1);
+    for (int o = 0; o < 2; ++o)
+      for (int s = 0; s < kSlots; ++s) { mbar_init(smem_u32(&sh.full[o][s]), 1); mbar_init(smem_u32(&sh.empty[o][s]), 1); }
+    for (uint64_t* b : {&sh.score, &sh.dp, &sh.acc, &sh.vec_full[0], &sh.vec_full[1]}) mbar_init(smem_u32(b), 1);
+    for (uint64_t* b : {&sh.weight, &sh.ds[0], &sh.ds[1]}) mbar_init(smem_u32(b), kX * kParts);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 0) tmem_alloc<Shape::tmem_cols>(&sh.tmem);
@@ -132,144 +134,176 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
   const int d16 = round16(a.D);
-  auto y_first = [&](int it) { return lo + (kKeys ? it % per_head : it) * kY; };
-  auto y_head = [&](int it) { return kKeys ? head * R + it / per_head : head / R; };
+  const long long q_rows = flat_rows(a.rq, a.B), q_flat = (a.rq.off ? 0 : (long long)qs.b * a.rq.T) + qs.first;
 
   if (warp == Shape::soft_warps) {
-    // ---- loads
+    // ---- loads: Y1 and Y2 of a step, each into a ring of its own
     const bool lead = elect_one();
     if (lead) {
       const uint32_t bar = smem_u32(&sh.x);
-      mbar_expect_tx(bar, 2 * Shape::x_bytes);
+      mbar_expect_tx(bar, 2 * Shape::bytes);
       for (int o = 0; o < 2; ++o)
         for (int c = 0; c < Shape::chunks; ++c)
-          for (int r = 0; r < kX; r += kY)
-            tma_load_4d(base + o * Shape::x_bytes + c * (kX * 128) + r * 128, kKeys ? (o ? &maps.v : &maps.k) : (o ? &maps.go : &maps.q), 64 * c,
-                        x_begin + r, head, xs.b, bar);
+          tma_load_4d(base + o * Shape::bytes + c * (kX * 128), kKeys ? (o ? &maps.v : &maps.k) : (o ? &maps.go : &maps.q), 64 * c, x_begin, head,
+                      xs.b, bar);
     }
     __syncwarp();
-    for (int it = 0; it < steps; ++it) {
+    int y0 = lo, h = kKeys ? head * R : head / R;
+    bool ok = true;
+    for (int it = 0; it < steps && ok; ++it) {
       const int s = it % kSlots;
-      if (it >= kSlots && !mbar_wait_warp(smem_u32(&sh.empty[s]), ((it / kSlots) & 1) ^ 1, s_abort)) { *s_abort = 1; break; }
-      if (lead) {
-        const uint32_t bar = smem_u32(&sh.full[s]), to = ring + s * 2 * Shape::y_bytes;
-        mbar_expect_tx(bar, 2 * Shape::y_bytes);
-        for (int o = 0; o < 2; ++o)
+#pragma unroll
+      for (int o = 0; o < 2; ++o) {
+        ok = ok && (it < kSlots || mbar_wait_warp(smem_u32(&sh.empty[o][s]), ((it / kSlots) & 1) ^ 1, s_abort));
+        if (!ok) { *s_abort = 1; break; }
+        if (lead) {
+          const uint32_t bar = smem_u32(&sh.full[o][s]);
+          mbar_expect_tx(bar, Shape::bytes);
           for (int c = 0; c < Shape::chunks; ++c)
-            tma_load_4d(to + o * Shape::y_bytes + c * (kY * 128), kKeys ? (o ? &maps.go : &maps.q) : (o ? &maps.v : &maps.k), 64 * c,
-                        y_begin + y_first(it), y_head(it), y_b, bar);
+            tma_load_4d(ring + (o * kSlots + s) * Shape::bytes + c * (kY * 128), kKeys ? (o ? &maps.go : &maps.q) : (o ? &maps.v : &maps.k), 64 * c,
+                        y_begin + y0, h, y_b, bar);
+        }
+        __syncwarp();
       }
-      __syncwarp();
+      y0 += kY;
+      if (kKeys && y0 >= hi) { y0 = lo; ++h; }
     }
   } else if (warp == Shape::soft_warps + 1) {
     // ---- products
     const bool lead = elect_one();
     const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
     bool ok = mbar_wait_warp(smem_u32(&sh.x), 0, s_abort);
-    auto scores = [&](int it) {
-      const int s = it % kSlots;
-      ok = ok && mbar_wait_warp(smem_u32(&sh.full[s]), (it / kSlots) & 1, s_abort);
-      if (!ok) return;
+    auto wait = [&](uint64_t& bar, int parity) {
+      ok = ok && mbar_wait_warp(smem_u32(&bar), parity, s_abort);
       tc_fence_after();
-      const int end = y_end - y_first(it);
-      if (end < kY && (end & 15)) {      // rows behind the sequence's end
-        zero_rows<kY>(ring_gen + s * 2 * Shape::y_bytes, Shape::chunks, end, round16(end), lane);
-        zero_rows<kY>(ring_gen + s * 2 * Shape::y_bytes + Shape::y_bytes, Shape::chunks, end, round16(end), lane);
-      }
-      const uint32_t y1 = ring + s * 2 * Shape::y_bytes, y2 = y1 + Shape::y_bytes;
-      const uint32_t to = tm + (it % kStages) * 2 * kY;
-      const uint32_t id = idesc_of(round16(min(kY, hi - y_first(it))), false);
+      return ok;
+    };
+    // X(o) Y(o)^T of step it, whose columns start at row y0 of Y
+    auto outer = [&](int o, int it, int y0, uint64_t& done) {
+      const int s = it % kSlots;
+      if (!wait(sh.full[o][s], (it / kSlots) & 1)) return;
+      const int end = y_end - y0;
+      if (end < kY && (end & 15))      // rows behind the sequence's end
+        zero_rows<kY>(ring_gen + (o * kSlots + s) * Shape::bytes, Shape::chunks, end, round16(end), lane);
+      const uint32_t id = idesc_of(round16(min(kY, hi - y0)), false);
       if (lead) {
-        const uint64_t x1 = make_smem_desc(base, 16u, 1024u), x2 = make_smem_desc(base + Shape::x_bytes, 16u, 1024u);
-        const uint64_t d1 = make_smem_desc(y1, 16u, 1024u), d2 = make_smem_desc(y2, 16u, 1024u);
+        const uint64_t xd = make_smem_desc(base + o * Shape::bytes, 16u, 1024u), yd = make_smem_desc(ring + (o * kSlots + s) * Shape::bytes, 16u, 1024u);
 #pragma unroll
         for (int k = 0; k < kD / 16; ++k)
-          if (k * 16 < d16) umma_f16(to, x1 + step_k<kX>(k), d1 + step_k<kY>(k), id, k > 0);
-#pragma unroll
-        for (int k = 0; k < kD / 16; ++k)
-          if (k * 16 < d16) umma_f16(to + kY, x2 + step_k<kX>(k), d2 + step_k<kY>(k), id, k > 0);
-        umma_commit(smem_u32(&sh.score[it % kStages]));
+          if (k * 16 < d16) umma_f16(tm + o * Shape::dp_col, xd + step_k<kX>(k), yd + step_k<kY>(k), id, k > 0);
+        umma_commit(smem_u32(&done));
       }
       __syncwarp();
     };
-    for (int it = 0; it < kStages && it < steps; ++it) scores(it);
-    for (int it = 0; it < steps && ok; ++it) {
-      const int st = it % kStages, s = it % kSlots;
-      ok = mbar_wait_warp(smem_u32(&sh.weight[st]), (it / kStages) & 1, s_abort);
-      if (!ok) break;
-      tc_fence_after();
-      const uint32_t y1 = ring + s * 2 * Shape::y_bytes, y2 = y1 + Shape::y_bytes;
-      const uint32_t from = tm + st * 2 * kY;
-      const int n = round16(min(kY, hi - y_first(it))) / 16;
+    // acc += left Y(o): left operands lie where s (for p) or dp (for ds) of each thread's columns began
+    auto inner = [&](int o, int it, int y0, uint32_t left, uint32_t acc) {
+      const int n = round16(min(kY, hi - y0)) / 16;
       const uint32_t id = idesc_of(d16, true);
       if (lead) {
-        const uint64_t d1 = make_smem_desc(y1, kY * 128, 1024u), d2 = make_smem_desc(y2, kY * 128, 1024u);
+        const uint64_t yd = make_smem_desc(ring + (o * kSlots + it % kSlots) * Shape::bytes, kY * 128, 1024u);
 #pragma unroll
         for (int k = 0; k < kY / 16; ++k)
-          if (k < n) umma_f16_ts(tm + Shape::acc_col, from + kY + k * 8, d1 + step_mn(k), id, it > 0 || k > 0);
-        if (kKeys)
-#pragma unroll
-          for (int k = 0; k < kY / 16; ++k)
-            if (k < n) umma_f16_ts(tm + Shape::acc_col + kD, from + k * 8, d2 + step_mn(k), id, it > 0 || k > 0);
-        umma_commit(it + 1 == steps ? smem_u32(&sh.acc) : smem_u32(&sh.empty[s]));
+          if (k < n) umma_f16_ts(tm + acc, tm + left + (k / 2) * kPart + (k & 1) * 8, yd + step_mn(k), id, it > 0 || k > 0);
       }
       __syncwarp();
-      if (it + kStages < steps) scores(it + kStages);
+    };
+    auto free_slot = [&](int o, int it) {
+      if (lead && it + kSlots < steps) umma_commit(smem_u32(&sh.empty[o][it % kSlots]));
+      __syncwarp();
+    };
+    int y0 = lo;
+    outer(0, 0, y0, sh.score);
+    outer(1, 0, y0, sh.dp);
+    if (!kKeys) free_slot(1, 0);
+    for (int it = 0; it < steps && ok; ++it) {
+      const bool more = it + 1 < steps;
+      const int next = kKeys && y0 + kY >= hi ? lo : y0 + kY;
+      if (!wait(sh.weight, it & 1)) break;
+      if (kKeys) {
+        inner(1, it, y0, 0, Shape::acc_col + kD);
+        free_slot(1, it);
+      }
+      if (more) outer(0, it + 1, next, sh.score);
+      if (!wait(sh.ds[it & 1], (it >> 1) & 1)) break;
+      inner(0, it, y0, Shape::dp_col, Shape::acc_col);
+      free_slot(0, it);
+      if (more) {
+        outer(1, it + 1, next, sh.dp);
+        if (!kKeys) free_slot(1, it + 1);
+      }
+      y0 = next;
     }
+    if (ok && lead) umma_commit(smem_u32(&sh.acc));
+    __syncwarp();
     if (!ok) *s_abort = 1;
+  } else if (warp == Shape::soft_warps + 2) {
+    // ---- lse and delta of the queries of a step
+    if (kKeys) {
+      int y0 = lo, h = head * R;
+      float l[kY / 32], d[kY / 32];
+      auto fetch = [&]() {
+#pragma unroll
+        for (int e = 0; e < kY / 32; ++e) {
+          const int i = y0 + e * 32 + lane;
+          const long long from = h * q_rows + q_flat + i;
+          l[e] = i < hi ? -a.lse[from] : 0.f;
+          d[e] = i < hi ? -a.delta[from] : 0.f;
+        }
+      };
+      fetch();
+      for (int it = 0; it < steps; ++it) {
+        // step it - 2 has been through with these places
+        if (it >= 2 && !mbar_wait_warp(smem_u32(&sh.ds[it & 1]), ((it >> 1) & 1) ^ 1, s_abort)) { *s_abort = 1; break; }
+#pragma unroll
+        for (int e = 0; e < kY / 32; ++e) {
+          sh.vec[it & 1][0][e * 32 + lane] = l[e];
+          sh.vec[it & 1][1][e * 32 + lane] = d[e];
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh.vec_full[it & 1]));
+        y0 += kY;
+        if (y0 >= hi) { y0 = lo; ++h; }
+        if (it + 1 < steps) fetch();
+      }
+    }
   } else {
-    // ---- p and ds: a row of X per thread, stages in turn
-    const int st = warp >> 3, c0 = (warp >> 2 & 1) * kHalf, r = (warp & 3) * 32 + lane;
+    // ---- p and ds: a quarter of a row of X per thread
+    const int c0 = (warp >> 2) * kPart, r = (warp & 3) * 32 + lane;
     const int x = tile.first + r;
     const uint32_t tm_row = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t tm = tm_row + st * 2 * kY;
+    const uint32_t tm = tm_row + c0;
     const float c = kCap ? a.scale / a.cap : a.scale * kLog2e;
     const float cap2 = a.cap * kLog2e;
-    const long long q_rows = flat_rows(a.rq, a.B), q_flat = (a.rq.off ? 0 : (long long)qs.b * a.rq.T) + qs.first;
     // keys: the queries [meet, qs.n) see this one; queries: keys [0, meet) are seen
     const int meet = x < xs.n ? (kKeys ? first_query(a, tile.seq, x, qs.n, ks.n) : keys_seen(a, tile.seq, x, qs.n, ks.n)) : (kKeys ? lo : hi);
     const int shift = ks.n - qs.n;
-    float lse = 0.f, delta = 0.f, next = 0.f;      // negative
-    auto fetch = [&](int it) {           // less lse (threads 0 to 63) or delta of a query of step `it`
-      const int i = y_first(it) + (r & (kY - 1));
-      return i < qs.n ? -(r < kY ? a.lse : a.delta)[y_head(it) * q_rows + q_flat + i] : 0.f;
-    };
-    if (kKeys) {
-      if (st < steps && c0 == 0) next = fetch(st);
-    } else if (x < xs.n) {
+    float lse = 0.f, delta = 0.f;      // negative
+    if (!kKeys && x < xs.n) {
       lse = -a.lse[head * q_rows + q_flat + x];
       delta = -a.delta[head * q_rows + q_flat + x];
     }
+    int y0 = lo, h = kKeys ? head * R : head;
     bool ok = true;
-    for (int it = st; it < steps; it += kStages) {
-      const int y0 = y_first(it);
-      float* vec = sh.vec[st][(it / kStages) & 1];
-      const float slope2 = kBias ? a.slopes[kKeys ? y_head(it) : head] * kLog2e : 0.f;
-      if (kKeys) {
-        if (c0 == 0) {
-          vec[r] = next;
-          if (it + kStages < steps) next = fetch(it + kStages);
-        }
-        asm volatile("bar.sync %0, 256;" ::"r"(st + 1) : "memory");
-      }
-      ok = ok && mbar_wait_warp(smem_u32(&sh.score[st]), (it / kStages) & 1, s_abort);
-      if (!ok) {         // the other warps of the stage still count on this one at its barrier
-        *s_abort = 1;
-        continue;
-      }
+    for (int it = 0; it < steps; ++it) {
+      const float slope2 = kBias ? a.slopes[h] * kLog2e : 0.f;
+      const float *lse_y = sh.vec[it & 1][0] + c0, *delta_y = sh.vec[it & 1][1] + c0;
+      const bool any = y0 + c0 < hi;                       // columns of this thread's
+      const bool masked = kKeys ? y0 + c0 < all_lo || y0 + c0 + kPart > all_hi : y0 + c0 + kPart > all_hi;
+      const int meets = meet - y0 - c0, ends = (kKeys ? hi : meet) - y0 - c0;
+      if (kKeys) ok = ok && mbar_wait_warp(smem_u32(&sh.vec_full[it & 1]), (it >> 1) & 1, s_abort);
+      ok = ok && mbar_wait_warp(smem_u32(&sh.score), it & 1, s_abort);
+      if (!ok) { *s_abort = 1; break; }
       tc_fence_after();
-      const int wide = min(kY, hi - y0);
-      const bool masked = kKeys ? y0 < all_lo || y0 + kY > all_hi : y0 + kY > all_hi;
-      if (c0 < wide) {
-        float2 s[16], d[16];
-        tmem_ld32_nowait(tm + c0, reinterpret_cast<uint32_t*>(s));
-        tmem_ld32_nowait(tm + kY + c0, reinterpret_cast<uint32_t*>(d));
+      float2 s[kPart / 2];
+      uint32_t w[kPart / 2];
+      if (any) {
+        tmem_ld32_nowait(tm, reinterpret_cast<uint32_t*>(s));
         tmem_ld_wait();
         bool near = true;
         if (kCap) {
           float far[2] = {0.f, 0.f};
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
+          for (int e = 0; e < kPart / 2; ++e) {
             s[e] = mul2(s[e], both(c));
             far[e & 1] = max3(far[e & 1], fabsf(s[e].x), fabsf(s[e].y));
           }
@@ -277,59 +311,64 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
         }
         // the distance of columns from a row is linear where all lie on one side
         const float from = (float)(kKeys ? y0 + c0 + shift - x : x + shift - y0 - c0), per = kKeys ? 1.f : -1.f;
-        const bool one_side = kBias && (kKeys ? y0 + c0 + shift >= tile.first + kX || y0 + c0 + 32 + shift <= tile.first
-                                              : tile.first + shift >= y0 + c0 + 32 || tile.first + kX + shift <= y0 + c0);
+        const bool one_side = kBias && (kKeys ? y0 + c0 + shift >= tile.first + kX || y0 + c0 + kPart + shift <= tile.first
+                                              : tile.first + shift >= y0 + c0 + kPart || tile.first + kX + shift <= y0 + c0);
         const float2 tilt = both(from + per > 0.f ? -slope2 : slope2);
-        const int meets = meet - y0 - c0, ends = (kKeys ? qs.n : meet) - y0 - c0;
-        uint32_t w[16];
 #pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-          float2 ls[2], de[2];
-          if (kKeys) {
-            const float4 l4 = *reinterpret_cast<const float4*>(vec + c0 + 2 * e), d4 = *reinterpret_cast<const float4*>(vec + kY + c0 + 2 * e);
-            ls[0] = make_float2(l4.x, l4.y); ls[1] = make_float2(l4.z, l4.w);
-            de[0] = make_float2(d4.x, d4.y); de[1] = make_float2(d4.z, d4.w);
+        for (int i = 0; i < kPart / 2; ++i) {
+          const float2 ls = kKeys ? *reinterpret_cast<const float2*>(lse_y + 2 * i) : both(lse);
+          float2 arg, slope;
+          if (kCap) {
+            const float2 th = near ? tanh_small(s[i]) : make_float2(tanh_any(s[i].x), tanh_any(s[i].y));
+            arg = fma2(th, both(cap2), ls);
+            slope = fma2(mul2(th, both(-1.f)), th, both(1.f));
           } else {
-            ls[0] = ls[1] = both(lse);
-            de[0] = de[1] = both(delta);
+            arg = fma2(s[i], both(c), ls);
           }
-#pragma unroll
-          for (int f = 0; f < 2; ++f) {
-            const int i = e + f;
-            float2 arg, slope;
-            if (kCap) {
-              const float2 th = near ? tanh_small(s[i]) : make_float2(tanh_any(s[i].x), tanh_any(s[i].y));
-              arg = fma2(th, both(cap2), ls[f]);
-              slope = fma2(mul2(th, both(-1.f)), th, both(1.f));
-            } else {
-              arg = fma2(s[i], both(c), ls[f]);
-            }
-            if (kBias) {
-              const float2 away = make_float2(from + per * (float)(2 * i), from + per * (float)(2 * i + 1));
-              if (one_side) arg = fma2(away, tilt, arg);
-              else arg = make_float2(fmaf(-slope2, fabsf(away.x), arg.x), fmaf(-slope2, fabsf(away.y), arg.y));
-            }
-            float2 p = make_float2(ex2(arg.x), ex2(arg.y));
-            float2 ds = mul2(p, add2(d[i], de[f]));
-            if (kCap) ds = mul2(ds, slope);
-            if (masked) {
-              if (kKeys ? 2 * i < meets || 2 * i >= ends : 2 * i >= ends) p.x = ds.x = 0.f;
-              if (kKeys ? 2 * i + 1 < meets || 2 * i + 1 >= ends : 2 * i + 1 >= ends) p.y = ds.y = 0.f;
-            }
-            s[i] = p;
-            w[i] = pack_bf16(ds.x, ds.y);
+          if (kBias) {
+            const float2 away = make_float2(from + per * (float)(2 * i), from + per * (float)(2 * i + 1));
+            if (one_side) arg = fma2(away, tilt, arg);
+            else arg = make_float2(fmaf(-slope2, fabsf(away.x), arg.x), fmaf(-slope2, fabsf(away.y), arg.y));
           }
+          float2 p = make_float2(ex2(arg.x), ex2(arg.y));
+          if (masked) {
+            if (kKeys ? 2 * i < meets || 2 * i >= ends : 2 * i >= ends) p.x = 0.f;
+            if (kKeys ? 2 * i + 1 < meets || 2 * i + 1 >= ends : 2 * i + 1 >= ends) p.y = 0.f;
+          }
+          if (kKeys) w[i] = pack_bf16(p.x, p.y);
+          s[i] = kCap ? mul2(p, slope) : p;
         }
-        tmem_st16(tm + kY + c0 / 2, w);
         if (kKeys) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) w[e] = pack_bf16(s[e].x, s[e].y);
-          tmem_st16(tm + c0 / 2, w);
+          tmem_st16(tm, w);
+          tmem_st_wait();
         }
       }
-      tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(smem_u32(&sh.weight[st]));
+      mbar_arrive(smem_u32(&sh.weight));      // the scores have been read; keys: p is there
+      ok = mbar_wait_warp(smem_u32(&sh.dp), it & 1, s_abort);
+      if (!ok) { *s_abort = 1; break; }
+      tc_fence_after();
+      if (any) {
+        float2 d[kPart / 2];
+        tmem_ld32_nowait(tm + Shape::dp_col, reinterpret_cast<uint32_t*>(d));
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < kPart / 2; ++i) {
+          const float2 de = kKeys ? *reinterpret_cast<const float2*>(delta_y + 2 * i) : both(delta);
+          float2 ds = mul2(s[i], add2(d[i], de));
+          if (masked) {                         // (what dp is made of there may be anything)
+            if (kKeys ? 2 * i < meets || 2 * i >= ends : 2 * i >= ends) ds.x = 0.f;
+            if (kKeys ? 2 * i + 1 < meets || 2 * i + 1 >= ends : 2 * i + 1 >= ends) ds.y = 0.f;
+          }
+          w[i] = pack_bf16(ds.x, ds.y);
+        }
+        tmem_st16(tm + Shape::dp_col, w);
+        tmem_st_wait();
+      }
+      tc_fence_before();
+      mbar_arrive(smem_u32(&sh.ds[it & 1]));
+      y0 += kY;
+      if (kKeys && y0 >= hi) { y0 = lo; ++h; }
     }
     if (ok) {
       ok = mbar_wait_warp(smem_u32(&sh.acc), 0, s_abort);
@@ -337,19 +376,18 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
       tc_fence_after();
     }
     if (ok) {
+      // each warpgroup stores some columns of a result
       const bool mine = r < tile_rows, some = x < xs.n;
       const long long row = tile.rows.first + x;
       const uint32_t acc = tm_row + Shape::acc_col;
-      // each warpgroup stores some columns of a result
-      constexpr int kGroups = 2 * kStages;
       const int group = warp >> 2;
       auto store = [&](uint32_t tm_acc, float w, const AttnOperand& to, int of, int n) {
         const int per = (d16 / 16 + n - 1) / n * 16;
         store_acc(tm_acc, of * per, min(a.D, (of + 1) * per), a.D, mine, some, w, at_out(to, tile.rows.b, row, head));
       };
-      if (!kKeys) store(acc, a.scale, a.gq, group, kGroups);
-      else if (group < kStages) store(acc, a.scale, a.gk, group, kStages);
-      else store(acc + kD, 1.f, a.gv, group - kStages, kStages);
+      if (!kKeys) store(acc, a.scale, a.gq, group, kParts);
+      else if (group < kParts / 2) store(acc, a.scale, a.gk, group, kParts / 2);
+      else store(acc + kD, 1.f, a.gv, group - kParts / 2, kParts / 2);
     }
   }
 
@@ -366,7 +404,7 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
 // The first key_tiles * G blocks own keys, the others queries.  Early keys are seen by the most queries and late queries see the most
 // keys: those go first.
 template <int kD, bool kCap, bool kBias>
-__global__ void __launch_bounds__(BwdShape<kD>::threads, kD == 128 ? 1 : 2)
+__global__ void __launch_bounds__(BwdShape<kD>::threads, 1)
 attention_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, const __grid_constant__ AttnArgs a, int key_tiles, int query_tiles) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ BwdShared<kD> sh;
@@ -424,8 +462,8 @@ const char* launch_attention_bwd(const AttnArgs& a, cudaStream_t st) {
   cudaError_t e = launch_pdl(attention_delta_kernel, dim3((unsigned)((rows * a.H * lanes + 255) / 256)), dim3(256), 0, st, a, rows, lanes);
   if (e == cudaSuccess && attention_short_takes(a)) return launch_attention_short_bwd(a, st);
   BwdMaps maps;
-  if (!operand_map(a.q, a.D, a.rq, a.B, a.H, kY, &maps.q) || !operand_map(a.k, a.D, a.rk, a.B, a.G, kY, &maps.k) ||
-      !operand_map(a.v, a.D, a.rk, a.B, a.G, kY, &maps.v) || !operand_map(a.go, a.D, a.rq, a.B, a.H, kY, &maps.go))
+  if (!operand_map(a.q, a.D, a.rq, a.B, a.H, kX, &maps.q) || !operand_map(a.k, a.D, a.rk, a.B, a.G, kX, &maps.k) ||
+      !operand_map(a.v, a.D, a.rk, a.B, a.G, kX, &maps.v) || !operand_map(a.go, a.D, a.rq, a.B, a.H, kX, &maps.go))
     return "attention: cuTensorMapEncodeTiled failed";
   if (e == cudaSuccess) e = a.D > 64 ? launch<128>(maps, a, st) : launch<64>(maps, a, st);
   if (e == cudaSuccess) e = cudaGetLastError();
