@@ -37,6 +37,8 @@ struct BwdShape {
   static constexpr int threads = 32 * (soft_warps + 3);      // and one each for loads, products, lse and delta
   static constexpr int smem = 2 * bytes * (1 + slots) + 1024;
   static constexpr int dp_col = kY, acc_col = 2 * kY;
+  static constexpr bool p_apart = kD == 64;            // p has columns of its own, by thread as s
+  static constexpr int p_col = p_apart ? acc_col + 2 * kD : 0;
   static constexpr int tmem_cols = 512;
 };
 
@@ -46,7 +48,7 @@ struct BwdMaps {
 
 template <int kD>
 struct BwdShared {
-  uint64_t x, full[2][BwdShape<kD>::slots], empty[2][BwdShape<kD>::slots], score, weight, dp, ds[2], acc, vec_full[2];      // ds by turns: two warps wait for it
+  uint64_t x, full[2][BwdShape<kD>::slots], empty[2][BwdShape<kD>::slots], score, read, weight, used, dp, ds[2], acc, vec_full[2];      // ds by turns: two warps wait for it
   uint32_t tmem;
   int abort;
   alignas(16) float vec[2][2][kY];      // of a tile of queries less lse, less delta; two tiles take turns
@@ -73,6 +75,7 @@ template <int kD, bool kKeys, bool kCap, bool kBias>
 __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a, BwdShared<kD>& sh, uint8_t* smem_raw, int tile_at, int head) {
   using Shape = BwdShape<kD>;
   constexpr int kSlots = Shape::slots;
+  constexpr bool kEarly = !kKeys || Shape::p_apart;      // the next scores need not wait for what is made of these
   volatile int* s_abort = &sh.abort;
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const Tile tile = tile_of(kKeys ? a.rk : a.rq, a.B, kX, tile_at);
@@ -124,8 +127,8 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
     mbar_init(smem_u32(&sh.x), 1);
     for (int o = 0; o < 2; ++o)
       for (int s = 0; s < kSlots; ++s) { mbar_init(smem_u32(&sh.full[o][s]), 1); mbar_init(smem_u32(&sh.empty[o][s]), 1); }
-    for (uint64_t* b : {&sh.score, &sh.dp, &sh.acc, &sh.vec_full[0], &sh.vec_full[1]}) mbar_init(smem_u32(b), 1);
-    for (uint64_t* b : {&sh.weight, &sh.ds[0], &sh.ds[1]}) mbar_init(smem_u32(b), kX * kParts);
+    for (uint64_t* b : {&sh.score, &sh.used, &sh.dp, &sh.acc, &sh.vec_full[0], &sh.vec_full[1]}) mbar_init(smem_u32(b), 1);
+    for (uint64_t* b : {&sh.read, &sh.weight, &sh.ds[0], &sh.ds[1]}) mbar_init(smem_u32(b), kX * kParts);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 0) tmem_alloc<Shape::tmem_cols>(&sh.tmem);
@@ -218,12 +221,17 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
     for (int it = 0; it < steps && ok; ++it) {
       const bool more = it + 1 < steps;
       const int next = kKeys && y0 + kY >= hi ? lo : y0 + kY;
-      if (!wait(sh.weight, it & 1)) break;
+      if (kEarly) {
+        if (!wait(sh.read, it & 1)) break;
+        if (more) outer(0, it + 1, next, sh.score);
+      }
       if (kKeys) {
-        inner(1, it, y0, 0, Shape::acc_col + kD);
+        if (!wait(sh.weight, it & 1)) break;
+        inner(1, it, y0, Shape::p_col, Shape::acc_col + kD);
+        if (Shape::p_apart && lead) umma_commit(smem_u32(&sh.used));
         free_slot(1, it);
       }
-      if (more) outer(0, it + 1, next, sh.score);
+      if (!kEarly && more) outer(0, it + 1, next, sh.score);
       if (!wait(sh.ds[it & 1], (it >> 1) & 1)) break;
       inner(0, it, y0, Shape::dp_col, Shape::acc_col);
       free_slot(0, it);
@@ -296,9 +304,16 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
       tc_fence_after();
       float2 s[kPart / 2];
       uint32_t w[kPart / 2];
+      float4 y4;
       if (any) {
         tmem_ld32_nowait(tm, reinterpret_cast<uint32_t*>(s));
         tmem_ld_wait();
+      }
+      if (kEarly) {
+        tc_fence_before();
+        mbar_arrive(smem_u32(&sh.read));
+      }
+      if (any) {
         bool near = true;
         if (kCap) {
           float far[2] = {0.f, 0.f};
@@ -316,7 +331,8 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
         const float2 tilt = both(from + per > 0.f ? -slope2 : slope2);
 #pragma unroll
         for (int i = 0; i < kPart / 2; ++i) {
-          const float2 ls = kKeys ? *reinterpret_cast<const float2*>(lse_y + 2 * i) : both(lse);
+          if (kKeys && i % 2 == 0) y4 = *reinterpret_cast<const float4*>(lse_y + 2 * i);
+          const float2 ls = !kKeys ? both(lse) : i % 2 == 0 ? make_float2(y4.x, y4.y) : make_float2(y4.z, y4.w);
           float2 arg, slope;
           if (kCap) {
             const float2 th = near ? tanh_small(s[i]) : make_float2(tanh_any(s[i].x), tanh_any(s[i].y));
@@ -338,14 +354,20 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
           if (kKeys) w[i] = pack_bf16(p.x, p.y);
           s[i] = kCap ? mul2(p, slope) : p;
         }
-        if (kKeys) {
-          tmem_st16(tm, w);
+      }
+      if (kKeys) {
+        // The last p has been used; where s had it, the scores of this step say as much.  All warps wait, those without columns too: one
+        // that did not could come by a second time before another has come by once.
+        if (Shape::p_apart && it > 0) ok = mbar_wait_warp(smem_u32(&sh.used), (it - 1) & 1, s_abort);
+        tc_fence_after();
+        if (any) {
+          tmem_st16(tm + Shape::p_col, w);
           tmem_st_wait();
         }
+        tc_fence_before();
+        mbar_arrive(smem_u32(&sh.weight));
       }
-      tc_fence_before();
-      mbar_arrive(smem_u32(&sh.weight));      // the scores have been read; keys: p is there
-      ok = mbar_wait_warp(smem_u32(&sh.dp), it & 1, s_abort);
+      ok = ok && mbar_wait_warp(smem_u32(&sh.dp), it & 1, s_abort);
       if (!ok) { *s_abort = 1; break; }
       tc_fence_after();
       if (any) {
@@ -354,7 +376,8 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
         tmem_ld_wait();
 #pragma unroll
         for (int i = 0; i < kPart / 2; ++i) {
-          const float2 de = kKeys ? *reinterpret_cast<const float2*>(delta_y + 2 * i) : both(delta);
+          if (kKeys && i % 2 == 0) y4 = *reinterpret_cast<const float4*>(delta_y + 2 * i);
+          const float2 de = !kKeys ? both(delta) : i % 2 == 0 ? make_float2(y4.x, y4.y) : make_float2(y4.z, y4.w);
           float2 ds = mul2(s[i], add2(d[i], de));
           if (masked) {                         // (what dp is made of there may be anything)
             if (kKeys ? 2 * i < meets || 2 * i >= ends : 2 * i >= ends) ds.x = 0.f;
