@@ -7,16 +7,22 @@
 // of all heads that share them (dk, dv), or owns 128 queries and walks over their keys (dq).  That costs the scores and dp twice,
 // seven products in place of five; sums of dq in memory would need a pass of their own over fp32 rows, and an order.
 //
-// Both kinds of block are one program.  X are the two operands of the 128 rows that it owns, Y those of the 128 rows at a time that
-// it walks over: (K, V) and (Q, dO), or (Q, dO) and (K, V).
-//   s = X1 Y1^T, dp = X2 Y2^T  [128, 128];   acc1 += ds Y1;   acc2 += p Y2 (keys' owners only)
-// Four threads have a quarter of a row's columns each.  p and ds are made in registers and go back into the columns of tensor memory
-// that each thread's s and dp had, as left operands; the tiles of Y serve as right operands of both kinds of product.  Where keys
-// own the rows, queries are columns, and a warp brings their lse and delta to shared memory.
+// Both kinds of block are one program.  X are the two operands of the 128 rows that it owns, Y those of the 128 or 64 rows at a time
+// that it walks over: (K, V) and (Q, dO), or (Q, dO) and (K, V).
+//   s = X1 Y1^T, dp = X2 Y2^T;   acc1 += ds Y1;   acc2 += p Y2 (keys' owners only)
+// A thread has 32 columns of a row.  p and ds are made in registers and go back into the columns of tensor memory that the thread's s
+// and dp had, as left operands; the tiles of Y serve as right operands of both kinds of product.  Where keys own the rows, queries
+// are columns, and the loading warp brings their lse and delta to shared memory.
 //
 // The products of a step are issued in the order  acc2(i) s(i + 1) | acc1(i) dp(i + 1):  p(i) is made while dp(i) is, ds(i) while acc2
-// and the next scores are.  A product of 128 x 64 x 16 takes 62 cycles, one of 128 x 128 x 16 72, so that steps of 64 rows with two
-// buffers of s and dp were bound by their products: 2700 cycles a step at 128 columns (this kind: see the figures below).
+// and the next scores are.
+//
+// What bounds it above 64 columns: a step of 128 x 128 takes 3300 cycles where keys are owned, of which its four products take 2300 and
+// p and ds 2400, partly beside them; and 2800 where queries are.  A product of 128 x 64 x 16 takes 62 cycles, one of 128 x 128 x 16
+// 72, so that steps of 64 rows with two buffers of s and dp were bound by their products.  8192 tokens x 16 heads x 128 columns
+// causal, us: steps of 64 with a row per thread 980, half a row 917, steps of 128 as they are 845; capped 1607, 1209, 1060.
+// Up to 64 columns the blocks of short sequences spend their time on setting up, and two per SM hide that from each other: 1562
+// sequences of 128, 4 heads x 64 causal, 635 us, with one block per SM and steps of 128 rows 846; documents of 60 to 8000, 944 and 1010.
 #include <cuda_bf16.h>
 #include "attention_tc.cuh"
 
@@ -26,32 +32,33 @@ namespace {
 
 using namespace attn;
 
-constexpr int kX = 128, kY = 128, kPart = 32, kParts = kY / kPart;      // rows, columns of a step, columns of a thread
+constexpr int kX = 128, kPart = 32;      // rows, columns of a thread
 
+// Above 64 columns a block per SM takes steps of 128 rows of Y; up to 64, two blocks per SM take steps of 64.
 template <int kD>
 struct BwdShape {
   static constexpr int chunks = kD / 64;
-  static constexpr int slots = 2;
-  static constexpr int bytes = kX * 128 * chunks;      // of one operand's tile
-  static constexpr int soft_warps = 4 * kParts;
-  static constexpr int threads = 32 * (soft_warps + 3);      // and one each for loads, products, lse and delta
-  static constexpr int smem = 2 * bytes * (1 + slots) + 1024;
-  static constexpr int dp_col = kY, acc_col = 2 * kY;
-  static constexpr bool p_apart = kD == 64;            // p has columns of its own, by thread as s
-  static constexpr int p_col = p_apart ? acc_col + 2 * kD : 0;
-  static constexpr int tmem_cols = 512;
+  static constexpr int y = kD == 128 ? 128 : 64, parts = y / kPart;
+  static constexpr int slots = kD == 128 ? 2 : 3;
+  static constexpr int x_bytes = kX * 128 * chunks, y_bytes = y * 128 * chunks;      // of one operand's tile
+  static constexpr int soft_warps = 4 * parts;
+  static constexpr int threads = 32 * (soft_warps + 2);
+  static constexpr int smem = 2 * x_bytes + 2 * slots * y_bytes + 1024;
+  static constexpr int dp_col = y, acc_col = 2 * y;
+  static constexpr int tmem_cols = kD == 128 ? 512 : 256;
+  static_assert(acc_col + 2 * kD <= tmem_cols, "s, dp and two results");
 };
 
 struct BwdMaps {
-  CUtensorMap q, k, v, go;      // boxes of 128 rows
+  CUtensorMap q, k, v, go;      // boxes of a step's rows
 };
 
 template <int kD>
 struct BwdShared {
-  uint64_t x, full[2][BwdShape<kD>::slots], empty[2][BwdShape<kD>::slots], score, read, weight, used, dp, ds[2], acc, vec_full[2];      // ds by turns: two warps wait for it
+  uint64_t x, full[2][BwdShape<kD>::slots], empty[2][BwdShape<kD>::slots], score, read, weight, dp, ds[2], acc, vec_full[2];      // ds by turns: two warps wait for it
   uint32_t tmem;
   int abort;
-  alignas(16) float vec[2][2][kY];      // of a tile of queries less lse, less delta; two tiles take turns
+  alignas(16) float vec[2][2][BwdShape<kD>::y];      // of a tile of queries less lse, less delta; two tiles take turns
 };
 
 // A thread's columns [c0, c0 + 16) of an accumulator, times w, to a row of the result; zeros where the row has no terms
@@ -74,8 +81,7 @@ __device__ __forceinline__ void store_acc(uint32_t tm, int from, int to, int D, 
 template <int kD, bool kKeys, bool kCap, bool kBias>
 __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a, BwdShared<kD>& sh, uint8_t* smem_raw, int tile_at, int head) {
   using Shape = BwdShape<kD>;
-  constexpr int kSlots = Shape::slots;
-  constexpr bool kEarly = !kKeys || Shape::p_apart;      // the next scores need not wait for what is made of these
+  constexpr int kSlots = Shape::slots, kY = Shape::y, kParts = Shape::parts;
   volatile int* s_abort = &sh.abort;
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const Tile tile = tile_of(kKeys ? a.rk : a.rq, a.B, kX, tile_at);
@@ -120,14 +126,14 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
   const int y_end = one_of_warp(ys.n), y_begin = one_of_warp(ys.first), y_b = one_of_warp(ys.b), x_begin = one_of_warp(xs.first + tile.first);
   head = one_of_warp(head);
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  uint8_t* ring_gen = smem_raw + (base - smem_u32(smem_raw)) + 2 * Shape::bytes;
-  const uint32_t ring = base + 2 * Shape::bytes;      // tiles of Y1, then of Y2
+  uint8_t* ring_gen = smem_raw + (base - smem_u32(smem_raw)) + 2 * Shape::x_bytes;
+  const uint32_t ring = base + 2 * Shape::x_bytes;      // tiles of Y1, then of Y2
   if (threadIdx.x == 0) {
     *s_abort = 0;
     mbar_init(smem_u32(&sh.x), 1);
     for (int o = 0; o < 2; ++o)
       for (int s = 0; s < kSlots; ++s) { mbar_init(smem_u32(&sh.full[o][s]), 1); mbar_init(smem_u32(&sh.empty[o][s]), 1); }
-    for (uint64_t* b : {&sh.score, &sh.used, &sh.dp, &sh.acc, &sh.vec_full[0], &sh.vec_full[1]}) mbar_init(smem_u32(b), 1);
+    for (uint64_t* b : {&sh.score, &sh.dp, &sh.acc, &sh.vec_full[0], &sh.vec_full[1]}) mbar_init(smem_u32(b), 1);
     for (uint64_t* b : {&sh.read, &sh.weight, &sh.ds[0], &sh.ds[1]}) mbar_init(smem_u32(b), kX * kParts);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -140,19 +146,31 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
   const long long q_rows = flat_rows(a.rq, a.B), q_flat = (a.rq.off ? 0 : (long long)qs.b * a.rq.T) + qs.first;
 
   if (warp == Shape::soft_warps) {
-    // ---- loads: Y1 and Y2 of a step, each into a ring of its own
+    // ---- loads: Y1 and Y2 of a step, each into a ring of its own, and where queries are columns their lse and delta
     const bool lead = elect_one();
     if (lead) {
       const uint32_t bar = smem_u32(&sh.x);
-      mbar_expect_tx(bar, 2 * Shape::bytes);
+      mbar_expect_tx(bar, 2 * Shape::x_bytes);
       for (int o = 0; o < 2; ++o)
         for (int c = 0; c < Shape::chunks; ++c)
-          tma_load_4d(base + o * Shape::bytes + c * (kX * 128), kKeys ? (o ? &maps.v : &maps.k) : (o ? &maps.go : &maps.q), 64 * c, x_begin, head,
-                      xs.b, bar);
+          for (int r = 0; r < kX; r += kY)
+            tma_load_4d(base + o * Shape::x_bytes + c * (kX * 128) + r * 128, kKeys ? (o ? &maps.v : &maps.k) : (o ? &maps.go : &maps.q), 64 * c,
+                        x_begin + r, head, xs.b, bar);
     }
     __syncwarp();
     int y0 = lo, h = kKeys ? head * R : head / R;
     bool ok = true;
+    float l[kY / 32], d[kY / 32];
+    auto fetch = [&]() {
+#pragma unroll
+      for (int e = 0; e < kY / 32; ++e) {
+        const int i = y0 + e * 32 + lane;
+        const long long from = h * q_rows + q_flat + i;
+        l[e] = i < hi ? -a.lse[from] : 0.f;
+        d[e] = i < hi ? -a.delta[from] : 0.f;
+      }
+    };
+    if (kKeys) fetch();
     for (int it = 0; it < steps && ok; ++it) {
       const int s = it % kSlots;
 #pragma unroll
@@ -161,15 +179,28 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
         if (!ok) { *s_abort = 1; break; }
         if (lead) {
           const uint32_t bar = smem_u32(&sh.full[o][s]);
-          mbar_expect_tx(bar, Shape::bytes);
+          mbar_expect_tx(bar, Shape::y_bytes);
           for (int c = 0; c < Shape::chunks; ++c)
-            tma_load_4d(ring + (o * kSlots + s) * Shape::bytes + c * (kY * 128), kKeys ? (o ? &maps.go : &maps.q) : (o ? &maps.v : &maps.k), 64 * c,
+            tma_load_4d(ring + (o * kSlots + s) * Shape::y_bytes + c * (kY * 128), kKeys ? (o ? &maps.go : &maps.q) : (o ? &maps.v : &maps.k), 64 * c,
                         y_begin + y0, h, y_b, bar);
         }
         __syncwarp();
       }
+      if (kKeys) {
+        // step it - 2 has been through with these places
+        ok = ok && (it < 2 || mbar_wait_warp(smem_u32(&sh.ds[it & 1]), ((it >> 1) & 1) ^ 1, s_abort));
+        if (!ok) *s_abort = 1;
+#pragma unroll
+        for (int e = 0; e < kY / 32; ++e) {
+          sh.vec[it & 1][0][e * 32 + lane] = l[e];
+          sh.vec[it & 1][1][e * 32 + lane] = d[e];
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh.vec_full[it & 1]));
+      }
       y0 += kY;
       if (kKeys && y0 >= hi) { y0 = lo; ++h; }
+      if (kKeys && it + 1 < steps) fetch();
     }
   } else if (warp == Shape::soft_warps + 1) {
     // ---- products
@@ -187,10 +218,10 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
       if (!wait(sh.full[o][s], (it / kSlots) & 1)) return;
       const int end = y_end - y0;
       if (end < kY && (end & 15))      // rows behind the sequence's end
-        zero_rows<kY>(ring_gen + (o * kSlots + s) * Shape::bytes, Shape::chunks, end, round16(end), lane);
+        zero_rows<kY>(ring_gen + (o * kSlots + s) * Shape::y_bytes, Shape::chunks, end, round16(end), lane);
       const uint32_t id = idesc_of(round16(min(kY, hi - y0)), false);
       if (lead) {
-        const uint64_t xd = make_smem_desc(base + o * Shape::bytes, 16u, 1024u), yd = make_smem_desc(ring + (o * kSlots + s) * Shape::bytes, 16u, 1024u);
+        const uint64_t xd = make_smem_desc(base + o * Shape::x_bytes, 16u, 1024u), yd = make_smem_desc(ring + (o * kSlots + s) * Shape::y_bytes, 16u, 1024u);
 #pragma unroll
         for (int k = 0; k < kD / 16; ++k)
           if (k * 16 < d16) umma_f16(tm + o * Shape::dp_col, xd + step_k<kX>(k), yd + step_k<kY>(k), id, k > 0);
@@ -203,7 +234,7 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
       const int n = round16(min(kY, hi - y0)) / 16;
       const uint32_t id = idesc_of(d16, true);
       if (lead) {
-        const uint64_t yd = make_smem_desc(ring + (o * kSlots + it % kSlots) * Shape::bytes, kY * 128, 1024u);
+        const uint64_t yd = make_smem_desc(ring + (o * kSlots + it % kSlots) * Shape::y_bytes, kY * 128, 1024u);
 #pragma unroll
         for (int k = 0; k < kY / 16; ++k)
           if (k < n) umma_f16_ts(tm + acc, tm + left + (k / 2) * kPart + (k & 1) * 8, yd + step_mn(k), id, it > 0 || k > 0);
@@ -221,17 +252,12 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
     for (int it = 0; it < steps && ok; ++it) {
       const bool more = it + 1 < steps;
       const int next = kKeys && y0 + kY >= hi ? lo : y0 + kY;
-      if (kEarly) {
-        if (!wait(sh.read, it & 1)) break;
-        if (more) outer(0, it + 1, next, sh.score);
-      }
+      if (!wait(kKeys ? sh.weight : sh.read, it & 1)) break;
       if (kKeys) {
-        if (!wait(sh.weight, it & 1)) break;
-        inner(1, it, y0, Shape::p_col, Shape::acc_col + kD);
-        if (Shape::p_apart && lead) umma_commit(smem_u32(&sh.used));
+        inner(1, it, y0, 0, Shape::acc_col + kD);
         free_slot(1, it);
       }
-      if (!kEarly && more) outer(0, it + 1, next, sh.score);
+      if (more) outer(0, it + 1, next, sh.score);
       if (!wait(sh.ds[it & 1], (it >> 1) & 1)) break;
       inner(0, it, y0, Shape::dp_col, Shape::acc_col);
       free_slot(0, it);
@@ -244,38 +270,8 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
     if (ok && lead) umma_commit(smem_u32(&sh.acc));
     __syncwarp();
     if (!ok) *s_abort = 1;
-  } else if (warp == Shape::soft_warps + 2) {
-    // ---- lse and delta of the queries of a step
-    if (kKeys) {
-      int y0 = lo, h = head * R;
-      float l[kY / 32], d[kY / 32];
-      auto fetch = [&]() {
-#pragma unroll
-        for (int e = 0; e < kY / 32; ++e) {
-          const int i = y0 + e * 32 + lane;
-          const long long from = h * q_rows + q_flat + i;
-          l[e] = i < hi ? -a.lse[from] : 0.f;
-          d[e] = i < hi ? -a.delta[from] : 0.f;
-        }
-      };
-      fetch();
-      for (int it = 0; it < steps; ++it) {
-        // step it - 2 has been through with these places
-        if (it >= 2 && !mbar_wait_warp(smem_u32(&sh.ds[it & 1]), ((it >> 1) & 1) ^ 1, s_abort)) { *s_abort = 1; break; }
-#pragma unroll
-        for (int e = 0; e < kY / 32; ++e) {
-          sh.vec[it & 1][0][e * 32 + lane] = l[e];
-          sh.vec[it & 1][1][e * 32 + lane] = d[e];
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sh.vec_full[it & 1]));
-        y0 += kY;
-        if (y0 >= hi) { y0 = lo; ++h; }
-        if (it + 1 < steps) fetch();
-      }
-    }
   } else {
-    // ---- p and ds: a quarter of a row of X per thread
+    // ---- p and ds: 32 columns of a row of X per thread
     const int c0 = (warp >> 2) * kPart, r = (warp & 3) * 32 + lane;
     const int x = tile.first + r;
     const uint32_t tm_row = tmem + ((uint32_t)((warp & 3) * 32) << 16);
@@ -309,7 +305,7 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
         tmem_ld32_nowait(tm, reinterpret_cast<uint32_t*>(s));
         tmem_ld_wait();
       }
-      if (kEarly) {
+      if (!kKeys) {      // the next scores need not wait for what is made of these
         tc_fence_before();
         mbar_arrive(smem_u32(&sh.read));
       }
@@ -356,12 +352,8 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
         }
       }
       if (kKeys) {
-        // The last p has been used; where s had it, the scores of this step say as much.  All warps wait, those without columns too: one
-        // that did not could come by a second time before another has come by once.
-        if (Shape::p_apart && it > 0) ok = mbar_wait_warp(smem_u32(&sh.used), (it - 1) & 1, s_abort);
-        tc_fence_after();
         if (any) {
-          tmem_st16(tm + Shape::p_col, w);
+          tmem_st16(tm, w);
           tmem_st_wait();
         }
         tc_fence_before();
@@ -427,7 +419,7 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
 // The first key_tiles * G blocks own keys, the others queries.  Early keys are seen by the most queries and late queries see the most
 // keys: those go first.
 template <int kD, bool kCap, bool kBias>
-__global__ void __launch_bounds__(BwdShape<kD>::threads, 1)
+__global__ void __launch_bounds__(BwdShape<kD>::threads, kD == 128 ? 1 : 2)
 attention_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, const __grid_constant__ AttnArgs a, int key_tiles, int query_tiles) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ BwdShared<kD> sh;
@@ -485,8 +477,9 @@ const char* launch_attention_bwd(const AttnArgs& a, cudaStream_t st) {
   cudaError_t e = launch_pdl(attention_delta_kernel, dim3((unsigned)((rows * a.H * lanes + 255) / 256)), dim3(256), 0, st, a, rows, lanes);
   if (e == cudaSuccess && attention_short_takes(a)) return launch_attention_short_bwd(a, st);
   BwdMaps maps;
-  if (!operand_map(a.q, a.D, a.rq, a.B, a.H, kX, &maps.q) || !operand_map(a.k, a.D, a.rk, a.B, a.G, kX, &maps.k) ||
-      !operand_map(a.v, a.D, a.rk, a.B, a.G, kX, &maps.v) || !operand_map(a.go, a.D, a.rq, a.B, a.H, kX, &maps.go))
+  const int box = a.D > 64 ? BwdShape<128>::y : BwdShape<64>::y;
+  if (!operand_map(a.q, a.D, a.rq, a.B, a.H, box, &maps.q) || !operand_map(a.k, a.D, a.rk, a.B, a.G, box, &maps.k) ||
+      !operand_map(a.v, a.D, a.rk, a.B, a.G, box, &maps.v) || !operand_map(a.go, a.D, a.rq, a.B, a.H, box, &maps.go))
     return "attention: cuTensorMapEncodeTiled failed";
   if (e == cudaSuccess) e = a.D > 64 ? launch<128>(maps, a, st) : launch<64>(maps, a, st);
   if (e == cudaSuccess) e = cudaGetLastError();
