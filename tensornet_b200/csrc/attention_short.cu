@@ -16,35 +16,54 @@ using namespace attn;
 
 constexpr int kWarps = 4, kM = 16;
 
-// Right operands of 16 rows from `first` on, n of them there, straight from memory
+// Right operands of 16 rows at a time, straight from memory.  The lane keeps its place in the rows and moves on by 16 of them.
 template <int kD>
-__device__ __forceinline__ void score_words(const __nv_bfloat16* base, long long st, int first, int n, int D, int g, int t,
-                                            uint32_t (*w)[Pieces<kD>::k_all]) {
+struct ScoreRows {      // rows as columns of the product
   using P = Pieces<kD>;
+  const __nv_bfloat16* p;
+  int left;             // rows behind the lane's first one, itself included
+  bool there[P::k_pieces];
+  __device__ __forceinline__ ScoreRows(const AttnOperand& o, int b, int first, int h, int from, int n, int D, int g, int t)
+      : p(at(o, b, first + from + g, h) + t * 2 * P::k_words), left(n - from - g) {
 #pragma unroll
-  for (int c = 0; c < 2; ++c)
+    for (int i = 0; i < P::k_pieces; ++i) there[i] = (i * 4 + t) * 2 * P::k_words < D;
+  }
+  __device__ __forceinline__ void load(long long st, uint32_t (*w)[P::k_all]) const {
 #pragma unroll
-    for (int p = 0; p < P::k_pieces; ++p) {
-      const int y = first + 8 * c + g, d = (p * 4 + t) * 2 * P::k_words;
+    for (int c = 0; c < 2; ++c)
 #pragma unroll
-      for (int i = 0; i < P::k_words; ++i) w[c][p * P::k_words + i] = 0u;
-      if (y < n && d < D) load_words<P::k_words>(base + y * st + d, &w[c][p * P::k_words]);
-    }
-}
+      for (int i = 0; i < P::k_pieces; ++i) {
+#pragma unroll
+        for (int k = 0; k < P::k_words; ++k) w[c][i * P::k_words + k] = 0u;
+        if (8 * c < left && there[i]) load_words<P::k_words>(p + 8 * c * st + i * 8 * P::k_words, &w[c][i * P::k_words]);
+      }
+  }
+  __device__ __forceinline__ void next(long long st) { p += 16 * st; left -= 16; }
+};
 template <int kD>
-__device__ __forceinline__ void value_words(const __nv_bfloat16* base, long long st, int first, int n, int D, int g, int t,
-                                            uint32_t (*w)[4][Pieces<kD>::v_words]) {
+struct ValueRows {      // rows as the contraction
   using P = Pieces<kD>;
+  const __nv_bfloat16* p;
+  int left;
+  bool there[P::v_pieces];
+  __device__ __forceinline__ ValueRows(const AttnOperand& o, int b, int first, int h, int from, int n, int D, int g, int t)
+      : p(at(o, b, first + from + 2 * t, h) + g * P::v_cols), left(n - from - 2 * t) {
 #pragma unroll
-  for (int p = 0; p < P::v_pieces; ++p)
+    for (int i = 0; i < P::v_pieces; ++i) there[i] = (i * 8 + g) * P::v_cols < D;
+  }
+  __device__ __forceinline__ void load(long long st, uint32_t (*w)[4][P::v_words]) const {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int y = first + 2 * t + (e & 1) + 8 * (e >> 1), d = (p * 8 + g) * P::v_cols;
+    for (int i = 0; i < P::v_pieces; ++i)
 #pragma unroll
-      for (int i = 0; i < P::v_words; ++i) w[p][e][i] = 0u;
-      if (y < n && d < D) load_words<P::v_words>(base + y * st + d, w[p][e]);
-    }
-}
+      for (int e = 0; e < 4; ++e) {
+        const int row = (e & 1) + 8 * (e >> 1);
+#pragma unroll
+        for (int k = 0; k < P::v_words; ++k) w[i][e][k] = 0u;
+        if (row < left && there[i]) load_words<P::v_words>(p + row * st + i * 8 * P::v_cols, w[i][e]);
+      }
+  }
+  __device__ __forceinline__ void next(long long st) { p += 16 * st; left -= 16; }
+};
 // Left operand: the words of rows g and g + 8
 template <int kD>
 __device__ __forceinline__ void row_words(const __nv_bfloat16* base, long long st, int first, int n, int D, int g, int t, uint32_t (*w)[2]) {
@@ -102,102 +121,128 @@ __device__ __forceinline__ void store_rows(const AttnOperand& to, int b, long lo
   }
 }
 
-template <int kD>
-__global__ void __launch_bounds__(32 * kWarps) attention_short_fwd_kernel(const __grid_constant__ AttnArgs a, int tiles) {
+// A warp takes `heads` heads of its tile, one after another.
+template <int kD, bool kCap, bool kBias>
+__global__ void __launch_bounds__(32 * kWarps, kD == 16 ? 6 : kD == 32 ? 4 : 3) attention_short_fwd_kernel(const __grid_constant__ AttnArgs a, unsigned tiles, unsigned heads) {
   using P = Pieces<kD>;
   pdl_sync();
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const long long unit = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
-  if (unit >= (long long)tiles * a.H) return;
-  const int h = (int)(unit % a.H), kh = h / (a.H / a.G);
-  const Tile tile = tile_of(a.rq, a.B, kM, (int)(unit / a.H));
+  const unsigned unit = blockIdx.x * kWarps + (threadIdx.x >> 5), groups = ((unsigned)a.H + heads - 1) / heads;
+  const unsigned tile_at = unit / groups;
+  if (tile_at >= tiles) return;
+  const int h0 = (unit - tile_at * groups) * heads, h1 = min(a.H, h0 + (int)heads), R = a.H / a.G;
+  const Tile tile = tile_of(a.rq, a.B, kM, (int)tile_at);
   if (!tile.any) return;
   Span qs{tile.rows.b, tile.rows.first, 0}, ks{0, 0, 0};
   if (tile.seq >= 0) {
     qs = span_of(a.rq, tile.seq);
     ks = span_of(a.rk, tile.seq);
   }
-  const int x0 = tile.first;
-  int lim[2];
-#pragma unroll
-  for (int e = 0; e < 2; ++e) lim[e] = x0 + g + 8 * e < qs.n ? keys_seen(a, tile.seq, x0 + g + 8 * e, qs.n, ks.n) : 0;
-  const int vis = x0 < qs.n ? keys_seen(a, tile.seq, min(x0 + kM, qs.n) - 1, qs.n, ks.n) : 0;      // keys_seen grows with the query
+  const int x0 = tile.first, shift = ks.n - qs.n;
+  // keys_seen grows with the query
+  const int vis = x0 < qs.n ? keys_seen(a, tile.seq, min(x0 + kM, qs.n) - 1, qs.n, ks.n) : 0;
   const int least = x0 + kM <= qs.n ? keys_seen(a, tile.seq, x0, qs.n, ks.n) : 0;
-  uint32_t q[P::k_all][2];
-  row_words<kD>(at(a.q, qs.b, qs.first, h), a.q.st, x0, qs.n, a.D, g, t, q);
-  const __nv_bfloat16 *k = at(a.k, ks.b, ks.first, kh), *v = at(a.v, ks.b, ks.first, kh);
-  const float cs = a.cap > 0.f ? 2.f * kLog2e * a.scale / a.cap : a.scale * kLog2e, cap2 = a.cap * kLog2e;
-  const float slope2 = a.slopes ? a.slopes[h] * kLog2e : 0.f;
-  float o[P::products][4];
+  int lim[2];            // from the lane's first column on
+  float row[2];          // the place of its rows, less its first column
 #pragma unroll
-  for (int i = 0; i < P::products; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-  float m[2] = {kNone, kNone}, l[2] = {0.f, 0.f};
-  uint32_t kw[2][P::k_all];
-  if (vis > 0) score_words<kD>(k, a.k.st, 0, vis, a.D, g, t, kw);
-  for (int j0 = 0; j0 < vis; j0 += 16) {
-    uint32_t vw[P::v_pieces][4][P::v_words];
-    value_words<kD>(v, a.v.st, j0, vis, a.D, g, t, vw);
-    float s[2][4];
-    mma_scores<kD>(s, q, kw);
-    if (j0 + 16 < vis) score_words<kD>(k, a.k.st, j0 + 16, vis, a.D, g, t, kw);
-    const bool masked = j0 + 16 > least;
-    float top[2] = {kNone, kNone};
+  for (int e = 0; e < 2; ++e) {
+    const int x = x0 + g + 8 * e;
+    lim[e] = (x < qs.n ? keys_seen(a, tile.seq, x, qs.n, ks.n) : 0) - 2 * t;
+    row[e] = (float)(x + shift - 2 * t);
+  }
+  const float cs = kCap ? a.scale / a.cap : a.scale * kLog2e, cap2 = a.cap * kLog2e;
+  const long long q_rows = flat_rows(a.rq, a.B), flat = (a.rq.off ? 0 : (long long)qs.b * a.rq.T) + qs.first + x0 + g;
+  for (int h = h0; h < h1; ++h) {
+    const float slope2 = kBias ? -a.slopes[h] * kLog2e : 0.f;
+    uint32_t q[P::k_all][2];
+    row_words<kD>(at(a.q, qs.b, qs.first, h), a.q.st, x0, qs.n, a.D, g, t, q);
+    ScoreRows<kD> k(a.k, ks.b, ks.first, h / R, 0, vis, a.D, g, t);
+    ValueRows<kD> v(a.v, ks.b, ks.first, h / R, 0, vis, a.D, g, t);
+    float o[P::products][4];
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
+    for (int i = 0; i < P::products; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    float m[2] = {kNone, kNone};
+    float2 l[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+    uint32_t kw[2][P::k_all];
+    k.load(a.k.st, kw);
+    for (int j0 = 0; j0 < vis; j0 += 16) {
+      uint32_t vw[P::v_pieces][4][P::v_words];
+      v.load(a.v.st, vw);
+      v.next(a.v.st);
+      float2 s[2][2];      // product (8 columns), row
+      mma_scores<kD>(reinterpret_cast<float(*)[4]>(s), q, kw);
+      k.next(a.k.st);
+      k.load(a.k.st, kw);      // (nothing behind the last)
+      float top[2] = {kNone, kNone};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int j = j0 + 8 * c + 2 * t + (e & 1), r = e >> 1;
-        float x = s[c][e] * cs;
-        if (a.cap > 0.f) x = cap2 - __fdividef(2.f * cap2, 1.f + ex2(x));
-        if (a.slopes != nullptr) x -= slope2 * fabsf((float)(x0 + g + 8 * r + ks.n - qs.n - j));
-        if (masked) x = j < lim[r] ? x : kNone;
-        s[c][e] = x;
-        top[r] = fmaxf(top[r], x);
-      }
+      for (int c = 0; c < 2; ++c)
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-      top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-    }
-    if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
+        for (int r = 0; r < 2; ++r) {
+          float2 x = s[c][r];
+          if (kCap) {
+            x = mul2(x, both(cs));
+            x = make_float2(cap2 * tanh_any(x.x), cap2 * tanh_any(x.y));
+          }
+          if (kBias) {
+            const float away = row[r] - (float)(j0 + 8 * c);
+            const float2 bias = make_float2(slope2 * fabsf(away), slope2 * fabsf(away - 1.f));
+            x = kCap ? add2(x, bias) : fma2(x, both(cs), bias);
+          }
+          if (!kCap && !kBias) x = mul2(x, both(cs));
+          if (j0 + 16 > least) {
+            const int there = lim[r] - j0 - 8 * c;
+            x.x = there > 0 ? x.x : kNone;
+            x.y = there > 1 ? x.y : kNone;
+          }
+          s[c][r] = x;
+          top[r] = max3(top[r], x.x, x.y);
+        }
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const float now = fmaxf(m[r], top[r]), by = now == kNone ? 1.f : ex2(m[r] - now);
-        m[r] = now;
-        l[r] *= by;
-        if (j0 > 0)
+        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+      }
+      if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float now = fmaxf(m[r], top[r]), by = now == kNone ? 1.f : ex2(m[r] - now);
+          m[r] = now;
+          l[r] = mul2(l[r], both(by));
 #pragma unroll
           for (int i = 0; i < P::products; ++i) { o[i][2 * r] *= by; o[i][2 * r + 1] *= by; }
+        }
       }
+      uint32_t p[4];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float2 ref = both(m[r] == kNone ? 0.f : -m[r]);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float2 x = add2(s[c][r], ref);
+          x = make_float2(ex2(x.x), ex2(x.y));
+          l[r] = add2(l[r], x);
+          p[2 * c + r] = pack_bf16(x.x, x.y);
+        }
+      }
+#pragma unroll
+      for (int pc = 0; pc < P::v_pieces; ++pc) mma_values<P::v_words>(o + pc * P::v_cols, p, vw[pc]);
     }
-    const float ref[2] = {m[0] == kNone ? 0.f : m[0], m[1] == kNone ? 0.f : m[1]};
+    float w[2];
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[c][e] = ex2(s[c][e] - ref[e >> 1]);
-        l[e >> 1] += s[c][e];
-      }
-    const uint32_t p[4] = {pack_bf16(s[0][0], s[0][1]), pack_bf16(s[0][2], s[0][3]), pack_bf16(s[1][0], s[1][1]), pack_bf16(s[1][2], s[1][3])};
-#pragma unroll
-    for (int pc = 0; pc < P::v_pieces; ++pc) mma_values<P::v_words>(o + pc * P::v_cols, p, vw[pc]);
+    for (int r = 0; r < 2; ++r) {
+      float sum = l[r].x + l[r].y;
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      w[r] = sum > 0.f ? __fdividef(1.f, sum) : 0.f;
+      if (a.lse != nullptr && t == 0 && x0 + g + 8 * r < qs.n) a.lse[h * q_rows + flat + 8 * r] = sum > 0.f ? m[r] + __log2f(sum) : CUDART_INF_F;
+    }
+    store_rows<kD>(a.o, tile.rows.b, tile.rows.first + x0, tile.rows.n - x0, qs.n - x0, h, a.D, g, t, o, w);
   }
-  float w[2];
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-    w[r] = l[r] > 0.f ? 1.f / l[r] : 0.f;
-    const int x = x0 + g + 8 * r;
-    if (a.lse != nullptr && t == 0 && x < qs.n)
-      a.lse[h * flat_rows(a.rq, a.B) + (a.rq.off ? 0 : (long long)qs.b * a.rq.T) + qs.first + x] = l[r] > 0.f ? m[r] + log2f(l[r]) : CUDART_INF_F;
-  }
-  store_rows<kD>(a.o, tile.rows.b, tile.rows.first + x0, tile.rows.n - x0, qs.n - x0, h, a.D, g, t, o, w);
 }
 
 // kKeys: the warp owns keys; see attention_bwd.cu for X and Y
-template <int kD, bool kKeys>
-__device__ __forceinline__ void short_bwd(const AttnArgs& a, int tile_at, int head) {
+template <int kD, bool kCap, bool kBias, bool kKeys>
+__device__ __forceinline__ void short_bwd(const AttnArgs& a, int tile_at, int head0, int head1) {
   using P = Pieces<kD>;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const Tile tile = tile_of(kKeys ? a.rk : a.rq, a.B, kM, tile_at);
@@ -208,7 +253,8 @@ __device__ __forceinline__ void short_bwd(const AttnArgs& a, int tile_at, int he
     ks = span_of(a.rk, tile.seq);
   }
   const Span& xs = kKeys ? ks : qs;
-  const int x0 = tile.first, R = a.H / a.G;
+  const Span& ys = kKeys ? qs : ks;
+  const int x0 = tile.first, R = a.H / a.G, shift = ks.n - qs.n;
   int lo = 0, hi = 0, all_lo = 0, all_hi = 0;      // rows of Y that rows of X meet, and where all meet all
   if (x0 < xs.n) {
     const int last = min(x0 + kM, xs.n) - 1;
@@ -222,126 +268,160 @@ __device__ __forceinline__ void short_bwd(const AttnArgs& a, int tile_at, int he
     }
   }
   const long long q_rows = flat_rows(a.rq, a.B), q_flat = (a.rq.off ? 0 : (long long)qs.b * a.rq.T) + qs.first;
-  // keys: the queries [meet, nq) see them; queries: keys [0, meet) are seen
+  // from the lane's first column on; keys: the queries [meet, hi) see them; queries: keys [0, meet) are seen
   int meet[2];
-  float lse[2] = {0.f, 0.f}, delta[2] = {0.f, 0.f};
+  float row[2];
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     const int x = x0 + g + 8 * e;
-    const bool there = x < xs.n;
-    if (kKeys) {
-      meet[e] = there ? first_query(a, tile.seq, x, qs.n, ks.n) : 0;
-    } else {
-      meet[e] = there ? keys_seen(a, tile.seq, x, qs.n, ks.n) : 0;
-      if (there) {
-        lse[e] = a.lse[head * q_rows + q_flat + x];
-        delta[e] = a.delta[head * q_rows + q_flat + x];
-      }
-    }
+    meet[e] = (x >= xs.n ? 0 : kKeys ? first_query(a, tile.seq, x, qs.n, ks.n) : keys_seen(a, tile.seq, x, qs.n, ks.n)) - 2 * t;
+    row[e] = (float)((kKeys ? x - shift : x + shift) - 2 * t);
   }
-  uint32_t x1[P::k_all][2], x2[P::k_all][2];
-  if (kKeys) {
-    row_words<kD>(at(a.k, ks.b, ks.first, head), a.k.st, x0, ks.n, a.D, g, t, x1);
-    row_words<kD>(at(a.v, ks.b, ks.first, head), a.v.st, x0, ks.n, a.D, g, t, x2);
-  } else {
-    row_words<kD>(at(a.q, qs.b, qs.first, head), a.q.st, x0, qs.n, a.D, g, t, x1);
-    row_words<kD>(at(a.go, qs.b, qs.first, head), a.go.st, x0, qs.n, a.D, g, t, x2);
-  }
-  float acc1[P::products][4], acc2[kKeys ? P::products : 1][4];
+  const float cs = kCap ? a.scale / a.cap : a.scale * kLog2e, cap2 = a.cap * kLog2e;
+  const AttnOperand &o1 = kKeys ? a.q : a.k, &o2 = kKeys ? a.go : a.v;
+  for (int head = head0; head < head1; ++head) {
+    uint32_t x1[P::k_all][2], x2[P::k_all][2];
+    const AttnOperand &r1 = kKeys ? a.k : a.q, &r2 = kKeys ? a.v : a.go;
+    row_words<kD>(at(r1, xs.b, xs.first, head), r1.st, x0, xs.n, a.D, g, t, x1);
+    row_words<kD>(at(r2, xs.b, xs.first, head), r2.st, x0, xs.n, a.D, g, t, x2);
+    float lse[2] = {0.f, 0.f}, delta[2] = {0.f, 0.f};      // negative
+    if (!kKeys)
 #pragma unroll
-  for (int i = 0; i < P::products; ++i) acc1[i][0] = acc1[i][1] = acc1[i][2] = acc1[i][3] = 0.f;
-  if (kKeys)
+      for (int e = 0; e < 2; ++e)
+        if (x0 + g + 8 * e < qs.n) {
+          const long long i = head * q_rows + q_flat + x0 + g + 8 * e;
+          lse[e] = -a.lse[i];
+          delta[e] = -a.delta[i];
+        }
+    float acc1[P::products][4], acc2[kKeys ? P::products : 1][4];
 #pragma unroll
-    for (int i = 0; i < P::products; ++i) acc2[i][0] = acc2[i][1] = acc2[i][2] = acc2[i][3] = 0.f;
-  const float cs = a.cap > 0.f ? 2.f * kLog2e * a.scale / a.cap : a.scale * kLog2e, cap2 = a.cap * kLog2e;
-  const int shift = ks.n - qs.n;
-  for (int hh = 0; hh < (kKeys ? R : 1); ++hh) {
-    const int h = kKeys ? head * R + hh : head;
-    const float slope2 = a.slopes ? a.slopes[h] * kLog2e : 0.f;
-    const __nv_bfloat16 *y1 = kKeys ? at(a.q, qs.b, qs.first, h) : at(a.k, ks.b, ks.first, head / R);
-    const __nv_bfloat16 *y2 = kKeys ? at(a.go, qs.b, qs.first, h) : at(a.v, ks.b, ks.first, head / R);
-    const long long st1 = kKeys ? a.q.st : a.k.st, st2 = kKeys ? a.go.st : a.v.st;
-    const float *lse_y = a.lse + h * q_rows + q_flat, *delta_y = a.delta + h * q_rows + q_flat;
-    for (int y0 = lo; y0 < hi; y0 += 16) {
-      uint32_t w1[2][P::k_all], w2[2][P::k_all];
-      score_words<kD>(y1, st1, y0, hi, a.D, g, t, w1);
-      score_words<kD>(y2, st2, y0, hi, a.D, g, t, w2);
-      float ly[2][2], dy[2][2];
-      if (kKeys)
+    for (int i = 0; i < P::products; ++i) acc1[i][0] = acc1[i][1] = acc1[i][2] = acc1[i][3] = 0.f;
+    if (kKeys)
+#pragma unroll
+      for (int i = 0; i < P::products; ++i) acc2[i][0] = acc2[i][1] = acc2[i][2] = acc2[i][3] = 0.f;
+    for (int hh = 0; hh < (kKeys ? R : 1); ++hh) {
+      const int h = kKeys ? head * R + hh : head, hy = kKeys ? h : head / R;
+      const float slope2 = kBias ? -a.slopes[h] * kLog2e : 0.f;
+      ScoreRows<kD> s1(o1, ys.b, ys.first, hy, lo, hi, a.D, g, t), s2(o2, ys.b, ys.first, hy, lo, hi, a.D, g, t);
+      ValueRows<kD> v1(o1, ys.b, ys.first, hy, lo, hi, a.D, g, t), v2(o2, ys.b, ys.first, hy, lo, hi, a.D, g, t);
+      const float *lse_y = a.lse + h * q_rows + q_flat + 2 * t, *delta_y = a.delta + h * q_rows + q_flat + 2 * t;
+      for (int y0 = lo; y0 < hi; y0 += 16) {
+        uint32_t w1[2][P::k_all], w2[2][P::k_all], u1[P::v_pieces][4][P::v_words], u2[kKeys ? P::v_pieces : 1][4][P::v_words];
+        s1.load(o1.st, w1);
+        s2.load(o2.st, w2);
+        s1.next(o1.st);
+        s2.next(o2.st);
+        float2 ly[2], dy[2];
+        if (kKeys)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int y = y0 + 8 * c, left = hi - y - 2 * t;
+            ly[c] = make_float2(left > 0 ? -lse_y[y] : 0.f, left > 1 ? -lse_y[y + 1] : 0.f);
+            dy[c] = make_float2(left > 0 ? -delta_y[y] : 0.f, left > 1 ? -delta_y[y + 1] : 0.f);
+          }
+        v1.load(o1.st, u1);
+        v1.next(o1.st);
+        if (kKeys) {
+          v2.load(o2.st, u2);
+          v2.next(o2.st);
+        }
+        float2 s[2][2], d[2][2];
+        mma_scores<kD>(reinterpret_cast<float(*)[4]>(s), x1, w1);
+        mma_scores<kD>(reinterpret_cast<float(*)[4]>(d), x2, w2);
+        const bool masked = y0 < all_lo || y0 + 16 > all_hi;
+        uint32_t da[4], pa[4];
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int f = 0; f < 2; ++f) {
-            const int y = y0 + 8 * c + 2 * t + f;
-            ly[c][f] = y < hi ? lse_y[y] : 0.f;
-            dy[c][f] = y < hi ? delta_y[y] : 0.f;
+          for (int r = 0; r < 2; ++r) {
+            const float2 lg = kKeys ? ly[c] : both(lse[r]), dl = kKeys ? dy[c] : both(delta[r]);
+            float2 arg, slope;
+            if (kCap) {
+              const float2 y = mul2(s[c][r], both(cs));
+              const float2 th = make_float2(tanh_any(y.x), tanh_any(y.y));
+              arg = fma2(th, both(cap2), lg);
+              slope = fma2(mul2(th, both(-1.f)), th, both(1.f));
+            } else {
+              arg = fma2(s[c][r], both(cs), lg);
+            }
+            if (kBias) {
+              const float away = row[r] - (float)(y0 + 8 * c);
+              arg = add2(arg, make_float2(slope2 * fabsf(away), slope2 * fabsf(away - 1.f)));
+            }
+            float2 p = make_float2(ex2(arg.x), ex2(arg.y));
+            float2 ds = mul2(p, add2(d[c][r], dl));
+            if (kCap) ds = mul2(ds, slope);
+            if (masked) {
+              const int y = y0 + 8 * c, n = (kKeys ? hi - 2 * t : meet[r]) - y, k = kKeys ? meet[r] - y : 0;      // of the lane's columns, [k, n)
+              if (!(n > 0 && k <= 0)) p.x = ds.x = 0.f;
+              if (!(n > 1 && k <= 1)) p.y = ds.y = 0.f;
+            }
+            da[2 * c + r] = pack_bf16(ds.x, ds.y);
+            if (kKeys) pa[2 * c + r] = pack_bf16(p.x, p.y);
           }
-      uint32_t u1[P::v_pieces][4][P::v_words], u2[kKeys ? P::v_pieces : 1][4][P::v_words];
-      value_words<kD>(y1, st1, y0, hi, a.D, g, t, u1);
-      if (kKeys) value_words<kD>(y2, st2, y0, hi, a.D, g, t, u2);
-      float s[2][4], d[2][4];
-      mma_scores<kD>(s, x1, w1);
-      mma_scores<kD>(d, x2, w2);
-      const bool masked = y0 < all_lo || y0 + 16 > all_hi;
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
+        for (int pc = 0; pc < P::v_pieces; ++pc) mma_values<P::v_words>(acc1 + pc * P::v_cols, da, u1[pc]);
+        if (kKeys)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = e >> 1, f = e & 1, x = x0 + g + 8 * r, y = y0 + 8 * c + 2 * t + f;
-          const float lg = kKeys ? ly[c][f] : lse[r], dl = kKeys ? dy[c][f] : delta[r];
-          float arg, slope = 1.f;
-          if (a.cap > 0.f) {
-            const float tt = __fdividef(1.f, 1.f + ex2(s[c][e] * cs));
-            arg = cap2 - 2.f * cap2 * tt - lg;
-            slope = 4.f * tt * (1.f - tt);
-          } else {
-            arg = fmaf(s[c][e], cs, -lg);
-          }
-          if (a.slopes != nullptr) arg -= slope2 * fabsf((float)(kKeys ? y + shift - x : x + shift - y));
-          float p = ex2(arg), ds = p * (d[c][e] - dl) * slope;
-          if (masked && !(kKeys ? y >= meet[r] && y < hi : y < meet[r])) p = ds = 0.f;
-          s[c][e] = p;
-          d[c][e] = ds;
-        }
-      const uint32_t da[4] = {pack_bf16(d[0][0], d[0][1]), pack_bf16(d[0][2], d[0][3]), pack_bf16(d[1][0], d[1][1]), pack_bf16(d[1][2], d[1][3])};
-#pragma unroll
-      for (int pc = 0; pc < P::v_pieces; ++pc) mma_values<P::v_words>(acc1 + pc * P::v_cols, da, u1[pc]);
-      if (kKeys) {
-        const uint32_t pa[4] = {pack_bf16(s[0][0], s[0][1]), pack_bf16(s[0][2], s[0][3]), pack_bf16(s[1][0], s[1][1]), pack_bf16(s[1][2], s[1][3])};
-#pragma unroll
-        for (int pc = 0; pc < P::v_pieces; ++pc) mma_values<P::v_words>(acc2 + pc * P::v_cols, pa, u2[pc]);
+          for (int pc = 0; pc < P::v_pieces; ++pc) mma_values<P::v_words>(acc2 + pc * P::v_cols, pa, u2[pc]);
       }
     }
+    const float scales[2] = {a.scale, a.scale}, ones[2] = {1.f, 1.f};
+    const long long first = tile.rows.first + x0;
+    const int there = tile.rows.n - x0, filled = xs.n - x0;
+    store_rows<kD>(kKeys ? a.gk : a.gq, tile.rows.b, first, there, filled, head, a.D, g, t, acc1, scales);
+    if (kKeys) store_rows<kD>(a.gv, tile.rows.b, first, there, filled, head, a.D, g, t, acc2, ones);
   }
-  const float scales[2] = {a.scale, a.scale}, ones[2] = {1.f, 1.f};
-  const long long first = tile.rows.first + x0;
-  const int there = tile.rows.n - x0, filled = xs.n - x0;
-  store_rows<kD>(kKeys ? a.gk : a.gq, tile.rows.b, first, there, filled, head, a.D, g, t, acc1, scales);
-  if (kKeys) store_rows<kD>(a.gv, tile.rows.b, first, there, filled, head, a.D, g, t, acc2, ones);
 }
 
 // The first key_units warps own keys, the others queries.
-template <int kD>
-__global__ void __launch_bounds__(32 * kWarps) attention_short_bwd_kernel(const __grid_constant__ AttnArgs a, long long key_units, long long units) {
+template <int kD, bool kCap, bool kBias>
+__global__ void __launch_bounds__(32 * kWarps, kD == 16 ? 4 : kD == 32 ? 3 : 2)
+attention_short_bwd_kernel(const __grid_constant__ AttnArgs a, unsigned key_units, unsigned units, unsigned key_heads, unsigned heads) {
   pdl_sync();
-  const long long unit = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  const unsigned unit = blockIdx.x * kWarps + (threadIdx.x >> 5);
   if (unit >= units) return;
-  if (unit < key_units) short_bwd<kD, true>(a, (int)(unit / a.G), (int)(unit % a.G));
-  else short_bwd<kD, false>(a, (int)((unit - key_units) / a.H), (int)((unit - key_units) % a.H));
+  if (unit < key_units) {
+    const unsigned groups = ((unsigned)a.G + key_heads - 1) / key_heads, tile = unit / groups, h0 = (unit - tile * groups) * key_heads;
+    short_bwd<kD, kCap, kBias, true>(a, (int)tile, (int)h0, min(a.G, (int)(h0 + key_heads)));
+  } else {
+    const unsigned at = unit - key_units, groups = ((unsigned)a.H + heads - 1) / heads, tile = at / groups, h0 = (at - tile * groups) * heads;
+    short_bwd<kD, kCap, kBias, false>(a, (int)tile, (int)h0, min(a.H, (int)(h0 + heads)));
+  }
 }
 
-template <int kD>
+// Heads that a warp takes of its tile: finding the tile costs as much as a step or two, but every SM wants some 32 warps, and again as
+// many in turn.
+unsigned heads_of(long long tiles, int H) {
+  unsigned n = 1;
+  while (n < 8 && n < (unsigned)H && tiles * ((H + 2 * n - 1) / (2 * n)) >= 148 * 64) n *= 2;
+  return n;
+}
+
+template <int kD, bool kCap, bool kBias>
 cudaError_t launch_fwd(const AttnArgs& a, cudaStream_t st) {
-  const long long tiles = tile_count(a.rq, a.B, kM), blocks = (tiles * a.H + kWarps - 1) / kWarps;
-  if (blocks >= (1LL << 31)) return cudaErrorInvalidConfiguration;
-  return launch_pdl(attention_short_fwd_kernel<kD>, dim3((unsigned)blocks), dim3(32 * kWarps), 0, st, a, (int)tiles);
+  const long long tiles = tile_count(a.rq, a.B, kM);
+  const unsigned heads = heads_of(tiles, a.H);
+  const long long units = tiles * ((a.H + heads - 1) / heads);
+  if (units >= (1LL << 31)) return cudaErrorInvalidConfiguration;
+  return launch_pdl(attention_short_fwd_kernel<kD, kCap, kBias>, dim3((unsigned)((units + kWarps - 1) / kWarps)), dim3(32 * kWarps), 0, st, a,
+                    (unsigned)tiles, heads);
+}
+template <int kD, bool kCap, bool kBias>
+cudaError_t launch_bwd(const AttnArgs& a, cudaStream_t st) {
+  const long long key_tiles = tile_count(a.rk, a.B, kM), tiles = tile_count(a.rq, a.B, kM);
+  const unsigned key_heads = heads_of(key_tiles, a.G), heads = heads_of(tiles, a.H);
+  const long long key_units = key_tiles * ((a.G + key_heads - 1) / key_heads), units = key_units + tiles * ((a.H + heads - 1) / heads);
+  if (units >= (1LL << 31)) return cudaErrorInvalidConfiguration;
+  return launch_pdl(attention_short_bwd_kernel<kD, kCap, kBias>, dim3((unsigned)((units + kWarps - 1) / kWarps)), dim3(32 * kWarps), 0, st, a,
+                    (unsigned)key_units, (unsigned)units, key_heads, heads);
 }
 template <int kD>
-cudaError_t launch_bwd(const AttnArgs& a, cudaStream_t st) {
-  const long long key_units = tile_count(a.rk, a.B, kM) * a.G, units = key_units + tile_count(a.rq, a.B, kM) * a.H;
-  const long long blocks = (units + kWarps - 1) / kWarps;
-  if (blocks >= (1LL << 31)) return cudaErrorInvalidConfiguration;
-  return launch_pdl(attention_short_bwd_kernel<kD>, dim3((unsigned)blocks), dim3(32 * kWarps), 0, st, a, key_units, units);
+cudaError_t launch(bool fwd, const AttnArgs& a, cudaStream_t st) {
+  if (a.cap > 0.f && a.slopes) return fwd ? launch_fwd<kD, true, true>(a, st) : launch_bwd<kD, true, true>(a, st);
+  if (a.cap > 0.f) return fwd ? launch_fwd<kD, true, false>(a, st) : launch_bwd<kD, true, false>(a, st);
+  if (a.slopes) return fwd ? launch_fwd<kD, false, true>(a, st) : launch_bwd<kD, false, true>(a, st);
+  return fwd ? launch_fwd<kD, false, false>(a, st) : launch_bwd<kD, false, false>(a, st);
 }
 const char* told(cudaError_t e) {
   if (e == cudaSuccess) e = cudaGetLastError();
@@ -356,10 +436,10 @@ long long length_of(const AttnRows& r, int B) { return r.off ? r.T / (B > 0 ? B 
 bool attention_short_takes(const AttnArgs& a) { return a.D <= 64 && length_of(a.rq, a.B) <= kAttnShort && length_of(a.rk, a.B) <= kAttnShort; }
 
 const char* launch_attention_short_fwd(const AttnArgs& a, cudaStream_t st) {
-  return told(a.D <= 16 ? launch_fwd<16>(a, st) : a.D <= 32 ? launch_fwd<32>(a, st) : launch_fwd<64>(a, st));
+  return told(a.D <= 16 ? launch<16>(true, a, st) : a.D <= 32 ? launch<32>(true, a, st) : launch<64>(true, a, st));
 }
 const char* launch_attention_short_bwd(const AttnArgs& a, cudaStream_t st) {
-  return told(a.D <= 16 ? launch_bwd<16>(a, st) : a.D <= 32 ? launch_bwd<32>(a, st) : launch_bwd<64>(a, st));
+  return told(a.D <= 16 ? launch<16>(false, a, st) : a.D <= 32 ? launch<32>(false, a, st) : launch<64>(false, a, st));
 }
 
 }  // namespace tn
