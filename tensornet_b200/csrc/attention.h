@@ -40,8 +40,7 @@ bool attention_few_takes(const AttnArgs& a);
 long long attention_few_floats(const AttnArgs& a);
 const char* launch_attention_few(const AttnArgs& a, float* work, cudaStream_t st);
 // Short sequences of up to 64 columns: whether the warp-per-tile kernels take the call.  launch_attention_bwd asks by itself.
-constexpr int kAttnShort = 64;      // the mean length up to which they do
-bool attention_short_takes(const AttnArgs& a);
+bool attention_short_takes(const AttnArgs& a, bool backward);
 const char* launch_attention_short_fwd(const AttnArgs& a, cudaStream_t st);
 const char* launch_attention_short_bwd(const AttnArgs& a, cudaStream_t st);
 const char* launch_attention_bwd(const AttnArgs& a, cudaStream_t st);

@@ -475,7 +475,7 @@ const char* launch_attention_bwd(const AttnArgs& a, cudaStream_t st) {
   int lanes = 1;
   while (lanes * 8 < a.D) lanes <<= 1;
   cudaError_t e = launch_pdl(attention_delta_kernel, dim3((unsigned)((rows * a.H * lanes + 255) / 256)), dim3(256), 0, st, a, rows, lanes);
-  if (e == cudaSuccess && attention_short_takes(a)) return launch_attention_short_bwd(a, st);
+  if (e == cudaSuccess && attention_short_takes(a, true)) return launch_attention_short_bwd(a, st);
   BwdMaps maps;
   const int box = a.D > 64 ? BwdShape<128>::y : BwdShape<64>::y;
   if (!operand_map(a.q, a.D, a.rq, a.B, a.H, box, &maps.q) || !operand_map(a.k, a.D, a.rk, a.B, a.G, box, &maps.k) ||

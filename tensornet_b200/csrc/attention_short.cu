@@ -433,7 +433,16 @@ long long length_of(const AttnRows& r, int B) { return r.off ? r.T / (B > 0 ? B 
 
 }  // namespace
 
-bool attention_short_takes(const AttnArgs& a) { return a.D <= 64 && length_of(a.rq, a.B) <= kAttnShort && length_of(a.rk, a.B) <= kAttnShort; }
+// By the mean length, which is what the host knows of packed sequences.  200000 tokens, 4 heads, causal, us of these kernels and of those
+// for long sequences:
+//   forward   16 columns: 200 tokens 135 and 246, 400: 205 and 293;  32: 200: 183 and 256, 400: 268 and 305;  64: 128: 233 and 252, 200: 295
+//             and 265
+//   backward  16 columns: 256 tokens 417 and 501, 400: 577 and 638;  32: 200: 562 and 663, 256: 632 and 545;  64: 64: 636 and 826, 100: 771
+//             and 769
+bool attention_short_takes(const AttnArgs& a, bool backward) {
+  const int most = backward ? (a.D <= 16 ? 400 : a.D <= 32 ? 224 : 96) : (a.D <= 16 ? 512 : a.D <= 32 ? 400 : 144);
+  return a.D <= 64 && length_of(a.rq, a.B) <= most && length_of(a.rk, a.B) <= most;
+}
 
 const char* launch_attention_short_fwd(const AttnArgs& a, cudaStream_t st) {
   return told(a.D <= 16 ? launch<16>(true, a, st) : a.D <= 32 ? launch<32>(true, a, st) : launch<64>(true, a, st));

@@ -17,7 +17,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <type_traits>
-#include "tn_device.cuh"
+#include "attention_tc.cuh"
 #include "tn_ops.h"
 
 namespace tn {
@@ -31,7 +31,7 @@ constexpr int kWideBlock = 512;
 template <typename T> struct Piece;
 template <> struct Piece<float> {
   static constexpr int n = 4;
-  __device__ static void unpack(const uint4& v, float* f) {
+  __device__ __forceinline__ static void unpack(const uint4& v, float* f) {
     f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y); f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
   }
   __device__ static uint4 pack(const float* f) {
@@ -42,7 +42,7 @@ template <> struct Piece<float> {
 };
 template <> struct Piece<__nv_bfloat16> {
   static constexpr int n = 8;
-  __device__ static void unpack(const uint4& v, float* f) {
+  __device__ __forceinline__ static void unpack(const uint4& v, float* f) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -64,7 +64,7 @@ template <> struct Piece<__nv_bfloat16> {
 };
 template <> struct Piece<__half> {
   static constexpr int n = 8;
-  __device__ static void unpack(const uint4& v, float* f) {
+  __device__ __forceinline__ static void unpack(const uint4& v, float* f) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -110,104 +110,116 @@ __device__ __forceinline__ void store_piece(T* p, long long at, const float* f, 
     if (e >= lo && e < hi) p[at * n + e] = Piece<T>::put(f[e]);
 }
 
-// Sum over the threads of a group: part of a warp, or the block.  `s`: two rows of 32 floats that take turns, so that one barrier
-// per sum is enough.
-template <bool kBlockRow, int kN>
-__device__ __forceinline__ void group_sum(float (&v)[kN], int tpr, float* s, int& turn) {
+// Sum over the tpr threads of a group in a warp
+template <int kN>
+__device__ __forceinline__ void warp_sum(float (&v)[kN], int tpr) {
 #pragma unroll
   for (int i = 0; i < kN; ++i)
-    for (int o = (kBlockRow ? 16 : tpr / 2); o > 0; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
-  if (!kBlockRow) return;
+    for (int o = tpr / 2; o > 0; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+}
+
+// Sum over the block.  `s`: two rows of 32 values that take turns, so that one barrier per sum is enough.
+template <int kN>
+__device__ __forceinline__ void block_sum(float (&v)[kN], int threads, float* s, int& turn) {
+  warp_sum<kN>(v, 32);
   float* row = s + turn * 32 * kN;
   turn ^= 1;
-  const int warp = threadIdx.x >> 5, warps = tpr >> 5;
+  const int warp = threadIdx.x >> 5, warps = threads >> 5;      // an even number
   if ((threadIdx.x & 31) == 0)
 #pragma unroll
     for (int i = 0; i < kN; ++i) row[warp * kN + i] = v[i];
   __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kN; ++i) v[i] = 0.f;
-  for (int w = 0; w < warps; ++w)
-#pragma unroll
-    for (int i = 0; i < kN; ++i) v[i] += row[w * kN + i];
+  float2 sum = make_float2(0.f, 0.f);
+  for (int w = 0; w < warps * kN / 2; ++w) sum = attn::add2(sum, *reinterpret_cast<const float2*>(row + 2 * w));
+  if (kN == 1) v[0] = sum.x + sum.y;
+  else { v[0] = sum.x; v[kN - 1] = sum.y; }
 }
 
 // Columns of a piece that lie in the row: the piece's first element is column `c0` (negative in front of the row).
 __device__ __forceinline__ bool in_row(int c, int C) { return (unsigned)c < (unsigned)C; }
 
-// kNV pieces per thread; kBlockRow: a row per block, else 32 / tpr rows or more per warp.
-template <typename T, int kNV, bool kBlockRow>
-__global__ void __launch_bounds__(kBlockRow ? kWideBlock : kBlock)
+// A thread's piece number p of a row: all of it lies in the row, or only some elements do.
+template <int n>
+__device__ __forceinline__ bool whole_piece(int p, int shift, int C) { return p * n >= shift && p * n + n <= shift + C; }
+template <int n>
+__device__ __forceinline__ void keep_row(float2 (&f)[n / 2], int p, int shift, int C) {
+#pragma unroll
+  for (int e = 0; e < n / 2; ++e) {
+    if (!in_row(p * n + 2 * e - shift, C)) f[e].x = 0.f;
+    if (!in_row(p * n + 2 * e + 1 - shift, C)) f[e].y = 0.f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void pairs_of(const uint4& v, float2* f) { Piece<T>::unpack(v, reinterpret_cast<float*>(f)); }
+
+// kNV pieces per thread, 32 / tpr rows or more per warp
+template <typename T, int kNV>
+__global__ void __launch_bounds__(kBlock)
 layer_norm_fwd_kernel(const T* __restrict__ x, const float* __restrict__ gamma, const float* __restrict__ beta, float eps, long long rows, int C,
                       int tpr, T* __restrict__ y, float* __restrict__ stats) {
   constexpr int n = Piece<T>::n;
+  using namespace attn;
   pdl_sync();
-  __shared__ float s_sum[64];
-  int turn = 0;
-  const int t = kBlockRow ? threadIdx.x : threadIdx.x % tpr;
-  const int per_block = kBlockRow ? 1 : blockDim.x / tpr;
+  const int t = threadIdx.x % tpr;
+  const int per_block = blockDim.x / tpr;
   const long long groups = (long long)gridDim.x * per_block;
-  const long long first = (long long)blockIdx.x * per_block + (kBlockRow ? 0 : threadIdx.x / tpr);
+  const long long first = (long long)blockIdx.x * per_block + threadIdx.x / tpr;
   const int shift = (int)((first * C) % n);            // the same for all rows of the group
-  const long long total = rows * C;
+  const long long total = rows * C, step = groups * C / n;
   const float inv = 1.f / (float)C;
 
-  float g[kNV * n], b[kNV * n];
+  float2 g[kNV][n / 2], b[kNV][n / 2];
 #pragma unroll
   for (int i = 0; i < kNV; ++i)
 #pragma unroll
     for (int e = 0; e < n; ++e) {
       const int c = (t + i * tpr) * n + e - shift;
-      g[i * n + e] = gamma != nullptr && in_row(c, C) ? gamma[c] : 1.f;
-      b[i * n + e] = beta != nullptr && in_row(c, C) ? beta[c] : 0.f;
+      reinterpret_cast<float*>(g[i])[e] = gamma != nullptr && in_row(c, C) ? gamma[c] : 1.f;
+      reinterpret_cast<float*>(b[i])[e] = beta != nullptr && in_row(c, C) ? beta[c] : 0.f;
     }
   const int pieces = (shift + C + n - 1) / n;
+  long long at = (first * C - shift) / n + t;           // of the thread's first piece
   uint4 v[kNV];
-  auto fetch = [&](long long r) {
-    const long long at = (r * C - shift) / n;
+  auto fetch = [&](long long from) {
 #pragma unroll
     for (int i = 0; i < kNV; ++i)
-      if (t + i * tpr < pieces) v[i] = load_piece(x, at + t + i * tpr, total);
+      if (t + i * tpr < pieces) v[i] = load_piece(x, from + i * tpr, total);
   };
   // Threads of one warp may belong to rows on both sides of the end; all of them take part in the sums.
-  const long long last = kBlockRow ? rows : first - (kBlockRow ? 0 : (threadIdx.x % 32) / tpr);
-  if (first < rows) fetch(first);
-  for (long long r = first, lead = last; kBlockRow ? r < rows : lead < rows; r += groups, lead += groups) {
-    float f[kNV * n];
-    float m[1] = {0.f};
+  if (first < rows) fetch(at);
+  for (long long r = first, lead = first - (threadIdx.x % 32) / tpr; lead < rows; r += groups, lead += groups, at += step) {
+    float2 f[kNV][n / 2], m2 = make_float2(0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < kNV; ++i) {
-      Piece<T>::unpack(v[i], f + i * n);
+      pairs_of<T>(v[i], f[i]);
+      if (!whole_piece<n>(t + i * tpr, shift, C)) keep_row<n>(f[i], t + i * tpr, shift, C);
 #pragma unroll
-      for (int e = 0; e < n; ++e) {
-        if (!in_row((t + i * tpr) * n + e - shift, C)) f[i * n + e] = 0.f;
-        m[0] += f[i * n + e];
-      }
+      for (int e = 0; e < n / 2; ++e) m2 = add2(m2, f[i][e]);
     }
-    if (r + groups < rows) fetch(r + groups);           // in flight beside the sums
-    group_sum<kBlockRow, 1>(m, tpr, s_sum, turn);
+    if (r + groups < rows) fetch(at + step);           // in flight beside the sums
+    float m[1] = {m2.x + m2.y};
+    warp_sum<1>(m, tpr);
     const float mean = m[0] * inv;
-    float q[1] = {0.f};
+    float2 q2 = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < kNV; ++i)
+    for (int i = 0; i < kNV; ++i) {
 #pragma unroll
-      for (int e = 0; e < n; ++e) {
-        const float d = f[i * n + e] - mean;
-        f[i * n + e] = d;
-        if (in_row((t + i * tpr) * n + e - shift, C)) q[0] += d * d;
-      }
-    group_sum<kBlockRow, 1>(q, tpr, s_sum, turn);
+      for (int e = 0; e < n / 2; ++e) f[i][e] = add2(f[i][e], both(-mean));
+      if (!whole_piece<n>(t + i * tpr, shift, C)) keep_row<n>(f[i], t + i * tpr, shift, C);
+#pragma unroll
+      for (int e = 0; e < n / 2; ++e) q2 = fma2(f[i][e], f[i][e], q2);
+    }
+    float q[1] = {q2.x + q2.y};
+    warp_sum<1>(q, tpr);
     const float rstd = 1.f / sqrtf(q[0] * inv + eps);
     if (r >= rows) continue;
-    const long long at = (r * C - shift) / n;
 #pragma unroll
     for (int i = 0; i < kNV; ++i) {
       const int p = t + i * tpr;
       if (p >= pieces) continue;
-      float o[n];
 #pragma unroll
-      for (int e = 0; e < n; ++e) o[e] = f[i * n + e] * rstd * g[i * n + e] + b[i * n + e];
-      store_piece(y, at + p, o, shift - p * n, shift + C - p * n);
+      for (int e = 0; e < n / 2; ++e) f[i][e] = fma2(mul2(f[i][e], both(rstd)), g[i][e], b[i][e]);
+      store_piece(y, at + i * tpr, reinterpret_cast<const float*>(f[i]), shift - p * n, shift + C - p * n);
     }
     if (stats != nullptr && t == 0) {
       stats[r] = mean;
@@ -217,85 +229,85 @@ layer_norm_fwd_kernel(const T* __restrict__ x, const float* __restrict__ gamma, 
 }
 
 // part: [gridDim.x][2][C], the block's sums of dgamma and dbeta; null where they are not wanted
-template <typename T, int kNV, bool kBlockRow>
-__global__ void __launch_bounds__(kBlockRow ? kWideBlock : kBlock)
+template <typename T, int kNV>
+__global__ void __launch_bounds__(kBlock)
 layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, const float* __restrict__ stats, const float* __restrict__ gamma,
                       long long rows, int C, int tpr, T* __restrict__ dx, float* __restrict__ part) {
   constexpr int n = Piece<T>::n;
+  using namespace attn;
   pdl_sync();
-  __shared__ float s_sum[128];
   extern __shared__ float s_part[];                      // [groups of the block][2][C]
-  int turn = 0;
-  const int t = kBlockRow ? threadIdx.x : threadIdx.x % tpr;
-  const int per_block = kBlockRow ? 1 : blockDim.x / tpr;
-  const int group = kBlockRow ? 0 : threadIdx.x / tpr;
+  const int t = threadIdx.x % tpr;
+  const int per_block = blockDim.x / tpr;
+  const int group = threadIdx.x / tpr;
   const long long groups = (long long)gridDim.x * per_block;
   const long long first = (long long)blockIdx.x * per_block + group;
   const int shift = (int)((first * C) % n);
-  const long long total = rows * C;
+  const long long total = rows * C, step = groups * C / n;
   const float inv = 1.f / (float)C;
 
-  float g[kNV * n], sg[kNV * n], sb[kNV * n];
+  float2 g[kNV][n / 2], sg[kNV][n / 2], sb[kNV][n / 2];
 #pragma unroll
-  for (int i = 0; i < kNV; ++i)
+  for (int i = 0; i < kNV; ++i) {
 #pragma unroll
     for (int e = 0; e < n; ++e) {
       const int c = (t + i * tpr) * n + e - shift;
-      g[i * n + e] = gamma != nullptr && in_row(c, C) ? gamma[c] : 1.f;
-      sg[i * n + e] = sb[i * n + e] = 0.f;
+      reinterpret_cast<float*>(g[i])[e] = gamma != nullptr && in_row(c, C) ? gamma[c] : 1.f;
     }
+#pragma unroll
+    for (int e = 0; e < n / 2; ++e) sg[i][e] = sb[i][e] = make_float2(0.f, 0.f);
+  }
   const int pieces = (shift + C + n - 1) / n;
+  long long at = (first * C - shift) / n + t;
   uint4 vx[kNV], vd[kNV];
   float mean_next = 0.f, rstd_next = 0.f;
-  auto fetch = [&](long long r) {
-    const long long at = (r * C - shift) / n;
+  auto fetch = [&](long long r, long long from) {
     mean_next = stats[r];
     rstd_next = stats[rows + r];
 #pragma unroll
     for (int i = 0; i < kNV; ++i)
       if (t + i * tpr < pieces) {
-        vx[i] = load_piece(x, at + t + i * tpr, total);
-        vd[i] = load_piece(dy, at + t + i * tpr, total);
+        vx[i] = load_piece(x, from + i * tpr, total);
+        vd[i] = load_piece(dy, from + i * tpr, total);
       }
   };
-  const long long lead0 = kBlockRow ? first : first - (threadIdx.x % 32) / tpr;
-  if (first < rows) fetch(first);
-  for (long long r = first, lead = lead0; lead < rows; r += groups, lead += groups) {
+  if (first < rows) fetch(first, at);
+  for (long long r = first, lead = first - (threadIdx.x % 32) / tpr; lead < rows; r += groups, lead += groups, at += step) {
     const bool there = r < rows;
     const float mean = mean_next, rstd = rstd_next;
-    float fx[kNV * n], fd[kNV * n];
-    float m[2] = {0.f, 0.f};
+    float2 fx[kNV][n / 2], fd[kNV][n / 2], m0 = make_float2(0.f, 0.f), m1 = m0;
 #pragma unroll
     for (int i = 0; i < kNV; ++i) {
-      Piece<T>::unpack(vx[i], fx + i * n);
-      Piece<T>::unpack(vd[i], fd + i * n);
+      pairs_of<T>(vx[i], fx[i]);
+      pairs_of<T>(vd[i], fd[i]);
 #pragma unroll
-      for (int e = 0; e < n; ++e) {
-        const int k = i * n + e;
-        const bool in = there && in_row((t + i * tpr) * n + e - shift, C);
-        fx[k] = in ? (fx[k] - mean) * rstd : 0.f;
-        fd[k] = in ? fd[k] : 0.f;
-        sb[k] += fd[k];
-        sg[k] += fd[k] * fx[k];
-        fd[k] *= g[k];
-        m[0] += fd[k];
-        m[1] += fd[k] * fx[k];
+      for (int e = 0; e < n / 2; ++e) fx[i][e] = mul2(add2(fx[i][e], both(-mean)), both(rstd));
+      if (!there || !whole_piece<n>(t + i * tpr, shift, C)) {
+        keep_row<n>(fx[i], t + i * tpr, shift, there ? C : 0);
+        keep_row<n>(fd[i], t + i * tpr, shift, there ? C : 0);
+      }
+#pragma unroll
+      for (int e = 0; e < n / 2; ++e) {
+        sb[i][e] = add2(sb[i][e], fd[i][e]);
+        sg[i][e] = fma2(fd[i][e], fx[i][e], sg[i][e]);
+        fd[i][e] = mul2(fd[i][e], g[i][e]);
+        m0 = add2(m0, fd[i][e]);
+        m1 = fma2(fd[i][e], fx[i][e], m1);
       }
     }
-    if (r + groups < rows) fetch(r + groups);
+    if (r + groups < rows) fetch(r + groups, at + step);
     if (dx == nullptr) continue;
-    group_sum<kBlockRow, 2>(m, tpr, s_sum, turn);
+    float m[2] = {m0.x + m0.y, m1.x + m1.y};
+    warp_sum<2>(m, tpr);
     if (!there) continue;
     const float c1 = m[0] * inv, c2 = m[1] * inv;
-    const long long at = (r * C - shift) / n;
 #pragma unroll
     for (int i = 0; i < kNV; ++i) {
       const int p = t + i * tpr;
       if (p >= pieces) continue;
-      float o[n];
 #pragma unroll
-      for (int e = 0; e < n; ++e) o[e] = rstd * (fd[i * n + e] - c1 - fx[i * n + e] * c2);
-      store_piece(dx, at + p, o, shift - p * n, shift + C - p * n);
+      for (int e = 0; e < n / 2; ++e) fd[i][e] = mul2(fma2(fx[i][e], both(-c2), add2(fd[i][e], both(-c1))), both(rstd));
+      store_piece(dx, at + i * tpr, reinterpret_cast<const float*>(fd[i]), shift - p * n, shift + C - p * n);
     }
   }
   if (part == nullptr) return;
@@ -306,11 +318,10 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, const f
     for (int e = 0; e < n; ++e) {
       const int c = (t + i * tpr) * n + e - shift;
       if (!in_row(c, C)) continue;
-      float* to = kBlockRow ? out : s_part + (size_t)group * 2 * C;
-      to[c] = sg[i * n + e];
-      to[C + c] = sb[i * n + e];
+      float* to = s_part + (size_t)group * 2 * C;
+      to[c] = reinterpret_cast<const float*>(sg[i])[e];
+      to[C + c] = reinterpret_cast<const float*>(sb[i])[e];
     }
-  if (kBlockRow) return;
   __syncthreads();
   for (int c = threadIdx.x; c < 2 * C; c += blockDim.x) {
     float s = 0.f;
@@ -337,6 +348,270 @@ __global__ void __launch_bounds__(32 * kAddRows) layer_norm_add_kernel(const flo
   if (to != nullptr) to[c < C ? c : c - C] = (float)v;
 }
 
+// ---- rows that a block shares: through a ring in shared memory --------------------------------------------------------------------
+// A block's sums have barriers in between, and what hides them is rows on their way: one lane asks for rows ahead with bulk copies, of
+// the 16-byte pieces that a row lies in.  Gain and shift lie in shared memory too, moved by the rows' shift.
+constexpr int kRing = 3;
+
+__device__ __forceinline__ void row_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+
+// Where the rows of a block lie.  The last piece of the tensor may be cut short: it is read by itself (tail).
+template <typename T>
+struct RowSpan {
+  static constexpr int n = Piece<T>::n;
+  long long total;
+  int C, shift, pieces;
+  __device__ __forceinline__ long long first_piece(long long r) const { return (r * C - shift) / n; }
+  __device__ __forceinline__ int whole_pieces(long long r) const {
+    const long long left = total / n - first_piece(r);
+    return left < pieces ? (int)left : pieces;
+  }
+};
+
+template <typename T, int kNV>
+__global__ void __launch_bounds__(kWideBlock, 2)
+layer_norm_row_fwd_kernel(const T* __restrict__ x, const float* __restrict__ gamma, const float* __restrict__ beta, float eps, long long rows, int C,
+                          int slot_bytes, T* __restrict__ y, float* __restrict__ stats, int* status) {
+  constexpr int n = Piece<T>::n;
+  using namespace attn;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ __align__(8) uint64_t s_full[kRing];
+  __shared__ float s_sum[64];
+  __shared__ int s_abort_i;
+  const int t = threadIdx.x, tpr = blockDim.x;
+  if (t == 0) {
+    for (int s = 0; s < kRing; ++s) tc::mbar_init(tc::smem_u32(&s_full[s]), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    s_abort_i = 0;
+  }
+  __syncthreads();
+  pdl_sync();
+  RowSpan<T> span{rows * C, C, (int)(((long long)blockIdx.x * C) % n), 0};
+  span.pieces = (span.shift + C + n - 1) / n;
+  const int shift = span.shift, pieces = span.pieces, pad = pieces * n;
+  float* s_g = reinterpret_cast<float*>(smem + kRing * slot_bytes);
+  float* s_b = s_g + pad;
+  const uint32_t ring = tc::smem_u32(smem);
+  // four elements of each piece, then the other four: neighbouring threads read neighbouring 16 bytes
+  auto place = [&](int i) { return (i % n / 4 * pieces + i / n) * 4 + i % 4; };
+  auto ask = [&](long long r, int s) {
+    const uint32_t bytes = span.whole_pieces(r) * 16, bar = tc::smem_u32(&s_full[s]);
+    tc::mbar_expect_tx(bar, bytes);
+    if (bytes) row_copy(ring + s * slot_bytes, reinterpret_cast<const uint4*>(x) + span.first_piece(r), bytes, bar);
+  };
+  if (t == 0)
+    for (int s = 0; s < kRing; ++s)
+      if (blockIdx.x + (long long)s * gridDim.x < rows) ask(blockIdx.x + (long long)s * gridDim.x, s);
+  for (int i = t; i < pad; i += tpr) {
+    const bool in = in_row(i - shift, C);
+    s_g[place(i)] = in && gamma != nullptr ? gamma[i - shift] : 1.f;
+    s_b[place(i)] = in && beta != nullptr ? beta[i - shift] : 0.f;
+  }
+  __syncthreads();
+  const float inv = 1.f / (float)C;
+  int turn = 0, s = 0, phase = 0;
+  bool ok = true;
+  for (long long r = blockIdx.x; r < rows; r += gridDim.x) {
+    ok = ok && tc::mbar_wait(tc::smem_u32(&s_full[s]), phase, &s_abort_i);
+    if (!ok) s_abort_i = 1;      // (the block's barriers are passed all the same)
+    const int whole = span.whole_pieces(r);
+    float2 f[kNV][n / 2], m2 = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < kNV; ++i) {
+      const int p = t + i * tpr;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (p < whole) v = *reinterpret_cast<const uint4*>(smem + s * slot_bytes + p * 16);
+      else if (p < pieces) v = load_piece(x, span.first_piece(r) + p, span.total);
+      pairs_of<T>(v, f[i]);
+      if (!whole_piece<n>(p, shift, C)) keep_row<n>(f[i], p, shift, C);
+#pragma unroll
+      for (int e = 0; e < n / 2; ++e) m2 = add2(m2, f[i][e]);
+    }
+    float m[1] = {m2.x + m2.y};
+    block_sum<1>(m, tpr, s_sum, turn);
+    // behind the barrier nobody reads the slot any more
+    if (t == 0 && r + (long long)kRing * gridDim.x < rows) ask(r + (long long)kRing * gridDim.x, s);
+    const float mean = m[0] * inv;
+    float2 q2 = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < kNV; ++i) {
+      const int p = t + i * tpr;
+#pragma unroll
+      for (int e = 0; e < n / 2; ++e) f[i][e] = add2(f[i][e], both(-mean));
+      if (!whole_piece<n>(p, shift, C)) keep_row<n>(f[i], p, shift, C);
+#pragma unroll
+      for (int e = 0; e < n / 2; ++e) q2 = fma2(f[i][e], f[i][e], q2);
+    }
+    float q[1] = {q2.x + q2.y};
+    block_sum<1>(q, tpr, s_sum, turn);
+    const float rstd = 1.f / sqrtf(q[0] * inv + eps);
+    const long long at = span.first_piece(r);
+#pragma unroll
+    for (int i = 0; i < kNV; ++i) {
+      const int p = t + i * tpr;
+      if (p < pieces) {
+#pragma unroll
+        for (int e = 0; e < n / 2; e += 2) {
+          const float4 g = *reinterpret_cast<const float4*>(s_g + (e / 2 * pieces + p) * 4), b = *reinterpret_cast<const float4*>(s_b + (e / 2 * pieces + p) * 4);
+          f[i][e] = fma2(mul2(f[i][e], both(rstd)), make_float2(g.x, g.y), make_float2(b.x, b.y));
+          f[i][e + 1] = fma2(mul2(f[i][e + 1], both(rstd)), make_float2(g.z, g.w), make_float2(b.z, b.w));
+        }
+        store_piece(y, at + p, reinterpret_cast<const float*>(f[i]), shift - p * n, shift + C - p * n);
+      }
+    }
+    if (stats != nullptr && t == 0) {
+      stats[r] = mean;
+      stats[rows + r] = rstd;
+    }
+    if (++s == kRing) { s = 0; phase ^= 1; }
+  }
+  __syncthreads();
+  if (s_abort_i) {
+    if (t == 0) set_status(status, kMbarTimeout, 44, (int)blockIdx.x);
+    for (int i = 0; i < 2000; ++i) __nanosleep(1000);        // copies in flight land
+  }
+}
+
+template <typename T, int kNV>
+__global__ void __launch_bounds__(kWideBlock)
+layer_norm_row_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, const float* __restrict__ stats, const float* __restrict__ gamma,
+                          long long rows, int C, int slot_bytes, T* __restrict__ dx, float* __restrict__ part, int* status) {
+  constexpr int n = Piece<T>::n;
+  using namespace attn;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ __align__(8) uint64_t s_full[kRing];
+  __shared__ float s_sum[128];
+  __shared__ int s_abort_i;
+  const int t = threadIdx.x, tpr = blockDim.x;
+  if (t == 0) {
+    for (int s = 0; s < kRing; ++s) tc::mbar_init(tc::smem_u32(&s_full[s]), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    s_abort_i = 0;
+  }
+  __syncthreads();
+  pdl_sync();
+  RowSpan<T> span{rows * C, C, (int)(((long long)blockIdx.x * C) % n), 0};
+  span.pieces = (span.shift + C + n - 1) / n;
+  const int shift = span.shift, pieces = span.pieces, pad = pieces * n;
+  float* s_g = reinterpret_cast<float*>(smem + 2 * kRing * slot_bytes);
+  const uint32_t ring = tc::smem_u32(smem);
+  // four elements of each piece, then the other four: neighbouring threads read neighbouring 16 bytes
+  auto place = [&](int i) { return (i % n / 4 * pieces + i / n) * 4 + i % 4; };
+  auto ask = [&](long long r, int s) {
+    const uint32_t bytes = span.whole_pieces(r) * 16, bar = tc::smem_u32(&s_full[s]);
+    tc::mbar_expect_tx(bar, 2 * bytes);
+    if (bytes) {
+      row_copy(ring + 2 * s * slot_bytes, reinterpret_cast<const uint4*>(x) + span.first_piece(r), bytes, bar);
+      row_copy(ring + (2 * s + 1) * slot_bytes, reinterpret_cast<const uint4*>(dy) + span.first_piece(r), bytes, bar);
+    }
+  };
+  if (t == 0)
+    for (int s = 0; s < kRing; ++s)
+      if (blockIdx.x + (long long)s * gridDim.x < rows) ask(blockIdx.x + (long long)s * gridDim.x, s);
+  for (int i = t; i < pad; i += tpr) s_g[place(i)] = gamma != nullptr && in_row(i - shift, C) ? gamma[i - shift] : 1.f;
+  __syncthreads();
+  const float inv = 1.f / (float)C;
+  float2 sg[kNV][n / 2], sb[kNV][n / 2];
+#pragma unroll
+  for (int i = 0; i < kNV; ++i)
+#pragma unroll
+    for (int e = 0; e < n / 2; ++e) sg[i][e] = sb[i][e] = make_float2(0.f, 0.f);
+  int turn = 0, s = 0, phase = 0;
+  bool ok = true;
+  float mean_next = 0.f, rstd_next = 0.f;
+  if (blockIdx.x < rows) { mean_next = stats[blockIdx.x]; rstd_next = stats[rows + blockIdx.x]; }
+  for (long long r = blockIdx.x; r < rows; r += gridDim.x) {
+    const float mean = mean_next, rstd = rstd_next;
+    if (r + gridDim.x < rows) { mean_next = stats[r + gridDim.x]; rstd_next = stats[rows + r + gridDim.x]; }
+    ok = ok && tc::mbar_wait(tc::smem_u32(&s_full[s]), phase, &s_abort_i);
+    if (!ok) s_abort_i = 1;
+    const int whole = span.whole_pieces(r);
+    uint4 vx[kNV], vd[kNV];
+    float2 m0 = make_float2(0.f, 0.f), m1 = m0;
+    auto gain = [&](int p, float2 (&g)[n / 2]) {
+#pragma unroll
+      for (int e = 0; e < n / 2; e += 2) {
+        const float4 v = *reinterpret_cast<const float4*>(s_g + (e / 2 * pieces + p) * 4);
+        g[e] = make_float2(v.x, v.y);
+        g[e + 1] = make_float2(v.z, v.w);
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < kNV; ++i) {
+      const int p = t + i * tpr;
+      if (p >= pieces) continue;
+      if (p < whole) {
+        vx[i] = *reinterpret_cast<const uint4*>(smem + 2 * s * slot_bytes + p * 16);
+        vd[i] = *reinterpret_cast<const uint4*>(smem + (2 * s + 1) * slot_bytes + p * 16);
+      } else {
+        vx[i] = load_piece(x, span.first_piece(r) + p, span.total);
+        vd[i] = load_piece(dy, span.first_piece(r) + p, span.total);
+      }
+      float2 fx[n / 2], fd[n / 2], g[n / 2];
+      pairs_of<T>(vx[i], fx);
+      pairs_of<T>(vd[i], fd);
+      gain(p, g);
+#pragma unroll
+      for (int e = 0; e < n / 2; ++e) fx[e] = mul2(add2(fx[e], both(-mean)), both(rstd));
+      if (!whole_piece<n>(p, shift, C)) {
+        keep_row<n>(fx, p, shift, C);
+        keep_row<n>(fd, p, shift, C);
+      }
+#pragma unroll
+      for (int e = 0; e < n / 2; ++e) {
+        sb[i][e] = add2(sb[i][e], fd[e]);
+        sg[i][e] = fma2(fd[e], fx[e], sg[i][e]);
+        fd[e] = mul2(fd[e], g[e]);
+        m0 = add2(m0, fd[e]);
+        m1 = fma2(fd[e], fx[e], m1);
+      }
+    }
+    float m[2] = {m0.x + m0.y, m1.x + m1.y};
+    block_sum<2>(m, tpr, s_sum, turn);
+    if (t == 0 && r + (long long)kRing * gridDim.x < rows) ask(r + (long long)kRing * gridDim.x, s);
+    const float c1 = m[0] * inv, c2 = m[1] * inv;
+    const long long at = span.first_piece(r);
+    if (dx != nullptr)
+#pragma unroll
+      for (int i = 0; i < kNV; ++i) {
+        const int p = t + i * tpr;
+        if (p >= pieces) continue;
+        float2 fx[n / 2], fd[n / 2], g[n / 2];
+        pairs_of<T>(vx[i], fx);
+        pairs_of<T>(vd[i], fd);
+        gain(p, g);
+#pragma unroll
+        for (int e = 0; e < n / 2; ++e) {
+          fx[e] = mul2(add2(fx[e], both(-mean)), both(rstd));
+          fd[e] = mul2(fma2(fx[e], both(-c2), fma2(fd[e], g[e], both(-c1))), both(rstd));
+        }
+        store_piece(dx, at + p, reinterpret_cast<const float*>(fd), shift - p * n, shift + C - p * n);
+      }
+    if (++s == kRing) { s = 0; phase ^= 1; }
+  }
+  if (part != nullptr) {
+    float* out = part + (size_t)blockIdx.x * 2 * C;
+#pragma unroll
+    for (int i = 0; i < kNV; ++i)
+#pragma unroll
+      for (int e = 0; e < n; ++e) {
+        const int c = (t + i * tpr) * n + e - shift;
+        if (in_row(c, C)) {
+          out[c] = reinterpret_cast<const float*>(sg[i])[e];
+          out[C + c] = reinterpret_cast<const float*>(sb[i])[e];
+        }
+      }
+  }
+  __syncthreads();
+  if (s_abort_i) {
+    if (t == 0) set_status(status, kMbarTimeout, 45, (int)blockIdx.x);
+    for (int i = 0; i < 2000; ++i) __nanosleep(1000);        // copies in flight land
+  }
+}
+
 // ---- rows too wide for the registers of a block: read again for each sum, out of L2 ----------------------------------------------
 template <typename T>
 __global__ void __launch_bounds__(1024) layer_norm_wide_fwd_kernel(const T* __restrict__ x, const float* __restrict__ gamma,
@@ -349,14 +624,14 @@ __global__ void __launch_bounds__(1024) layer_norm_wide_fwd_kernel(const T* __re
     const T* row = x + r * C;
     float m[1] = {0.f};
     for (int c = threadIdx.x; c < C; c += 1024) m[0] += Piece<T>::get(row[c]);
-    group_sum<true, 1>(m, 1024, s_sum, turn);
+    block_sum<1>(m, 1024, s_sum, turn);
     const float mean = m[0] / (float)C;
     float q[1] = {0.f};
     for (int c = threadIdx.x; c < C; c += 1024) {
       const float d = Piece<T>::get(row[c]) - mean;
       q[0] += d * d;
     }
-    group_sum<true, 1>(q, 1024, s_sum, turn);
+    block_sum<1>(q, 1024, s_sum, turn);
     const float rstd = 1.f / sqrtf(q[0] / (float)C + eps);
     for (int c = threadIdx.x; c < C; c += 1024) {
       const float v = (Piece<T>::get(row[c]) - mean) * rstd;
@@ -384,7 +659,7 @@ __global__ void __launch_bounds__(1024) layer_norm_wide_bwd_kernel(const T* __re
       m[0] += d;
       m[1] += d * (Piece<T>::get(x[r * C + c]) - mean) * rstd;
     }
-    group_sum<true, 2>(m, 1024, s_sum, turn);
+    block_sum<2>(m, 1024, s_sum, turn);
     const float c1 = m[0] / (float)C, c2 = m[1] / (float)C;
     for (int c = threadIdx.x; c < C; c += 1024) {
       const float d = Piece<T>::get(dy[r * C + c]) * (gamma ? gamma[c] : 1.f);
@@ -434,6 +709,10 @@ Plan plan_of(long long rows, int C) {
 }
 
 // As many blocks as fit on the GPU at a time, a multiple of eight: rows of a group then start at one place in a 16-byte piece.
+// of a row in the ring, wherever it starts in a piece
+template <typename T>
+int slot_bytes(int C) { return (C + 2 * (Piece<T>::n - 1)) / Piece<T>::n * 16; }
+
 template <typename K>
 int resident_grid(K kernel, int block, size_t smem, long long blocks) {
   int dev = 0, sms = 148, per_sm = 1;
@@ -446,16 +725,11 @@ int resident_grid(K kernel, int block, size_t smem, long long blocks) {
 }
 
 template <typename T, typename F>
-const char* with_kernel(const Plan& p, F&& f) {
+const char* with_pieces(const Plan& p, F&& f) {
   constexpr int most = kPerThread / Piece<T>::n;
-  if (p.tpr > 32) {
-    if (p.nv == 1) return f(std::integral_constant<int, 1>{}, std::true_type{});
-    if (p.nv == 2) return f(std::integral_constant<int, 2>{}, std::true_type{});
-    return f(std::integral_constant<int, most>{}, std::true_type{});
-  }
-  if (p.nv == 1) return f(std::integral_constant<int, 1>{}, std::false_type{});
-  if (p.nv == 2) return f(std::integral_constant<int, 2>{}, std::false_type{});
-  return f(std::integral_constant<int, most>{}, std::false_type{});
+  if (p.nv == 1) return f(std::integral_constant<int, 1>{});
+  if (p.nv == 2) return f(std::integral_constant<int, 2>{});
+  return f(std::integral_constant<int, most>{});
 }
 
 const char* told(cudaError_t e) {
@@ -473,10 +747,19 @@ const char* fwd(const LayerNormArgs& a, cudaStream_t st) {
     return told(launch_pdl(layer_norm_wide_fwd_kernel<T>, dim3(grid), dim3(1024), 0, st, (const T*)a.x, a.gamma, a.beta, a.eps, a.rows, a.C,
                            (T*)a.y, a.stats));
   }
-  return with_kernel<T>(p, [&](auto nv, auto block_row) {
-    auto* k = layer_norm_fwd_kernel<T, decltype(nv)::value, decltype(block_row)::value>;
-    return told(launch_pdl(k, dim3(resident_grid(k, p.block, 0, p.blocks)), dim3(p.block), 0, st, (const T*)a.x, a.gamma, a.beta, a.eps, a.rows,
-                           a.C, p.tpr, (T*)a.y, a.stats));
+  return with_pieces<T>(p, [&](auto nv) -> const char* {
+    constexpr int kNV = decltype(nv)::value;
+    if (p.tpr <= 32) {
+      auto* k = layer_norm_fwd_kernel<T, kNV>;
+      return told(launch_pdl(k, dim3(resident_grid(k, p.block, 0, p.blocks)), dim3(p.block), 0, st, (const T*)a.x, a.gamma, a.beta, a.eps, a.rows,
+                             a.C, p.tpr, (T*)a.y, a.stats));
+    }
+    auto* k = layer_norm_row_fwd_kernel<T, kNV>;
+    const int slot = slot_bytes<T>(a.C);
+    const size_t smem = kRing * slot + 2 * slot / sizeof(T) * sizeof(float);
+    cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);      // of the current device
+    return told(launch_pdl(k, dim3(resident_grid(k, p.block, smem, p.blocks)), dim3(p.block), smem, st, (const T*)a.x, a.gamma, a.beta, a.eps,
+                           a.rows, a.C, slot, (T*)a.y, a.stats, a.status));
   });
 }
 
@@ -500,15 +783,29 @@ const char* bwd(const LayerNormArgs& a, int* part_rows, cudaStream_t st) {
     }
     return nullptr;
   }
-  return with_kernel<T>(p, [&](auto nv, auto block_row) -> const char* {
-    auto* k = layer_norm_bwd_kernel<T, decltype(nv)::value, decltype(block_row)::value>;
-    const size_t smem = p.tpr > 32 ? 0 : (size_t)p.per_block * 2 * a.C * sizeof(float);      // at most 32 KiB: a thread has 16 elements
-    const int grid = resident_grid(k, p.block, smem, p.blocks);
+  return with_pieces<T>(p, [&](auto nv) -> const char* {
+    constexpr int kNV = decltype(nv)::value;
+    int grid;
+    const char* err = nullptr;
+    if (p.tpr <= 32) {
+      auto* k = layer_norm_bwd_kernel<T, kNV>;
+      const size_t smem = (size_t)p.per_block * 2 * a.C * sizeof(float);      // at most 32 KiB: a thread has 16 elements
+      grid = resident_grid(k, p.block, smem, p.blocks);
+      if (!part_rows)
+        err = told(launch_pdl(k, dim3(grid), dim3(p.block), smem, st, (const T*)a.dy, (const T*)a.x, a.stats, a.gamma, a.rows, a.C, p.tpr, (T*)a.dx,
+                              sums ? a.part : nullptr));
+    } else {
+      auto* k = layer_norm_row_bwd_kernel<T, kNV>;
+      const int slot = slot_bytes<T>(a.C);
+      const size_t smem = 2 * kRing * slot + slot / sizeof(T) * sizeof(float);
+      cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);      // of the current device
+      grid = resident_grid(k, p.block, smem, p.blocks);
+      if (!part_rows)
+        err = told(launch_pdl(k, dim3(grid), dim3(p.block), smem, st, (const T*)a.dy, (const T*)a.x, a.stats, a.gamma, a.rows, a.C, slot, (T*)a.dx,
+                              sums ? a.part : nullptr, a.status));
+    }
     if (part_rows) { *part_rows = grid; return nullptr; }
-    if (const char* err = told(launch_pdl(k, dim3(grid), dim3(p.block), smem, st, (const T*)a.dy, (const T*)a.x, a.stats, a.gamma, a.rows, a.C,
-                                          p.tpr, (T*)a.dx, sums ? a.part : nullptr)))
-      return err;
-    if (!sums) return nullptr;
+    if (err || !sums) return err;
     return told(launch_pdl(layer_norm_add_kernel, dim3((2 * a.C + 31) / 32), dim3(32 * kAddRows), 0, st, a.part, grid, a.C, a.dgamma, a.dbeta));
   });
 }

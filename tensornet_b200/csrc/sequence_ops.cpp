@@ -26,6 +26,13 @@ void once_differentiable(const char* what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), what, " is differentiable once: its backward pass builds no graph");
 }
 
+// The runtime's status words, where a wait that runs out is told
+int* status_of(const at::Tensor& status, const at::Tensor& x) {
+  TORCH_CHECK(status.device() == x.device() && status.scalar_type() == at::kInt, "operands must be on the runtime's GPU, ", status.device(), ", not on ",
+              x.device());
+  return status.data_ptr<int>();
+}
+
 // ---- layer normalisation ------------------------------------------------------------------------------------------------------
 // `t` as [rows, C], contiguous from a 16-byte boundary
 at::Tensor rows16(const at::Tensor& t, int64_t C) {
@@ -52,13 +59,13 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     return a;
   }
 
-  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const OptTensor& gamma, const OptTensor& beta, double eps, bool keep) {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const OptTensor& gamma, const OptTensor& beta, double eps, const at::Tensor& status, bool keep) {
     c10::cuda::CUDAGuard guard(x.device());
     const int64_t C = x.size(-1);
     at::Tensor x2 = rows16(x, C), y = at::empty_like(x2), stats, kg, kb;
     tn::LayerNormArgs a = args_of(x2);
     a.gamma = column_vec(gamma, x, "gamma", kg); a.beta = column_vec(beta, x, "beta", kb);
-    a.eps = (float)eps; a.y = y.data_ptr();
+    a.eps = (float)eps; a.y = y.data_ptr(); a.status = status_of(status, x);
     if (keep) {
       stats = at::empty({2, a.rows}, x2.options().dtype(at::kFloat));
       a.stats = stats.data_ptr<float>();
@@ -68,6 +75,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
       const bool has_gamma = gamma && gamma->defined(), has_beta = beta && beta->defined();
       ctx->save_for_backward({x2.data_ptr() == x.data_ptr() ? x : x2, stats, has_gamma ? *gamma : at::Tensor()});
       ctx->saved_data["gamma"] = has_gamma ? 1 : -1;                      // the place among the arguments that are tensors
+      ctx->saved_data["status"] = status;
       ctx->saved_data["beta"] = has_beta ? (has_gamma ? 2 : 1) : -1;
     }
     return y.view(x.sizes());
@@ -81,6 +89,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     const int64_t C = x.size(-1);
     at::Tensor x2 = x.view({x.numel() / C, C}), dy = rows16(grads[0], C), kg, dx, dg, db, part;
     tn::LayerNormArgs a = args_of(x2);
+    a.status = status_of(ctx->saved_data["status"].toTensor(), x);
     a.dy = dy.data_ptr(); a.stats = stats.data_ptr<float>(); a.gamma = column_vec(some(gamma), x2, "gamma", kg);
     const auto f32 = x2.options().dtype(at::kFloat);
     if (ctx->needs_input_grad(0)) { dx = at::empty_like(x2); a.dx = dx.data_ptr(); }
@@ -98,13 +107,13 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
       if (dg.defined()) dg.zero_();
       if (db.defined()) db.zero_();
     }
-    return {dx.defined() ? dx.view(grads[0].sizes()) : dx, dg, db, at::Tensor(), at::Tensor()};
+    return {dx.defined() ? dx.view(grads[0].sizes()) : dx, dg, db, at::Tensor(), at::Tensor(), at::Tensor()};
   }
 };
 
-at::Tensor layer_norm(const at::Tensor& x, const OptTensor& gamma, const OptTensor& beta, double eps) {
+at::Tensor layer_norm(const at::Tensor& x, const OptTensor& gamma, const OptTensor& beta, double eps, const at::Tensor& status) {
   const bool keep = at::GradMode::is_enabled() && (x.requires_grad() || wanted(gamma) || wanted(beta));
-  return LayerNorm::apply(x, gamma, beta, eps, keep);
+  return LayerNorm::apply(x, gamma, beta, eps, status, keep);
 }
 
 // ---- attention ------------------------------------------------------------------------------------------------------------------
@@ -142,7 +151,6 @@ struct Attention : torch::autograd::Function<Attention> {
     TORCH_CHECK(k.sizes() == v.sizes(), "attention: keys and values differ in shape");
     TORCH_CHECK(q.size(-1) % 8 == 0 && q.size(-1) >= 8 && q.size(-1) <= 128, "attention: 8 to 128 columns, a multiple of 8");
     TORCH_CHECK(k.size(-2) >= 1 && q.size(-2) % k.size(-2) == 0 && q.size(-2) <= 65535, "attention: query heads must be a multiple of the key heads");
-    TORCH_CHECK(status.device() == q.device() && status.scalar_type() == at::kInt, "attention: operands must be on the runtime's GPU");
     tn::AttnArgs a{};
     a.H = (int)q.size(-2); a.G = (int)k.size(-2); a.D = (int)q.size(-1);
     const bool pq = q.dim() == 3, pk = k.dim() == 3;
@@ -163,7 +171,7 @@ struct Attention : torch::autograd::Function<Attention> {
                   "attention: slopes must be fp32, one per query head");
       a.slopes = slopes->data_ptr<float>();
     }
-    a.causal = causal; a.cap = (float)cap; a.scale = (float)scale; a.status = status.data_ptr<int>();
+    a.causal = causal; a.cap = (float)cap; a.scale = (float)scale; a.status = status_of(status, q);
     return a;
   }
 
@@ -181,7 +189,7 @@ struct Attention : torch::autograd::Function<Attention> {
         lse = at::empty({a.H, q.numel() / (a.H * a.D)}, q.options().dtype(at::kFloat));
         a.lse = lse.data_ptr<float>();
       }
-      if (tn::attention_short_takes(a)) {
+      if (tn::attention_short_takes(a, false)) {
         told(tn::launch_attention_short_fwd(a, counted_stream()));
       } else if (tn::attention_few_takes(a)) {
         at::Tensor work;

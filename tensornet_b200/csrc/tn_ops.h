@@ -130,6 +130,7 @@ struct LayerNormArgs {
   void* dx;                             // null: not wanted
   float* dgamma;                        // [C]; null: not wanted
   float* dbeta;
+  int* status;
   float* part;                          // workspace of bwd where dgamma or dbeta is wanted: layer_norm_part_rows() x [2][C]
 };
 const char* launch_layer_norm_fwd(const LayerNormArgs& a, cudaStream_t st);

@@ -669,7 +669,7 @@ def layer_norm(x: torch.Tensor, gamma: Optional[torch.Tensor] = None, beta: Opti
     if not 0.0 < eps < float("inf"):
         raise ValueError(f"layer_norm: eps must be above zero, not {eps}")
     if x.is_cuda:
-        return _ext().layer_norm(x, gamma, beta, eps)
+        return _ext().layer_norm(x, gamma, beta, eps, _status())
     f = x.float()
     c = f - f.mean(dim=-1, keepdim=True)
     y = c / torch.sqrt((c * c).mean(dim=-1, keepdim=True) + eps)
