@@ -22,6 +22,7 @@ struct AttnArgs {
   int B, H, G, D;              // sequences, query heads, key heads (H a multiple of G), columns (a multiple of 8, up to 128)
   AttnRows rq, rk;
   AttnOperand q, k, v, o;      // o: written forward, read backward
+  AttnOperand rest;            // what rounding took off o, rounded itself (p null: not kept); the backward pass sums do (o + rest)
   float* lse;                  // [H][rows of q] log2 of the sums of exponentials, +inf where a row sees nothing; forward: may be null
   float scale;                 // of the products, above 0
   float cap;                   // 0: none

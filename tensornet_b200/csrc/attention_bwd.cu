@@ -1,6 +1,8 @@
 // Attention within sequences, backward, on the tensor cores.
 //
 //   p = 2^(s - lse);  dp = do v^T;  ds = p (dp - delta) ds/dx  with delta = sum(do o)
+// (o with what rounding it to bf16 took off: without, gradients of sequences of 40 were off by 0.0030 of their norm, now by 0.0024,
+// where rounding them in the end alone takes 0.0017)
 //   dv = p^T do;  dk = scale ds^T q;  dq = scale ds k
 //
 // Every result has one owner, so no sums meet in memory and their order is fixed: a block owns 128 keys and walks over the queries
@@ -432,7 +434,7 @@ attention_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, const __grid_const
     bwd_block<kD, false, kCap, kBias>(maps, a, sh, smem_raw, query_tiles - 1 - (at - key_tiles * a.G) / a.H, (at - key_tiles * a.G) % a.H);
 }
 
-// delta[h][row] = sum over the columns of do o; `lanes` threads, a power of two, per row of a head
+// delta[h][row] = sum over the columns of do (o + rest); `lanes` threads, a power of two, per row of a head
 __global__ void __launch_bounds__(256) attention_delta_kernel(const AttnArgs a, long long rows, int lanes) {
   pdl_sync();
   const long long at_row = ((long long)blockIdx.x * 256 + threadIdx.x) / lanes;
@@ -444,10 +446,12 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(const AttnArgs a, 
     const int b = a.rq.off ? 0 : (int)(row / a.rq.T);
     const long long t = a.rq.off ? row : row % a.rq.T;
     const uint4 x = *reinterpret_cast<const uint4*>(at(a.go, b, t, h) + lane * 8), y = *reinterpret_cast<const uint4*>(at(a.o, b, t, h) + lane * 8);
-    const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+    const uint4 z = *reinterpret_cast<const uint4*>(at(a.rest, b, t, h) + lane * 8);
+    const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w}, zw[4] = {z.x, z.y, z.z, z.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      v += __uint_as_float(xw[i] << 16) * __uint_as_float(yw[i] << 16) + __uint_as_float(xw[i] & 0xffff0000u) * __uint_as_float(yw[i] & 0xffff0000u);
+      v += __uint_as_float(xw[i] << 16) * (__uint_as_float(yw[i] << 16) + __uint_as_float(zw[i] << 16)) +
+           __uint_as_float(xw[i] & 0xffff0000u) * (__uint_as_float(yw[i] & 0xffff0000u) + __uint_as_float(zw[i] & 0xffff0000u));
   }
   for (int o = lanes / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   if (row < rows && lane == 0) a.delta[h * rows + row] = v;

@@ -246,11 +246,15 @@ attention_few_kernel(const __grid_constant__ FewMaps maps, const __grid_constant
         for (int f = 0; f < 2; ++f) {
           const int d = column(p, f);
           if (d >= a.D) continue;
-          uint32_t v[S::v_words];
+          uint32_t v[S::v_words], rest[S::v_words];
 #pragma unroll
-          for (int k = 0; k < S::v_words; ++k)
-            v[k] = pack_bf16(o[p * S::v_cols + 2 * k][2 * r + f] * w, o[p * S::v_cols + 2 * k + 1][2 * r + f] * w);
+          for (int k = 0; k < S::v_words; ++k) {
+            const float x = o[p * S::v_cols + 2 * k][2 * r + f] * w, y = o[p * S::v_cols + 2 * k + 1][2 * r + f] * w;
+            v[k] = pack_bf16(x, y);
+            rest[k] = rest_of(x, y, v[k]);
+          }
           store_words<S::v_words>(out + d, v);
+          if (a.rest.p != nullptr) store_words<S::v_words>(at_out(a.rest, seq, i, h) + d, rest);
         }
       if (a.lse != nullptr && t == 0) a.lse[h * q_rows + (long long)seq * a.rq.T + i] = l[r] > 0.f ? m[r] + log2f(l[r]) : CUDART_INF_F;
     }
@@ -294,7 +298,9 @@ attention_few_kernel(const __grid_constant__ FewMaps maps, const __grid_constant
     }
     const int i = row / R, h = kh * R + row % R;
     const float w = sum > 0.f ? 1.f / sum : 0.f;
-    *reinterpret_cast<uint32_t*>(at_out(a.o, seq, i, h) + d) = pack_bf16(x * w, y * w);
+    const uint32_t v = pack_bf16(x * w, y * w);
+    *reinterpret_cast<uint32_t*>(at_out(a.o, seq, i, h) + d) = v;
+    if (a.rest.p != nullptr) *reinterpret_cast<uint32_t*>(at_out(a.rest, seq, i, h) + d) = rest_of(x * w, y * w, v);
     if (a.lse != nullptr && d == 0) a.lse[h * q_rows + (long long)seq * a.rq.T + i] = sum > 0.f ? all + log2f(sum) : CUDART_INF_F;
   }
 }
@@ -344,7 +350,9 @@ __global__ void __launch_bounds__(kJoin) attention_few_join_kernel(const __grid_
   for (int k = 0; k < kTurns; ++k) sum += s_sum[k];
   const int i = row / R, h = kh * R + row % R;
   const float w = sum > 0.f ? 1.f / sum : 0.f;
-  *reinterpret_cast<uint32_t*>(at_out(a.o, seq, i, h) + pair * 2) = pack_bf16(x * w, y * w);
+  const uint32_t v = pack_bf16(x * w, y * w);
+  *reinterpret_cast<uint32_t*>(at_out(a.o, seq, i, h) + pair * 2) = v;
+  if (a.rest.p != nullptr) *reinterpret_cast<uint32_t*>(at_out(a.rest, seq, i, h) + pair * 2) = rest_of(x * w, y * w, v);
   if (a.lse != nullptr && pair == 0) a.lse[h * ((long long)a.B * a.rq.T) + (long long)seq * a.rq.T + i] = sum > 0.f ? all + log2f(sum) : CUDART_INF_F;
 }
 

@@ -103,7 +103,9 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
   if (most == 0) {
     const int per = a.D / 8;
     for (int i = threadIdx.x; i < tile_rows * per; i += Shape::threads)
-      *reinterpret_cast<uint4*>(at_out(a.o, tile.rows.b, tile.rows.first + tile.first + i / per, h) + i % per * 8) = make_uint4(0, 0, 0, 0);
+      for (const AttnOperand* to : {&a.o, &a.rest})
+        if (to->p != nullptr)
+          *reinterpret_cast<uint4*>(at_out(*to, tile.rows.b, tile.rows.first + tile.first + i / per, h) + i % per * 8) = make_uint4(0, 0, 0, 0);
     if (a.lse != nullptr && tile.seq >= 0)
       for (int i = threadIdx.x; i < tile_rows; i += Shape::threads)
         a.lse[(long long)h * (a.rq.off ? a.rq.T : (long long)a.B * a.rq.T) + (a.rq.off ? 0 : (long long)tile.rows.b * a.rq.T) + tile.rows.first +
@@ -385,8 +387,14 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
           const bool some = w != 0.f;         // (what a row without weights holds may be anything)
 #pragma unroll
           for (int e = 0; e < 16; ++e) o[e] = some ? o[e] : 0.f;
-          *reinterpret_cast<uint4*>(out + c0) = pack8(o, w);
-          if (c0 + 8 < a.D) *reinterpret_cast<uint4*>(out + c0 + 8) = pack8(o + 8, w);
+          __nv_bfloat16* rest = a.rest.p ? at_out(a.rest, tile.rows.b, row, h) : nullptr;
+#pragma unroll
+          for (int e = 0; e < 16; e += 8)
+            if (c0 + e < a.D) {
+              const uint4 v = pack8(o + e, w);
+              *reinterpret_cast<uint4*>(out + c0 + e) = v;
+              if (rest) *reinterpret_cast<uint4*>(rest + c0 + e) = rest8(o + e, w, v);
+            }
         }
         __syncwarp();
       }

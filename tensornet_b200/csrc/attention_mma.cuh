@@ -34,6 +34,11 @@ __device__ __forceinline__ void store_words(__nv_bfloat16* p, const uint32_t* w)
   else *reinterpret_cast<uint32_t*>(p) = w[0];
 }
 
+// Two fp32 values rounded to bf16, and what that took off
+__device__ __forceinline__ uint32_t rest_of(float a, float b, uint32_t r) {
+  return pack_bf16(a - __uint_as_float(r << 16), b - __uint_as_float(r & 0xffff0000u));
+}
+
 // Pieces of a row of up to kD columns
 template <int kD>
 struct Pieces {

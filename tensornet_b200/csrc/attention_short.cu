@@ -92,7 +92,8 @@ __device__ __forceinline__ void mma_scores(float (*s)[4], const uint32_t (*x)[2]
   }
 }
 // The lane has of row g + 8 r the columns (8 p + 2 t + f) vc + i: acc[p vc + i][2 r + f], two runs of vc columns side by side.
-template <int kD>
+// kRest: not the rounded values, but what rounding took off them
+template <int kD, bool kRest = false>
 __device__ __forceinline__ void store_rows(const AttnOperand& to, int b, long long first, int there, int filled, int h, int D, int g, int t,
                                            const float (*acc)[4], const float* w) {
   using P = Pieces<kD>;
@@ -108,7 +109,11 @@ __device__ __forceinline__ void store_rows(const AttnOperand& to, int b, long lo
       for (int f = 0; f < 2; ++f)
 #pragma unroll
         for (int k = 0; k < P::v_words; ++k)
-          v[f * P::v_words + k] = x < filled ? pack_bf16(acc[p * P::v_cols + 2 * k][2 * r + f] * w[r], acc[p * P::v_cols + 2 * k + 1][2 * r + f] * w[r]) : 0u;
+          {
+            const float x0 = acc[p * P::v_cols + 2 * k][2 * r + f] * w[r], x1 = acc[p * P::v_cols + 2 * k + 1][2 * r + f] * w[r];
+            const uint32_t both = pack_bf16(x0, x1);
+            v[f * P::v_words + k] = x >= filled ? 0u : kRest ? rest_of(x0, x1, both) : both;
+          }
       const int d = (p * 8 + 2 * t) * P::v_cols;
       if constexpr (P::v_words <= 2) {
         if (d + 2 * P::v_cols <= D) store_words<2 * P::v_words>(row + d, v);
@@ -237,6 +242,7 @@ __global__ void __launch_bounds__(32 * kWarps, kD == 16 ? 6 : kD == 32 ? 4 : 3) 
       if (a.lse != nullptr && t == 0 && x0 + g + 8 * r < qs.n) a.lse[h * q_rows + flat + 8 * r] = sum > 0.f ? m[r] + __log2f(sum) : CUDART_INF_F;
     }
     store_rows<kD>(a.o, tile.rows.b, tile.rows.first + x0, tile.rows.n - x0, qs.n - x0, h, a.D, g, t, o, w);
+    if (a.rest.p != nullptr) store_rows<kD, true>(a.rest, tile.rows.b, tile.rows.first + x0, tile.rows.n - x0, qs.n - x0, h, a.D, g, t, o, w);
   }
 }
 

@@ -142,6 +142,18 @@ __device__ __forceinline__ uint4 pack8(const float* f, float w) {
   return make_uint4(pack_bf16(f[0] * w, f[1] * w), pack_bf16(f[2] * w, f[3] * w), pack_bf16(f[4] * w, f[5] * w), pack_bf16(f[6] * w, f[7] * w));
 }
 
+// What is left of eight fp32 values times w when pack8 has rounded them
+__device__ __forceinline__ uint4 rest8(const float* f, float w, const uint4& r) {
+  const uint32_t v[4] = {r.x, r.y, r.z, r.w};
+  float d[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    d[2 * i] = f[2 * i] * w - __uint_as_float(v[i] << 16);
+    d[2 * i + 1] = f[2 * i + 1] * w - __uint_as_float(v[i] & 0xffff0000u);
+  }
+  return pack8(d, 1.f);
+}
+
 // [rows, 64 columns] boxes of an operand; columns beyond D and rows beyond T come as zeros
 bool operand_map(const AttnOperand& o, int D, const AttnRows& r, int B, int heads, int box_rows, CUtensorMap* out);
 

@@ -181,13 +181,15 @@ struct Attention : torch::autograd::Function<Attention> {
     c10::cuda::CUDAGuard guard(q_in.device());
     const at::Tensor q = operand(q_in), k = operand(k_in), v = operand(v_in);
     tn::AttnArgs a = args_of(q, k, v, q_rows, k_rows, prefix, slopes, causal, cap, scale, status);
-    at::Tensor out = at::empty(q.sizes(), q.options()), lse;
+    at::Tensor out = at::empty(q.sizes(), q.options()), lse, rest;
     a.o = view_of(out);
     if (out.numel() > 0 && k.numel() == 0) out.zero_();
     if (out.numel() > 0 && k.numel() > 0) {
       if (keep) {
         lse = at::empty({a.H, q.numel() / (a.H * a.D)}, q.options().dtype(at::kFloat));
         a.lse = lse.data_ptr<float>();
+        rest = at::empty_like(out);
+        a.rest = view_of(rest);
       }
       if (tn::attention_short_takes(a, false)) {
         told(tn::launch_attention_short_fwd(a, counted_stream()));
@@ -204,7 +206,7 @@ struct Attention : torch::autograd::Function<Attention> {
     }
     if (keep) {
       auto opt = [](const OptTensor& t) { return t ? *t : at::Tensor(); };
-      ctx->save_for_backward({q, k, v, out, lse, opt(q_rows), opt(k_rows), opt(prefix), opt(slopes)});
+      ctx->save_for_backward({q, k, v, out, lse, rest, opt(q_rows), opt(k_rows), opt(prefix), opt(slopes)});
       ctx->saved_data["causal"] = causal;
       ctx->saved_data["cap"] = cap;
       ctx->saved_data["scale"] = scale;
@@ -216,16 +218,16 @@ struct Attention : torch::autograd::Function<Attention> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     once_differentiable("attention");
     const auto s = ctx->get_saved_variables();
-    const at::Tensor &q = s[0], &k = s[1], &v = s[2], &out = s[3], &lse = s[4];
+    const at::Tensor &q = s[0], &k = s[1], &v = s[2], &out = s[3], &lse = s[4], &rest = s[5];
     c10::cuda::CUDAGuard guard(q.device());
     const at::Tensor go = operand(grads[0]);
-    tn::AttnArgs a = args_of(q, k, v, some(s[5]), some(s[6]), some(s[7]), some(s[8]), ctx->saved_data["causal"].toBool(),
+    tn::AttnArgs a = args_of(q, k, v, some(s[6]), some(s[7]), some(s[8]), some(s[9]), ctx->saved_data["causal"].toBool(),
                              ctx->saved_data["cap"].toDouble(), ctx->saved_data["scale"].toDouble(), ctx->saved_data["status"].toTensor());
     TORCH_CHECK(go.scalar_type() == at::kBFloat16 && go.sizes() == q.sizes(), "attention: the output's gradient must be like the output");
     at::Tensor gq = at::empty(q.sizes(), q.options()), gk = at::empty(k.sizes(), k.options()), gv = at::empty(v.sizes(), v.options());
     if (q.numel() > 0 && k.numel() > 0) {
       at::Tensor delta = at::empty_like(lse);
-      a.o = view_of(out); a.go = view_of(go); a.gq = view_of(gq); a.gk = view_of(gk); a.gv = view_of(gv);
+      a.o = view_of(out); a.rest = view_of(rest); a.go = view_of(go); a.gq = view_of(gq); a.gk = view_of(gk); a.gv = view_of(gv);
       a.lse = lse.data_ptr<float>(); a.delta = delta.data_ptr<float>();
       count_launches(1);
       told(tn::launch_attention_bwd(a, counted_stream()));
