@@ -335,7 +335,7 @@ __device__ __forceinline__ void short_bwd(const AttnArgs& a, int tile_at, int he
         mma_scores<kD>(reinterpret_cast<float(*)[4]>(s), x1, w1);
         mma_scores<kD>(reinterpret_cast<float(*)[4]>(d), x2, w2);
         const bool masked = y0 < all_lo || y0 + 16 > all_hi;
-        uint32_t da[4], pa[4];
+        uint32_t da[4], dr[4], pa[4];      // ds and what rounding took off it: products cost little here, and few terms average little out
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -363,10 +363,14 @@ __device__ __forceinline__ void short_bwd(const AttnArgs& a, int tile_at, int he
               if (!(n > 1 && k <= 1)) p.y = ds.y = 0.f;
             }
             da[2 * c + r] = pack_bf16(ds.x, ds.y);
+            dr[2 * c + r] = rest_of(ds.x, ds.y, da[2 * c + r]);
             if (kKeys) pa[2 * c + r] = pack_bf16(p.x, p.y);
           }
 #pragma unroll
-        for (int pc = 0; pc < P::v_pieces; ++pc) mma_values<P::v_words>(acc1 + pc * P::v_cols, da, u1[pc]);
+        for (int pc = 0; pc < P::v_pieces; ++pc) {
+          mma_values<P::v_words>(acc1 + pc * P::v_cols, da, u1[pc]);
+          mma_values<P::v_words>(acc1 + pc * P::v_cols, dr, u1[pc]);
+        }
         if (kKeys)
 #pragma unroll
           for (int pc = 0; pc < P::v_pieces; ++pc) mma_values<P::v_words>(acc2 + pc * P::v_cols, pa, u2[pc]);
