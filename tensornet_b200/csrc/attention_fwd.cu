@@ -68,7 +68,7 @@ struct FwdMaps {
 
 template <int kD, int kTiles, bool kCap, bool kBias>
 __global__ void __launch_bounds__(FwdShape<kD, kTiles, kCap ? 2 : 1>::threads, kTiles == 2 ? 1 : 2)
-attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_constant__ AttnArgs a) {
+attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_constant__ AttnArgs a, int tiles, int heads_first) {
   constexpr int kHalves = kCap ? 2 : 1, kHalf = kRows / kHalves;      // threads per query, keys of a step per thread
   using Shape = FwdShape<kD, kTiles, kHalves>;
   constexpr int kSlots = Shape::slots;
@@ -79,12 +79,13 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
   __shared__ int s_abort_i;
   volatile int* s_abort = &s_abort_i;
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
-  const int h = blockIdx.y;
+  const int h = heads_first ? blockIdx.x % a.H : blockIdx.x / tiles;
 
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  // the last tiles of causal sequences have the most keys: they go first
-  const Tile tile = tile_of(a.rq, a.B, kRows * kTiles, (int)(gridDim.x - 1 - blockIdx.x));
+  // The last tiles of causal sequences have the most keys: they go first, those of all heads (8192 tokens x 16 heads, capped: 498 -> 404
+  // us); where sequences are short, blocks of one head follow each other (780 of 256 x 4 heads: 263 -> 233).
+  const Tile tile = tile_of(a.rq, a.B, kRows * kTiles, tiles - 1 - (int)(heads_first ? blockIdx.x / a.H : blockIdx.x % tiles));
   if (!tile.any) return;
   const int tile_rows = min(kRows * kTiles, tile.rows.n - tile.first);      // of the output that are this block's
   Span qs{tile.rows.b, tile.rows.first, 0}, ks{0, 0, 0};
@@ -420,7 +421,9 @@ cudaError_t launch(const FwdMaps& maps, const AttnArgs& a, cudaStream_t st) {
   auto* k = attention_fwd_tc_kernel<kD, kTiles, kCap, kBias>;
   cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::smem);      // of the current device
   if (e != cudaSuccess) return e;
-  return launch_pdl(k, dim3((unsigned)tile_count(a.rq, a.B, kRows * kTiles), a.H), dim3(Shape::threads), Shape::smem, st, maps, a);
+  const long long tiles = tile_count(a.rq, a.B, kRows * kTiles), blocks = tiles * a.H;
+  if (blocks >= (1LL << 31)) return cudaErrorInvalidConfiguration;
+  return launch_pdl(k, dim3((unsigned)blocks), dim3(Shape::threads), Shape::smem, st, maps, a, (int)tiles, mean_length(a.rq, a.B) > 512);
 }
 template <int kD, int kTiles>
 cudaError_t launch(const FwdMaps& maps, const AttnArgs& a, cudaStream_t st) {
@@ -469,7 +472,10 @@ const char* launch_attention_fwd(const AttnArgs& a, cudaStream_t st) {
   if (!operand_map(a.q, a.D, a.rq, a.B, a.H, kRows, &maps.q) || !operand_map(a.k, a.D, a.rk, a.B, a.G, kRows, &maps.k) ||
       !operand_map(a.v, a.D, a.rk, a.B, a.G, kRows, &maps.v))
     return "attention: cuTensorMapEncodeTiled failed";
-  const bool two = a.rq.off ? a.rq.T > 256LL * a.B : a.rq.T > kRows;
+  // Two tiles share what is loaded; one leaves room for another block, whose set-up and end it hides.  us with two and with one:
+  // documents of 60 to 8000 (mean 1650) x 8 heads 341 and 364, 8192 tokens x 16 heads 404 and 418; 64 x 512 x 8 heads 103 and 98, 500
+  // sequences of 400 x 4 heads 340 and 320, 6 of 333 to 1999 x 6 heads, which is 288 blocks of two, 72 and 66.
+  const bool two = mean_length(a.rq, a.B) > 1024 && tile_count(a.rq, a.B, 2 * kRows) * a.H >= 2 * 148;
   cudaError_t e = a.D > 64 ? (two ? launch<128, 2>(maps, a, st) : launch<128, 1>(maps, a, st))
                            : (two ? launch<64, 2>(maps, a, st) : launch<64, 1>(maps, a, st));
   if (e == cudaSuccess) e = cudaGetLastError();

@@ -25,7 +25,8 @@ __device__ __forceinline__ Span span_of(const AttnRows& r, int seq) {
   return {0, lo, cut(r.off[seq + 1], lo, r.T) - lo};
 }
 
-// Tiles of `m` rows over all rows of an operand.  Padded: ceil(T / m) for each sequence.  Packed: the rows in front of the first
+// Tiles of `m` rows over all rows of an operand.  Padded: the first of every sequence, then the second of every sequence: the work of
+// a tile goes by its place where attention is causal, and blocks are started in the order of their work.  Packed: the rows in front of the first
 // sequence, the sequences and the rows behind the last are segments 0 to B + 1 of [0, T); segment s has its first tile at number
 // start(s) / m + s, which leaves room for ceil(n / m) tiles in each.
 struct Tile {
@@ -40,9 +41,8 @@ __host__ __device__ __forceinline__ long long tile_count(const AttnRows& r, int 
 // By a converged warp, all of whose lanes look at a segment each: three rounds of loads find one of 32768 sequences.
 __device__ __forceinline__ Tile tile_of(const AttnRows& r, int B, int m, int at) {
   if (r.off == nullptr) {
-    const int per = (r.T + m - 1) / m;
-    const int seq = at / per;
-    return {seq, {seq, 0, r.T}, (at - seq * per) * m, true};
+    const int tile = at / B, seq = at - tile * B;
+    return {seq, {seq, 0, r.T}, tile * m, true};
   }
   auto start = [&](int s) { return s == 0 ? 0 : (s > B + 1 ? r.T : cut(r.off[s - 1], 0, r.T)); };
   int lo = 0, hi = B + 1;                                  // between them lies the last segment that starts at or before tile `at`
@@ -70,6 +70,9 @@ __device__ __forceinline__ int first_query(const AttnArgs& a, int seq, int j, in
   if (!a.causal || (a.prefix != nullptr && j < a.prefix[seq])) return 0;
   return max(0, j + nq - nk);
 }
+
+// of the sequences, as far as the host knows
+__host__ __device__ __forceinline__ long long mean_length(const AttnRows& r, int B) { return r.off ? r.T / (B > 0 ? B : 1) : r.T; }
 
 __device__ __forceinline__ long long flat_rows(const AttnRows& r, int B) { return r.off ? r.T : (long long)B * r.T; }
 

@@ -438,9 +438,6 @@ const char* told(cudaError_t e) {
   return e == cudaSuccess ? nullptr : cudaGetErrorString(e);
 }
 
-// the mean length where the host knows no more
-long long length_of(const AttnRows& r, int B) { return r.off ? r.T / (B > 0 ? B : 1) : r.T; }
-
 }  // namespace
 
 // By the mean length, which is what the host knows of packed sequences.  200000 tokens, 4 heads, causal, us of these kernels and of those
@@ -451,7 +448,7 @@ long long length_of(const AttnRows& r, int B) { return r.off ? r.T / (B > 0 ? B 
 //             and 769
 bool attention_short_takes(const AttnArgs& a, bool backward) {
   const int most = backward ? (a.D <= 16 ? 400 : a.D <= 32 ? 224 : 96) : (a.D <= 16 ? 512 : a.D <= 32 ? 400 : 144);
-  return a.D <= 64 && length_of(a.rq, a.B) <= most && length_of(a.rk, a.B) <= most;
+  return a.D <= 64 && mean_length(a.rq, a.B) <= most && mean_length(a.rk, a.B) <= most;
 }
 
 const char* launch_attention_short_fwd(const AttnArgs& a, cudaStream_t st) {
