@@ -38,13 +38,16 @@ constexpr float kGrowth = 8.f;
 template <int kD, int kTiles, int kHalves>
 struct FwdShape {
   static constexpr int chunks = kD / 64;
-  static constexpr int tile_bytes = kRows * 128 * chunks;
+  static constexpr bool small = kD == 64 && kTiles == 1;      // three blocks per SM
+  static constexpr int keys = small ? 64 : 128;                // of a step
+  static constexpr int q_bytes = kRows * 128 * chunks, slot_bytes = keys * 128 * chunks;
   static constexpr int slots = kTiles == 2 ? (kD == 128 ? 4 : 6) : (kD == 128 ? 2 : 4);
   static constexpr int softmax_warps = 4 * kHalves * kTiles;
   static constexpr int threads = 32 * (softmax_warps + 2);
-  static constexpr int smem = tile_bytes * (kTiles + slots) + 1024;
-  static constexpr int tmem_cols = kTiles == 2 ? 512 : 256;
-  static constexpr int o_col = 128 * kTiles;
+  static constexpr int blocks = kTiles == 2 ? 1 : small && kHalves == 1 ? 3 : 2;      // per SM
+  static constexpr int smem = q_bytes * kTiles + slot_bytes * slots + 1024;
+  static constexpr int tmem_cols = kTiles == 2 ? 512 : small ? 128 : 256;
+  static constexpr int o_col = keys * kTiles;
 };
 
 // The two warps that have half of the same queries' keys each
@@ -67,10 +70,11 @@ struct FwdMaps {
 };
 
 template <int kD, int kTiles, bool kCap, bool kBias>
-__global__ void __launch_bounds__(FwdShape<kD, kTiles, kCap ? 2 : 1>::threads, kTiles == 2 ? 1 : 2)
+__global__ void __launch_bounds__(FwdShape<kD, kTiles, kCap ? 2 : 1>::threads, FwdShape<kD, kTiles, kCap ? 2 : 1>::blocks)
 attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_constant__ AttnArgs a, int tiles, int heads_first) {
-  constexpr int kHalves = kCap ? 2 : 1, kHalf = kRows / kHalves;      // threads per query, keys of a step per thread
+  constexpr int kHalves = kCap ? 2 : 1;      // threads per query
   using Shape = FwdShape<kD, kTiles, kHalves>;
+  constexpr int kKeys = Shape::keys, kHalf = kKeys / kHalves;      // of a step; of a thread
   constexpr int kSlots = Shape::slots;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t s_q, s_full[kSlots], s_empty[kSlots], s_score[kTiles], s_weight[kTiles], s_out[kTiles];
@@ -116,10 +120,10 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
   // what one lane's loads and products are addressed with is known to be the same for the warp
 #pragma unroll
   for (int t = 0; t < kTiles; ++t) vis[t] = one_of_warp(vis[t]);
-  const int steps = one_of_warp((most + kRows - 1) / kRows);
+  const int steps = one_of_warp((most + kKeys - 1) / kKeys);
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_gen = smem_raw + (base - smem_u32(smem_raw));
-  const uint32_t ring = base + kTiles * Shape::tile_bytes;
+  const uint32_t ring = base + kTiles * Shape::q_bytes;
 
   if (threadIdx.x == 0) {
     *s_abort = 0;
@@ -146,11 +150,11 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
     if (lead) {
       int n = 0;
       for (int t = 0; t < kTiles; ++t) n += vis[t] > 0;
-      mbar_expect_tx(smem_u32(&s_q), n * Shape::tile_bytes);
+      mbar_expect_tx(smem_u32(&s_q), n * Shape::q_bytes);
       for (int t = 0; t < kTiles; ++t)
         if (vis[t] > 0)
           for (int c = 0; c < Shape::chunks; ++c)
-            tma_load_4d(base + t * Shape::tile_bytes + c * (kRows * 128), &maps.q, 64 * c, q_first + t * kRows, h, qs.b, smem_u32(&s_q));
+            tma_load_4d(base + t * Shape::q_bytes + c * (kRows * 128), &maps.q, 64 * c, q_first + t * kRows, h, qs.b, smem_u32(&s_q));
     }
     __syncwarp();
     for (int i = 0; i < 2 * steps; ++i) {
@@ -158,9 +162,9 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
       if (i >= kSlots && !mbar_wait_warp(smem_u32(&s_empty[s]), ((i / kSlots) & 1) ^ 1, s_abort)) { *s_abort = 1; break; }
       if (lead) {
         const uint32_t bar = smem_u32(&s_full[s]);
-        mbar_expect_tx(bar, Shape::tile_bytes);
+        mbar_expect_tx(bar, Shape::slot_bytes);
         for (int c = 0; c < Shape::chunks; ++c)
-          tma_load_4d(ring + s * Shape::tile_bytes + c * (kRows * 128), (i & 1) ? &maps.v : &maps.k, 64 * c, k_first + (i >> 1) * kRows, g, k_b, bar);
+          tma_load_4d(ring + s * Shape::slot_bytes + c * (kKeys * 128), (i & 1) ? &maps.v : &maps.k, 64 * c, k_first + (i >> 1) * kKeys, g, k_b, bar);
       }
       __syncwarp();
     }
@@ -174,26 +178,26 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
       tc_fence_after();
     };
     auto scores = [&](int t, int j) {
-      const uint32_t q = base + t * Shape::tile_bytes, k = ring + (2 * j % kSlots) * Shape::tile_bytes;
-      const uint32_t id = idesc_of(round16(min(kRows, vis[t] - j * kRows)), false);
+      const uint32_t q = base + t * Shape::q_bytes, k = ring + (2 * j % kSlots) * Shape::slot_bytes;
+      const uint32_t id = idesc_of(round16(min(kKeys, vis[t] - j * kKeys)), false);
       if (lead) {
         const uint64_t qd = make_smem_desc(q, 16u, 1024u), kd = make_smem_desc(k, 16u, 1024u);
 #pragma unroll
         for (int s = 0; s < kD / 16; ++s)
-          if (s * 16 < d16) umma_f16(tm + t * 128, qd + step_k<kRows>(s), kd + step_k<kRows>(s), id, s > 0);
+          if (s * 16 < d16) umma_f16(tm + t * kKeys, qd + step_k<kRows>(s), kd + step_k<kKeys>(s), id, s > 0);
         umma_commit(smem_u32(&s_score[t]));
       }
       __syncwarp();
     };
     auto values = [&](int t, int j) {
-      const uint32_t v = ring + ((2 * j + 1) % kSlots) * Shape::tile_bytes;
-      const int n = round16(min(kRows, vis[t] - j * kRows)) / 16;
+      const uint32_t v = ring + ((2 * j + 1) % kSlots) * Shape::slot_bytes;
+      const int n = round16(min(kKeys, vis[t] - j * kKeys)) / 16;
       const uint32_t id = idesc_of(d16, true);
       if (lead) {
-        const uint64_t vd = make_smem_desc(v, kRows * 128, 1024u);
+        const uint64_t vd = make_smem_desc(v, kKeys * 128, 1024u);
 #pragma unroll
-        for (int s = 0; s < kRows / 16; ++s)
-          if (s < n) umma_f16_ts(tm + Shape::o_col + t * kD, tm + t * 128 + s * 8, vd + step_mn(s), id, j > 0 || s > 0);
+        for (int s = 0; s < kKeys / 16; ++s)
+          if (s < n) umma_f16_ts(tm + Shape::o_col + t * kD, tm + t * kKeys + s * 8, vd + step_mn(s), id, j > 0 || s > 0);
       }
       __syncwarp();
     };
@@ -210,17 +214,17 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
     for (int j = 0; j < steps && ok; ++j) {
       full(2 * j + 1);
       if (!ok) break;
-      const int end = ks.n - j * kRows;            // rows of this tile of values that the sequence has
-      if (end < kRows && (end & 15)) zero_rows<kRows>(smem_gen + (ring - base) + ((2 * j + 1) % kSlots) * Shape::tile_bytes, Shape::chunks, end, round16(end), lane);
+      const int end = ks.n - j * kKeys;            // rows of this tile of values that the sequence has
+      if (end < kKeys && (end & 15)) zero_rows<kKeys>(smem_gen + (ring - base) + ((2 * j + 1) % kSlots) * Shape::slot_bytes, Shape::chunks, end, round16(end), lane);
       bool next = false;
 #pragma unroll
       for (int t = 0; t < kTiles; ++t) {
-        if (j * kRows >= vis[t]) continue;
+        if (j * kKeys >= vis[t]) continue;
         ok = ok && mbar_wait_warp(smem_u32(&s_weight[t]), j & 1, s_abort);
         if (!ok) break;
         tc_fence_after();
         values(t, j);
-        if ((j + 1) * kRows < vis[t]) {
+        if ((j + 1) * kKeys < vis[t]) {
           if (!next) full(2 * j + 2);
           if (!ok) break;
           next = true;
@@ -240,7 +244,7 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
     const int pair = 1 + t * 4 + (warp & 3);           // the barrier of the two warps that share 32 queries
     const int i = tile.first + t * kRows + r;
     const uint32_t tm = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t tm_s = tm + t * 128 + half * kHalf, tm_p = tm + t * 128 + half * (kHalf / 2), tm_o = tm + Shape::o_col + t * kD;
+    const uint32_t tm_s = tm + t * kKeys + half * kHalf, tm_p = tm + t * kKeys + half * (kHalf / 2), tm_o = tm + Shape::o_col + t * kD;
     const int my_vis = t == 0 ? vis[0] : vis[kTiles - 1];
     const int lim = i < qs.n ? keys_seen(a, tile.seq, i, qs.n, ks.n) : my_vis;
     const int least = keys_seen(a, tile.seq, tile.first + t * kRows, qs.n, ks.n);      // of the tile's queries
@@ -252,11 +256,11 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
     float m = kNone, l = 0.f;
     const int d_half = kHalves == 2 ? round16(d16 / 2) : d16;
     bool ok = true;
-    for (int j = 0; j * kRows < my_vis; ++j) {
+    for (int j = 0; j * kKeys < my_vis; ++j) {
       ok = ok && mbar_wait_warp(smem_u32(&s_score[t]), j & 1, s_abort);
       if (!ok) *s_abort = 1;         // (the pair's barriers are passed all the same)
       tc_fence_after();
-      const int j0 = j * kRows + half * kHalf, wide = min(kHalf, my_vis - j0);              // columns of scores
+      const int j0 = j * kKeys + half * kHalf, wide = min(kHalf, my_vis - j0);              // columns of scores
       const bool masked = j0 + kHalf > least;
       float2 s[kHalf / 2];
 #pragma unroll
@@ -468,14 +472,15 @@ bool operand_map(const AttnOperand& o, int D, const AttnRows& r, int B, int head
 }  // namespace attn
 
 const char* launch_attention_fwd(const AttnArgs& a, cudaStream_t st) {
-  FwdMaps maps;
-  if (!operand_map(a.q, a.D, a.rq, a.B, a.H, kRows, &maps.q) || !operand_map(a.k, a.D, a.rk, a.B, a.G, kRows, &maps.k) ||
-      !operand_map(a.v, a.D, a.rk, a.B, a.G, kRows, &maps.v))
-    return "attention: cuTensorMapEncodeTiled failed";
   // Two tiles share what is loaded; one leaves room for another block, whose set-up and end it hides.  us with two and with one:
   // documents of 60 to 8000 (mean 1650) x 8 heads 341 and 364, 8192 tokens x 16 heads 404 and 418; 64 x 512 x 8 heads 103 and 98, 500
   // sequences of 400 x 4 heads 340 and 320, 6 of 333 to 1999 x 6 heads, which is 288 blocks of two, 72 and 66.
   const bool two = mean_length(a.rq, a.B) > 1024 && tile_count(a.rq, a.B, 2 * kRows) * a.H >= 2 * 148;
+  const int keys = two || a.D > 64 ? FwdShape<128, 1, 1>::keys : FwdShape<64, 1, 1>::keys;
+  FwdMaps maps;
+  if (!operand_map(a.q, a.D, a.rq, a.B, a.H, kRows, &maps.q) || !operand_map(a.k, a.D, a.rk, a.B, a.G, keys, &maps.k) ||
+      !operand_map(a.v, a.D, a.rk, a.B, a.G, keys, &maps.v))
+    return "attention: cuTensorMapEncodeTiled failed";
   cudaError_t e = a.D > 64 ? (two ? launch<128, 2>(maps, a, st) : launch<128, 1>(maps, a, st))
                            : (two ? launch<64, 2>(maps, a, st) : launch<64, 1>(maps, a, st));
   if (e == cudaSuccess) e = cudaGetLastError();
