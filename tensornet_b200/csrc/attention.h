@@ -36,7 +36,7 @@ struct AttnArgs {
 };
 
 const char* launch_attention_fwd(const AttnArgs& a, cudaStream_t st);
-// Few queries, padded: whether launch_attention_few takes the call, and the fp32 values of workspace that it wants then.
+// Few queries, padded: whether launch_attention_few takes the call (it is asked first), and the fp32 values of workspace that it wants then.
 bool attention_few_takes(const AttnArgs& a);
 long long attention_few_floats(const AttnArgs& a);
 const char* launch_attention_few(const AttnArgs& a, float* work, cudaStream_t st);

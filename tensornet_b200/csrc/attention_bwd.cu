@@ -86,7 +86,7 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
   constexpr int kSlots = Shape::slots, kY = Shape::y, kParts = Shape::parts;
   volatile int* s_abort = &sh.abort;
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
-  const Tile tile = tile_of(kKeys ? a.rk : a.rq, a.B, kX, tile_at);
+  const Tile tile = tile_of<true>(kKeys ? a.rk : a.rq, a.B, kX, tile_at);
   if (!tile.any) return;
   const int tile_rows = min(kX, tile.rows.n - tile.first);
   Span qs{tile.rows.b, tile.rows.first, 0}, ks = qs;

@@ -1,7 +1,7 @@
 // Attention of a few queries against many keys, forward: up to 16 rows, a query head's query each, that share a key head.
 //
 // What bounds it is reading keys and values once.  A warp takes 16 or 32 keys at a time with a softmax and a ring of its own: one
-// lane asks for tiles of keys and values by TMA, three steps ahead, so that a GPU's worth of warps has 28 MB on the way; products
+// lane asks for tiles of keys and values by TMA, two or three steps ahead, so that a GPU's worth of warps has 28 MB on the way; products
 // are mma.sync of 16 rows (at these rates far from what bounds it).  Tiles lie in rows of 128 bytes, swizzled, and are read
 // 16 bytes at a time in the layout that the instruction wants, without conflicts:
 //   * scores: the contraction may go over the columns in any order that both sides share.  A lane of group g = lane / 4, t = lane % 4
@@ -40,7 +40,7 @@ struct FewShape : Pieces<kD> {
   static constexpr int chunks = kD == 128 ? 2 : 1;                    // of 64 columns
   static constexpr int chunk_bytes = keys * 128;
   static constexpr int stage_bytes = 2 * chunks * chunk_bytes;        // keys, then values: 8 KiB
-  static constexpr int stages = 3;
+  static constexpr int stages = kD == 128 ? 3 : 2;
   static constexpr int smem = kWarps * stages * stage_bytes + 1024;
 };
 
@@ -50,7 +50,7 @@ struct FewMaps {
 
 // part: [unit][split][16][kD] sums and [unit][split][16][2] references and sums of weights, where there are several splits
 template <int kD>
-__global__ void __launch_bounds__(32 * kWarps, 2)
+__global__ void __launch_bounds__(32 * kWarps, kD == 128 ? 2 : 3)
 attention_few_kernel(const __grid_constant__ FewMaps maps, const __grid_constant__ AttnArgs a, const FewPlan plan, float* __restrict__ part,
                      float* __restrict__ part_ml) {
   using S = FewShape<kD>;
@@ -268,6 +268,7 @@ attention_few_kernel(const __grid_constant__ FewMaps maps, const __grid_constant
   constexpr int kPitch = kD + 4;
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
+    if (row0 + g + 8 * r >= rows) continue;
     float all = kNone;
     for (int w = 0; w < kWarps; ++w) all = fmaxf(all, s_m[w][g + 8 * r]);
     const float by = m[r] == kNone ? 0.f : ex2(m[r] - all);
@@ -276,8 +277,9 @@ attention_few_kernel(const __grid_constant__ FewMaps maps, const __grid_constant
 #pragma unroll
       for (int f = 0; f < 2; ++f)
 #pragma unroll
-        for (int i = 0; i < S::v_cols; ++i)
-          s_o[(warp * kRowsM + g + 8 * r) * kPitch + column(p, f) + i] = by == 0.f ? 0.f : o[p * S::v_cols + i][2 * r + f] * by;
+        for (int i = 0; i < S::v_cols; i += 2)
+          *reinterpret_cast<float2*>(s_o + (warp * kRowsM + g + 8 * r) * kPitch + column(p, f) + i) =
+              by == 0.f ? make_float2(0.f, 0.f) : make_float2(o[p * S::v_cols + i][2 * r + f] * by, o[p * S::v_cols + i + 1][2 * r + f] * by);
   }
   __syncthreads();
   for (int e = threadIdx.x; e < min(kRowsM, rows - row0) * (kD / 2); e += 32 * kWarps) {
@@ -363,7 +365,8 @@ FewPlan plan_of(const AttnArgs& a) {
   p.row_blocks = (int)(((long long)a.rq.T * (a.H / a.G) + kRowsM - 1) / kRowsM);
   const long long units = (long long)a.B * a.G * p.row_blocks;
   const int keys = a.rk.T;
-  p.per_unit = keys <= 256 && units >= 148 * 8 ? 1 : kWarps;
+  // A warp each where that fills the GPU: 512 histories of 20 to 2000 x 8 heads 126 -> 94 us, 2048 of 10 to 600 x 4 heads 119 -> 64.
+  p.per_unit = keys <= 2048 && units >= 148 * 8 ? 1 : kWarps;
   p.splits = 1;
   p.chunk = keys;
   if (p.per_unit > 1) {
@@ -398,7 +401,18 @@ cudaError_t launch(const FewMaps& maps, const AttnArgs& a, const FewPlan& p, flo
 
 }  // namespace
 
-bool attention_few_takes(const AttnArgs& a) { return a.rq.off == nullptr && (long long)a.rq.T * (a.H / a.G) <= 4 * kRowsM; }
+// Where the kernels for short sequences take the call too, they start fewer warps that do more.  600000 keys in sequences of 50, 100 and
+// 200, 4 heads, us of those and of these:
+//   1 query    16 columns 78, 68, 65 and 109, 86, 70;  32: 113, 92, 88 and 119, 100, 83;  64: 178, 160 and 135, 111
+//   50         16 columns 273, 336, 373 and 461, 324, 250;  32: 432, 440, 547 and 514, 379, 299;  64: 746, 686 and 576, 399
+// and one sequence of 200 with one query, 18 and 10.
+bool attention_few_takes(const AttnArgs& a) {
+  const long long rows = (long long)a.rq.T * (a.H / a.G), keys = mean_length(a.rk, a.B);
+  if (a.rq.off != nullptr || rows > 4 * kRowsM) return false;
+  if (!attention_short_takes(a, false)) return true;
+  if (tile_count(a.rq, a.B, 16) * a.H < 148 * 8) return keys > 32;
+  return a.D > 32 ? keys > 24 : rows > kRowsM ? keys > 80 : a.D > 16 && keys > 160;
+}
 
 long long attention_few_floats(const AttnArgs& a) {
   const FewPlan p = plan_of(a);

@@ -89,7 +89,7 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   // The last tiles of causal sequences have the most keys: they go first, those of all heads (8192 tokens x 16 heads, capped: 498 -> 404
   // us); where sequences are short, blocks of one head follow each other (780 of 256 x 4 heads: 263 -> 233).
-  const Tile tile = tile_of(a.rq, a.B, kRows * kTiles, tiles - 1 - (int)(heads_first ? blockIdx.x / a.H : blockIdx.x % tiles));
+  const Tile tile = tile_of<true>(a.rq, a.B, kRows * kTiles, tiles - 1 - (int)(heads_first ? blockIdx.x / a.H : blockIdx.x % tiles));
   if (!tile.any) return;
   const int tile_rows = min(kRows * kTiles, tile.rows.n - tile.first);      // of the output that are this block's
   Span qs{tile.rows.b, tile.rows.first, 0}, ks{0, 0, 0};

@@ -25,8 +25,9 @@ __device__ __forceinline__ Span span_of(const AttnRows& r, int seq) {
   return {0, lo, cut(r.off[seq + 1], lo, r.T) - lo};
 }
 
-// Tiles of `m` rows over all rows of an operand.  Padded: the first of every sequence, then the second of every sequence: the work of
-// a tile goes by its place where attention is causal, and blocks are started in the order of their work.  Packed: the rows in front of the first
+// Tiles of `m` rows over all rows of an operand.  Padded: ceil(T / m) for each sequence, sequence after sequence, or, kByPlace, the first
+// of every sequence, then the second: the work of a tile goes by its place where attention is causal, and blocks are started in the
+// order of their work.  Packed: the rows in front of the first
 // sequence, the sequences and the rows behind the last are segments 0 to B + 1 of [0, T); segment s has its first tile at number
 // start(s) / m + s, which leaves room for ceil(n / m) tiles in each.
 struct Tile {
@@ -39,10 +40,11 @@ __host__ __device__ __forceinline__ long long tile_count(const AttnRows& r, int 
   return r.off == nullptr ? (long long)B * ((r.T + m - 1) / m) : (long long)r.T / m + B + 2;
 }
 // By a converged warp, all of whose lanes look at a segment each: three rounds of loads find one of 32768 sequences.
+template <bool kByPlace>
 __device__ __forceinline__ Tile tile_of(const AttnRows& r, int B, int m, int at) {
   if (r.off == nullptr) {
-    const int tile = at / B, seq = at - tile * B;
-    return {seq, {seq, 0, r.T}, tile * m, true};
+    const int per = kByPlace ? B : (r.T + m - 1) / m, slow = at / per, fast = at - slow * per, seq = kByPlace ? fast : slow;
+    return {seq, {seq, 0, r.T}, (kByPlace ? slow : fast) * m, true};
   }
   auto start = [&](int s) { return s == 0 ? 0 : (s > B + 1 ? r.T : cut(r.off[s - 1], 0, r.T)); };
   int lo = 0, hi = B + 1;                                  // between them lies the last segment that starts at or before tile `at`

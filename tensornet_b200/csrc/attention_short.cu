@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(32 * kWarps, kD == 16 ? 6 : kD == 32 ? 4 : 3) 
   const unsigned tile_at = unit / groups;
   if (tile_at >= tiles) return;
   const int h0 = (unit - tile_at * groups) * heads, h1 = min(a.H, h0 + (int)heads), R = a.H / a.G;
-  const Tile tile = tile_of(a.rq, a.B, kM, (int)tile_at);
+  const Tile tile = tile_of<false>(a.rq, a.B, kM, (int)tile_at);
   if (!tile.any) return;
   Span qs{tile.rows.b, tile.rows.first, 0}, ks{0, 0, 0};
   if (tile.seq >= 0) {
@@ -251,7 +251,7 @@ template <int kD, bool kCap, bool kBias, bool kKeys>
 __device__ __forceinline__ void short_bwd(const AttnArgs& a, int tile_at, int head0, int head1) {
   using P = Pieces<kD>;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const Tile tile = tile_of(kKeys ? a.rk : a.rq, a.B, kM, tile_at);
+  const Tile tile = tile_of<false>(kKeys ? a.rk : a.rq, a.B, kM, tile_at);
   if (!tile.any) return;
   Span qs{tile.rows.b, tile.rows.first, 0}, ks = qs;
   if (tile.seq >= 0) {

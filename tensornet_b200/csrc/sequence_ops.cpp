@@ -191,15 +191,15 @@ struct Attention : torch::autograd::Function<Attention> {
         rest = at::empty_like(out);
         a.rest = view_of(rest);
       }
-      if (tn::attention_short_takes(a, false)) {
-        told(tn::launch_attention_short_fwd(a, counted_stream()));
-      } else if (tn::attention_few_takes(a)) {
+      if (tn::attention_few_takes(a)) {
         at::Tensor work;
         if (const long long n = tn::attention_few_floats(a)) {
           work = at::empty({n}, q.options().dtype(at::kFloat));
           count_launches(1);
         }
         told(tn::launch_attention_few(a, work.defined() ? work.data_ptr<float>() : nullptr, counted_stream()));
+      } else if (tn::attention_short_takes(a, false)) {
+        told(tn::launch_attention_short_fwd(a, counted_stream()));
       } else {
         told(tn::launch_attention_fwd(a, counted_stream()));
       }
