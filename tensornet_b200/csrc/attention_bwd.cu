@@ -143,6 +143,9 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // The kernel behind this one may start now, and not before: it may want tensor memory ahead of its own wait, and a block of this kernel
+  // that had none yet would then wait for a block that waits for this kernel.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t tmem = sh.tmem;
   const int d16 = round16(a.D);
   const long long q_rows = flat_rows(a.rq, a.B), q_flat = (a.rq.off ? 0 : (long long)qs.b * a.rq.T) + qs.first;
@@ -426,7 +429,6 @@ attention_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, const __grid_const
   extern __shared__ uint8_t smem_raw[];
   __shared__ BwdShared<kD> sh;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int at = blockIdx.x;
   if (at < key_tiles * a.G)
     bwd_block<kD, true, kCap, kBias>(maps, a, sh, smem_raw, at / a.G, at % a.G);

@@ -86,7 +86,6 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
   const int h = heads_first ? blockIdx.x % a.H : blockIdx.x / tiles;
 
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   // The last tiles of causal sequences have the most keys: they go first, those of all heads (8192 tokens x 16 heads, capped: 498 -> 404
   // us); where sequences are short, blocks of one head follow each other (780 of 256 x 4 heads: 263 -> 233).
   const Tile tile = tile_of<true>(a.rq, a.B, kRows * kTiles, tiles - 1 - (int)(heads_first ? blockIdx.x / a.H : blockIdx.x % tiles));
@@ -140,6 +139,9 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // The kernel behind this one may start now, and not before: it may want tensor memory ahead of its own wait, and a block of this kernel
+  // that had none yet would then wait for a block that waits for this kernel.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t tmem = s_tmem;
   const int d16 = round16(a.D);
 

@@ -666,8 +666,8 @@ def layer_norm(x: torch.Tensor, gamma: Optional[torch.Tensor] = None, beta: Opti
         if p is not None and (p.dtype != torch.float32 or p.shape != (x.shape[-1],) or p.device != x.device):
             raise ValueError(f"layer_norm: {name} must be fp32 [{x.shape[-1]}] on {x.device}, not {p.dtype} {tuple(p.shape)} on {p.device}")
     eps = float(eps)
-    if not 0.0 < eps < float("inf"):
-        raise ValueError(f"layer_norm: eps must be above zero, not {eps}")
+    if not torch.finfo(torch.float32).tiny <= eps < 1e30:
+        raise ValueError(f"layer_norm: eps must be above zero, in fp32, not {eps}")
     if x.is_cuda:
         return _ext().layer_norm(x, gamma, beta, eps, _status())
     f = x.float()
@@ -697,7 +697,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, lengths: Opt
     do not start on 16 bytes are copied first.
 
     A sequence's queries stand at the end of its keys: query ``i`` of ``nq`` is at place ``i + nk - nq`` of ``nk`` keys, so that one
-    query is the newest token.  Its score with key ``j`` is ``scale * q.k``, with ``cap`` as ``cap * tanh(scale * q.k / cap)``, less
+    query is the newest token.  Its score with key ``j`` is ``scale * q.k``, with ``cap`` (0 and None: none) as ``cap * tanh(scale * q.k / cap)``, less
     ``slopes[h] * |place - j|`` (fp32 ``[heads]``, constants).  ``causal`` hides the keys behind a query's place, but for the first
     ``prefix[b]`` (int32 ``[B]``) keys of the sequence, which all its queries see.  ``scale`` defaults to ``columns ** -0.5``.
 
@@ -744,8 +744,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, lengths: Opt
         slopes = slopes.contiguous()
     cap = 0.0 if cap is None else float(cap)
     scale = D ** -0.5 if scale is None else float(scale)
-    if not 0.0 <= cap < float("inf") or not 0.0 < scale < float("inf"):
-        raise ValueError(f"attention: scale ({scale}) must be above zero, and so must cap ({cap or None})")
+    if not cap >= 0.0 or not all(1e-30 < f < 1e30 for f in ((scale, cap, scale / cap) if cap else (scale,))):
+        raise ValueError(f"attention: scale ({scale}) must be above zero, and so must cap ({cap or None}); they and their ratio are fp32")
     if q.is_cuda:
         return _ext().attention(q, k, v, rows[0], rows[1], prefix, slopes, bool(causal), cap, scale, _status())
     return _attention_cpu(q, k, v, rows, B, bool(causal), prefix, cap, slopes, scale)

@@ -65,8 +65,12 @@ OK = dict(q=bf(2, 3, 4, 8), k=bf(2, 3, 2, 8), v=bf(2, 3, 2, 8))
     (dict(slopes=torch.ones(2)), "slopes"),
     (dict(slopes=torch.ones(4, requires_grad=True)), "no gradient"),
     (dict(cap=-1.0), "above zero"),
+    (dict(cap=-0.5), "above zero"),
     (dict(cap=float("inf")), "above zero"),
     (dict(scale=0.0), "above zero"),
+    (dict(scale=1e-40), "above zero"),
+    (dict(scale=1e20, cap=1e-20), "above zero"),
+    (dict(cap=float("nan")), "above zero"),
     (dict(scale=float("nan")), "above zero"),
 ])
 def test_refusals(kw, text):

@@ -44,6 +44,7 @@ def test_layer_has_its_configuration_and_parameters():
     (dict(x=torch.zeros(3, 4), gamma=torch.ones(1, 4)), "gamma"),
     (dict(x=torch.zeros(3, 4), beta=torch.ones(4, dtype=torch.bfloat16)), "beta"),
     (dict(x=torch.zeros(3, 4), eps=0.0), "eps"),
+    (dict(x=torch.zeros(3, 4), eps=1e-40), "eps"),
     (dict(x=torch.zeros(3, 4), eps=float("nan")), "eps"),
 ])
 def test_refusals(kw, text):
