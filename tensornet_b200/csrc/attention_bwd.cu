@@ -317,13 +317,21 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
       if (any) {
         bool near = true;
         if (kCap) {
+          // which tanh it is goes by scores that are seen, not by what else the columns hold
           float far[2] = {0.f, 0.f};
+          if (masked) {
+#pragma unroll
+            for (int i = 0; i < kPart / 2; ++i) {
+              if (kKeys ? 2 * i < meets || 2 * i >= ends : 2 * i >= ends) s[i].x = 0.f;
+              if (kKeys ? 2 * i + 1 < meets || 2 * i + 1 >= ends : 2 * i + 1 >= ends) s[i].y = 0.f;
+            }
+          }
 #pragma unroll
           for (int e = 0; e < kPart / 2; ++e) {
             s[e] = mul2(s[e], both(c));
             far[e & 1] = max3(far[e & 1], fabsf(s[e].x), fabsf(s[e].y));
           }
-          near = __all_sync(0xffffffffu, fmaxf(far[0], far[1]) <= 1.f);
+          near = __all_sync(0xffffffffu, x >= xs.n || fmaxf(far[0], far[1]) <= 1.f);
         }
         // the distance of columns from a row is linear where all lie on one side
         const float from = (float)(kKeys ? y0 + c0 + shift - x : x + shift - y0 - c0), per = kKeys ? 1.f : -1.f;

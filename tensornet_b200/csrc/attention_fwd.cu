@@ -277,13 +277,19 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
         if (c0 >= wide) continue;
         float2* x = s + c0 / 2;
         if (kCap) {
+          // which tanh it is goes by scores that are seen, not by what else the columns hold
           float far[2] = {0.f, 0.f};
+          if (masked) {
+            const int there = lim - j0 - c0;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[e] = make_float2(2 * e < there ? x[e].x : 0.f, 2 * e + 1 < there ? x[e].y : 0.f);
+          }
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             x[e] = mul2(x[e], both(c));
             far[e & 1] = max3(far[e & 1], fabsf(x[e].x), fabsf(x[e].y));
           }
-          if (__all_sync(0xffffffffu, fmaxf(far[0], far[1]) <= 1.f)) {
+          if (__all_sync(0xffffffffu, i >= qs.n || fmaxf(far[0], far[1]) <= 1.f)) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) x[e] = mul2(tanh_small(x[e]), both(cap2));
           } else {

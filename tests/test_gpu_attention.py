@@ -299,3 +299,28 @@ def test_second_derivatives_are_refused(tn_gpu, status_ok):
     q = normal(tn_gpu.core.runtime().device, 1, 5, 1, 8).requires_grad_()
     with pytest.raises(RuntimeError, match="once"):
         torch.autograd.grad(F.attention(q, q, q).float().sum(), q, create_graph=True)
+
+
+@pytest.mark.parametrize("D", [16, 64, 80])
+@pytest.mark.parametrize("cap", [None, 5.0])
+@pytest.mark.parametrize("L, causal", [(50, True), (290, True), (290, False), (1100, False)])
+def test_bits_do_not_depend_on_what_lies_behind_a_sequence(tn_gpu, status_ok, D, cap, L, causal):
+    """Nor on what another call has left on the chip: one with far larger scores runs between two that have to agree."""
+    from tensornet_b200.ops import functional as F
+
+    dev = tn_gpu.core.runtime().device
+    n = ints(dev, L, L - 13, 1, 0, L // 2 + 5)
+    q, k, v, go = [normal(dev, 5, L + 30, 4, D, seed=s) for s in range(4)]
+    big = normal(dev, 3, 700, 4, D, seed=9, by=300.0)
+    behind = torch.arange(L + 30, device=dev) >= n[:, None]
+
+    def once(fill):
+        a = [t.masked_fill(behind[:, :, None, None], fill).requires_grad_() for t in (q, k, v)]
+        out = F.attention(*a, lengths=n, kv_lengths=n, causal=causal, cap=cap, slopes=slopes_of(dev, 4))
+        return [out.detach(), *torch.autograd.grad(out, a, go.masked_fill(behind[:, :, None, None], fill))]
+
+    want = once(0.0)
+    for fill in (0.0, 1.0, 200.0, float("inf"), float("nan"), 0.0):
+        x = big.requires_grad_()
+        F.attention(x, x, x, cap=cap).sum().backward()
+        assert all(torch.equal(a, b) for a, b in zip(once(fill), want)), fill
