@@ -19,6 +19,12 @@
 // The products of a step are issued in the order  acc2(i) s(i + 1) | acc1(i) dp(i + 1):  p(i) is made while dp(i) is, ds(i) while acc2
 // and the next scores are.
 //
+// ds goes into its product as a sum of two bf16, the second in the columns that the first leaves free, where sequences are short or
+// columns few.  sum ds k loses the part of k that the weights agree on, as sum ds = 0, and a rounding of ds does not: with 8 columns
+// dq was off by 0.0030 of its norm so, with 128 columns of sequences of 2 by 0.0029, now by 0.0017.  Sequences of up to 128 take 3 % more
+// time, up to 24 columns 10 to 17 % (8 of 4000 x 4 heads, us: 297 and 338); with more columns and keys 0.0025 is left as it is
+// (128 columns: 479 and 530).
+//
 // What bounds it above 64 columns: a step of 128 x 128 takes 3300 cycles where keys are owned, of which its four products take 2300 and
 // p and ds 2400, partly beside them; and 2800 where queries are.  A product of 128 x 64 x 16 takes 62 cycles, one of 128 x 128 x 16
 // 72, so that steps of 64 rows with two buffers of s and dp were bound by their products.  8192 tokens x 16 heads x 128 columns
@@ -81,7 +87,7 @@ __device__ __forceinline__ void store_acc(uint32_t tm, int from, int to, int D, 
 
 // kKeys: the block owns keys
 template <int kD, bool kKeys, bool kCap, bool kBias>
-__device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a, BwdShared<kD>& sh, uint8_t* smem_raw, int tile_at, int head) {
+__device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a, BwdShared<kD>& sh, uint8_t* smem_raw, int tile_at, int head, bool split) {
   using Shape = BwdShape<kD>;
   constexpr int kSlots = Shape::slots, kY = Shape::y, kParts = Shape::parts;
   volatile int* s_abort = &sh.abort;
@@ -235,14 +241,14 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
       __syncwarp();
     };
     // acc += left Y(o): left operands lie where s (for p) or dp (for ds) of each thread's columns began
-    auto inner = [&](int o, int it, int y0, uint32_t left, uint32_t acc) {
+    auto inner = [&](int o, int it, int y0, uint32_t left, uint32_t acc, bool first) {
       const int n = round16(min(kY, hi - y0)) / 16;
       const uint32_t id = idesc_of(d16, true);
       if (lead) {
         const uint64_t yd = make_smem_desc(ring + (o * kSlots + it % kSlots) * Shape::y_bytes, kY * 128, 1024u);
 #pragma unroll
         for (int k = 0; k < kY / 16; ++k)
-          if (k < n) umma_f16_ts(tm + acc, tm + left + (k / 2) * kPart + (k & 1) * 8, yd + step_mn(k), id, it > 0 || k > 0);
+          if (k < n) umma_f16_ts(tm + acc, tm + left + (k / 2) * kPart + (k & 1) * 8, yd + step_mn(k), id, !first || k > 0);
       }
       __syncwarp();
     };
@@ -259,12 +265,13 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
       const int next = kKeys && y0 + kY >= hi ? lo : y0 + kY;
       if (!wait(kKeys ? sh.weight : sh.read, it & 1)) break;
       if (kKeys) {
-        inner(1, it, y0, 0, Shape::acc_col + kD);
+        inner(1, it, y0, 0, Shape::acc_col + kD, it == 0);
         free_slot(1, it);
       }
       if (more) outer(0, it + 1, next, sh.score);
       if (!wait(sh.ds[it & 1], (it >> 1) & 1)) break;
-      inner(0, it, y0, Shape::dp_col, Shape::acc_col);
+      inner(0, it, y0, Shape::dp_col, Shape::acc_col, it == 0);
+      if (split) inner(0, it, y0, Shape::dp_col + kPart / 2, Shape::acc_col, false);
       free_slot(0, it);
       if (more) {
         outer(1, it + 1, next, sh.dp);
@@ -389,8 +396,15 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
             if (kKeys ? 2 * i + 1 < meets || 2 * i + 1 >= ends : 2 * i + 1 >= ends) ds.y = 0.f;
           }
           w[i] = pack_bf16(ds.x, ds.y);
+          s[i] = ds;
         }
         tmem_st16(tm + Shape::dp_col, w);
+        if (split) {
+#pragma unroll
+          for (int i = 0; i < kPart / 2; ++i)
+            w[i] = pack_bf16(s[i].x - __uint_as_float(w[i] << 16), s[i].y - __uint_as_float(w[i] & 0xffff0000u));
+          tmem_st16(tm + Shape::dp_col + kPart / 2, w);
+        }
         tmem_st_wait();
       }
       tc_fence_before();
@@ -433,15 +447,16 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
 // keys: those go first.
 template <int kD, bool kCap, bool kBias>
 __global__ void __launch_bounds__(BwdShape<kD>::threads, kD == 128 ? 1 : 2)
-attention_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, const __grid_constant__ AttnArgs a, int key_tiles, int query_tiles) {
+attention_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, const __grid_constant__ AttnArgs a, int key_tiles, int query_tiles, int split_) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ BwdShared<kD> sh;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int at = blockIdx.x;
+  const bool split = split_ != 0;
   if (at < key_tiles * a.G)
-    bwd_block<kD, true, kCap, kBias>(maps, a, sh, smem_raw, at / a.G, at % a.G);
+    bwd_block<kD, true, kCap, kBias>(maps, a, sh, smem_raw, at / a.G, at % a.G, split);
   else
-    bwd_block<kD, false, kCap, kBias>(maps, a, sh, smem_raw, query_tiles - 1 - (at - key_tiles * a.G) / a.H, (at - key_tiles * a.G) % a.H);
+    bwd_block<kD, false, kCap, kBias>(maps, a, sh, smem_raw, query_tiles - 1 - (at - key_tiles * a.G) / a.H, (at - key_tiles * a.G) % a.H, split);
 }
 
 // delta[h][row] = sum over the columns of do (o + rest); `lanes` threads, a power of two, per row of a head
@@ -472,9 +487,10 @@ cudaError_t launch(const BwdMaps& maps, const AttnArgs& a, cudaStream_t st) {
   auto* k = attention_bwd_tc_kernel<kD, kCap, kBias>;
   cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, BwdShape<kD>::smem);      // of the current device
   if (e != cudaSuccess) return e;
+  const int split = a.D < 32 || (mean_length(a.rq, a.B) <= 128 && mean_length(a.rk, a.B) <= 128);
   const long long kt = tile_count(a.rk, a.B, kX), qt = tile_count(a.rq, a.B, kX);
   if (kt * a.G + qt * a.H >= (1LL << 31)) return cudaErrorInvalidConfiguration;
-  return launch_pdl(k, dim3((unsigned)(kt * a.G + qt * a.H)), dim3(BwdShape<kD>::threads), BwdShape<kD>::smem, st, maps, a, (int)kt, (int)qt);
+  return launch_pdl(k, dim3((unsigned)(kt * a.G + qt * a.H)), dim3(BwdShape<kD>::threads), BwdShape<kD>::smem, st, maps, a, (int)kt, (int)qt, split);
 }
 template <int kD>
 cudaError_t launch(const BwdMaps& maps, const AttnArgs& a, cudaStream_t st) {
