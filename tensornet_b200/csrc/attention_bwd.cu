@@ -85,9 +85,9 @@ __device__ __forceinline__ void store_acc(uint32_t tm, int from, int to, int D, 
   }
 }
 
-// kKeys: the block owns keys
-template <int kD, bool kKeys, bool kCap, bool kBias>
-__device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a, BwdShared<kD>& sh, uint8_t* smem_raw, int tile_at, int head, bool split) {
+// kKeys: the block owns keys; kSplit: ds in two terms
+template <int kD, bool kKeys, bool kCap, bool kBias, bool kSplit>
+__device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a, BwdShared<kD>& sh, uint8_t* smem_raw, int tile_at, int head) {
   using Shape = BwdShape<kD>;
   constexpr int kSlots = Shape::slots, kY = Shape::y, kParts = Shape::parts;
   volatile int* s_abort = &sh.abort;
@@ -271,7 +271,7 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
       if (more) outer(0, it + 1, next, sh.score);
       if (!wait(sh.ds[it & 1], (it >> 1) & 1)) break;
       inner(0, it, y0, Shape::dp_col, Shape::acc_col, it == 0);
-      if (split) inner(0, it, y0, Shape::dp_col + kPart / 2, Shape::acc_col, false);
+      if (kSplit) inner(0, it, y0, Shape::dp_col + kPart / 2, Shape::acc_col, false);
       free_slot(0, it);
       if (more) {
         outer(1, it + 1, next, sh.dp);
@@ -396,10 +396,10 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
             if (kKeys ? 2 * i + 1 < meets || 2 * i + 1 >= ends : 2 * i + 1 >= ends) ds.y = 0.f;
           }
           w[i] = pack_bf16(ds.x, ds.y);
-          s[i] = ds;
+          if (kSplit) s[i] = ds;
         }
         tmem_st16(tm + Shape::dp_col, w);
-        if (split) {
+        if (kSplit) {
 #pragma unroll
           for (int i = 0; i < kPart / 2; ++i)
             w[i] = pack_bf16(s[i].x - __uint_as_float(w[i] << 16), s[i].y - __uint_as_float(w[i] & 0xffff0000u));
@@ -445,18 +445,17 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
 
 // The first key_tiles * G blocks own keys, the others queries.  Early keys are seen by the most queries and late queries see the most
 // keys: those go first.
-template <int kD, bool kCap, bool kBias>
+template <int kD, bool kCap, bool kBias, bool kSplit>
 __global__ void __launch_bounds__(BwdShape<kD>::threads, kD == 128 ? 1 : 2)
-attention_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, const __grid_constant__ AttnArgs a, int key_tiles, int query_tiles, int split_) {
+attention_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, const __grid_constant__ AttnArgs a, int key_tiles, int query_tiles) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ BwdShared<kD> sh;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int at = blockIdx.x;
-  const bool split = split_ != 0;
   if (at < key_tiles * a.G)
-    bwd_block<kD, true, kCap, kBias>(maps, a, sh, smem_raw, at / a.G, at % a.G, split);
+    bwd_block<kD, true, kCap, kBias, kSplit>(maps, a, sh, smem_raw, at / a.G, at % a.G);
   else
-    bwd_block<kD, false, kCap, kBias>(maps, a, sh, smem_raw, query_tiles - 1 - (at - key_tiles * a.G) / a.H, (at - key_tiles * a.G) % a.H, split);
+    bwd_block<kD, false, kCap, kBias, kSplit>(maps, a, sh, smem_raw, query_tiles - 1 - (at - key_tiles * a.G) / a.H, (at - key_tiles * a.G) % a.H);
 }
 
 // delta[h][row] = sum over the columns of do (o + rest); `lanes` threads, a power of two, per row of a head
@@ -482,20 +481,19 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(const AttnArgs a, 
   if (row < rows && lane == 0) a.delta[h * rows + row] = v;
 }
 
-template <int kD, bool kCap, bool kBias>
+template <int kD, bool kCap, bool kBias, bool kSplit>
 cudaError_t launch(const BwdMaps& maps, const AttnArgs& a, cudaStream_t st) {
-  auto* k = attention_bwd_tc_kernel<kD, kCap, kBias>;
+  auto* k = attention_bwd_tc_kernel<kD, kCap, kBias, kSplit>;
   cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, BwdShape<kD>::smem);      // of the current device
   if (e != cudaSuccess) return e;
-  const int split = a.D < 32 || (mean_length(a.rq, a.B) <= 128 && mean_length(a.rk, a.B) <= 128);
   const long long kt = tile_count(a.rk, a.B, kX), qt = tile_count(a.rq, a.B, kX);
   if (kt * a.G + qt * a.H >= (1LL << 31)) return cudaErrorInvalidConfiguration;
-  return launch_pdl(k, dim3((unsigned)(kt * a.G + qt * a.H)), dim3(BwdShape<kD>::threads), BwdShape<kD>::smem, st, maps, a, (int)kt, (int)qt, split);
+  return launch_pdl(k, dim3((unsigned)(kt * a.G + qt * a.H)), dim3(BwdShape<kD>::threads), BwdShape<kD>::smem, st, maps, a, (int)kt, (int)qt);
 }
-template <int kD>
+template <int kD, bool kSplit>
 cudaError_t launch(const BwdMaps& maps, const AttnArgs& a, cudaStream_t st) {
-  if (a.cap > 0.f) return a.slopes ? launch<kD, true, true>(maps, a, st) : launch<kD, true, false>(maps, a, st);
-  return a.slopes ? launch<kD, false, true>(maps, a, st) : launch<kD, false, false>(maps, a, st);
+  if (a.cap > 0.f) return a.slopes ? launch<kD, true, true, kSplit>(maps, a, st) : launch<kD, true, false, kSplit>(maps, a, st);
+  return a.slopes ? launch<kD, false, true, kSplit>(maps, a, st) : launch<kD, false, false, kSplit>(maps, a, st);
 }
 
 }  // namespace
@@ -511,7 +509,10 @@ const char* launch_attention_bwd(const AttnArgs& a, cudaStream_t st) {
   if (!operand_map(a.q, a.D, a.rq, a.B, a.H, box, &maps.q) || !operand_map(a.k, a.D, a.rk, a.B, a.G, box, &maps.k) ||
       !operand_map(a.v, a.D, a.rk, a.B, a.G, box, &maps.v) || !operand_map(a.go, a.D, a.rq, a.B, a.H, box, &maps.go))
     return "attention: cuTensorMapEncodeTiled failed";
-  if (e == cudaSuccess) e = a.D > 64 ? launch<128>(maps, a, st) : launch<64>(maps, a, st);
+  const bool split = a.D < 32 || (mean_length(a.rq, a.B) <= 128 && mean_length(a.rk, a.B) <= 128);
+  if (e == cudaSuccess)
+    e = a.D > 64 ? (split ? launch<128, true>(maps, a, st) : launch<128, false>(maps, a, st))
+                 : (split ? launch<64, true>(maps, a, st) : launch<64, false>(maps, a, st));
   if (e == cudaSuccess) e = cudaGetLastError();
   return e == cudaSuccess ? nullptr : cudaGetErrorString(e);
 }
