@@ -27,9 +27,8 @@ __device__ __forceinline__ Span span_of(const AttnRows& r, int seq) {
 
 // Tiles of `m` rows over all rows of an operand.  Padded: ceil(T / m) for each sequence, sequence after sequence, or, kByPlace, the first
 // of every sequence, then the second: the work of a tile goes by its place where attention is causal, and blocks are started in the
-// order of their work.  Packed: the rows in front of the first
-// sequence, the sequences and the rows behind the last are segments 0 to B + 1 of [0, T); segment s has its first tile at number
-// start(s) / m + s, which leaves room for ceil(n / m) tiles in each.
+// order of their work.  Packed: the rows in front of the first sequence, the sequences and the rows behind the last are segments 0 to
+// B + 1 of [0, T); segment s has its first tile at number start(s) / m + s, which leaves room for ceil(n / m) tiles in each.
 struct Tile {
   int seq;          // -1: rows that belong to no sequence
   Span rows;        // of the segment; padded: all T rows of the sequence

@@ -3,7 +3,8 @@
 // A tile of 128 rows is mostly empty where sequences have 40, and a block that fills tiles, barriers and tensor memory for each is
 // bound by the time that takes.  Here a warp needs none of them: its rows are the left operand of mma.sync, the others' rows come
 // straight from memory (from L1 and L2 after the first reader) as right operands, and what bounds it is the number of
-// instructions.  The mathematics is that of the kernels for long sequences (attention_fwd.cu, attention_bwd.cu): every result has one
+// instructions (0.6 of the issue slots forward, 0.5 backward) and the latency of those loads.  4096 causal sequences of 1 to 200, 4
+// heads x 16 columns, with a bias: 104 us forward, 250 us backward.  The mathematics is that of the kernels for long sequences (attention_fwd.cu, attention_bwd.cu): every result has one
 // owner, so sums have a fixed order.
 #include <cuda_bf16.h>
 #include "attention_mma.cuh"
