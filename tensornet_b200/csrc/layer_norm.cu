@@ -723,11 +723,22 @@ int slot_bytes(int C) { return (C + 2 * (Piece<T>::n - 1)) / Piece<T>::n * 16; }
 // As many blocks as fit on the GPU at a time, a multiple of eight: rows of a group then start at one place in a 16-byte piece.
 template <typename K>
 int resident_grid(K kernel, int block, size_t smem, long long blocks) {
-  int dev = 0, sms = 148, per_sm = 1;
+  struct Fit { const void* kernel; int dev, block, all; size_t smem; };      // what the driver has said before
+  thread_local Fit known[16] = {};
+  thread_local int next = 0;
+  int dev = 0, all = 0;
   cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, block, smem) != cudaSuccess || per_sm < 1) per_sm = 1;
-  long long g = (long long)sms * per_sm / 8 * 8;
+  for (const Fit& f : known)
+    if (f.kernel == (const void*)kernel && f.dev == dev && f.block == block && f.smem == smem) all = f.all;
+  if (all == 0) {
+    int sms = 148, per_sm = 1;
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, block, smem) != cudaSuccess || per_sm < 1) per_sm = 1;
+    all = sms * per_sm;
+    known[next] = {(const void*)kernel, dev, block, all, smem};
+    next = (next + 1) % 16;
+  }
+  long long g = all / 8 * 8;
   if (blocks < g) g = (blocks + 7) / 8 * 8;
   return (int)(g < 8 ? 8 : g);
 }
