@@ -21,6 +21,9 @@ void told(const char* err) {
   if (err != nullptr) throw std::runtime_error(err);
 }
 bool wanted(const OptTensor& t) { return t.has_value() && t->defined() && t->requires_grad(); }
+// A tensor with a tangent (forward-mode differentiation), which the functions below refuse; without one, and where no graph is
+// built, their kernels are called straight away.
+bool dual(const at::Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
 const OptTensor some(const at::Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 void once_differentiable(const char* what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), what, " is differentiable once: its backward pass builds no graph");
@@ -113,6 +116,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 
 at::Tensor layer_norm(const at::Tensor& x, const OptTensor& gamma, const OptTensor& beta, double eps, const at::Tensor& status) {
   const bool keep = at::GradMode::is_enabled() && (x.requires_grad() || wanted(gamma) || wanted(beta));
+  if (!keep && !dual(x) && !(gamma && dual(*gamma)) && !(beta && dual(*beta))) return LayerNorm::forward(nullptr, x, gamma, beta, eps, status, false);
   return LayerNorm::apply(x, gamma, beta, eps, status, keep);
 }
 
@@ -245,6 +249,8 @@ struct Attention : torch::autograd::Function<Attention> {
 at::Tensor attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const OptTensor& q_rows, const OptTensor& k_rows,
                      const OptTensor& prefix, const OptTensor& slopes, bool causal, double cap, double scale, const at::Tensor& status) {
   const bool keep = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad());
+  if (!keep && !dual(q) && !dual(k) && !dual(v))
+    return Attention::forward(nullptr, q, k, v, q_rows, k_rows, prefix, slopes, causal, cap, scale, status, false);
   return Attention::apply(q, k, v, q_rows, k_rows, prefix, slopes, causal, cap, scale, status, keep);
 }
 

@@ -654,19 +654,24 @@ def embed_input(anchor, link, ids, offsets, B, S, D, combiner, labels=None, labe
 # =========================================================================================
 # layer normalisation
 # =========================================================================================
+_NORM_TYPES = (torch.float32, torch.bfloat16, torch.float16)
+_FP32_TINY = torch.finfo(torch.float32).tiny
+
+
 def layer_norm(x: torch.Tensor, gamma: Optional[torch.Tensor] = None, beta: Optional[torch.Tensor] = None, eps: float = 1e-5) -> torch.Tensor:
     """``(x - mean) / sqrt(var + eps) * gamma + beta`` with the moments of each row, the last dimension of ``x`` (fp32, bf16 or
     fp16); the result has ``x``'s shape and type.  ``gamma`` and ``beta``: fp32 ``[columns]``, either may be left out.  Moments
     and sums are fp32, and the gradients of ``gamma`` and ``beta`` are summed in a fixed order.  Differentiable once."""
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"layer_norm: rows of one column or more, not {tuple(x.shape)}")
-    if x.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+    if x.dtype not in _NORM_TYPES:
         raise ValueError(f"layer_norm: fp32, bf16 or fp16, not {x.dtype}")
+    columns, dev = x.shape[-1:], x.device
     for name, p in (("gamma", gamma), ("beta", beta)):
-        if p is not None and (p.dtype != torch.float32 or p.shape != (x.shape[-1],) or p.device != x.device):
-            raise ValueError(f"layer_norm: {name} must be fp32 [{x.shape[-1]}] on {x.device}, not {p.dtype} {tuple(p.shape)} on {p.device}")
+        if p is not None and (p.dtype != torch.float32 or p.shape != columns or p.device != dev):
+            raise ValueError(f"layer_norm: {name} must be fp32 [{columns[0]}] on {dev}, not {p.dtype} {tuple(p.shape)} on {p.device}")
     eps = float(eps)
-    if not torch.finfo(torch.float32).tiny <= eps < 1e30:
+    if not _FP32_TINY <= eps < 1e30:
         raise ValueError(f"layer_norm: eps must be above zero, in fp32, not {eps}")
     if x.is_cuda:
         return _ext().layer_norm(x, gamma, beta, eps, _status())
@@ -703,32 +708,26 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, lengths: Opt
 
     A query that sees no key has a zero result, and so have rows that belong to no sequence; their gradients are zero, and what
     such rows hold is not looked at.  What a sequence holds has to be finite.  Differentiable once, in a fixed order of sums."""
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        if t.dtype != torch.bfloat16 or t.dim() not in (3, 4) or t.device != q.device:
-            raise ValueError(f"attention: {name} must be bf16 [N, heads, columns] or [B, T, heads, columns] on {q.device}, "
-                             f"not {t.dtype} {tuple(t.shape)} on {t.device}")
-    H, D = q.shape[-2:]
-    G = k.shape[-2]
-    if k.shape != v.shape or k.shape[-1] != D:
-        raise ValueError(f"attention: keys {tuple(k.shape)} and values {tuple(v.shape)} must be alike, with the queries' {D} columns")
+    dev, bf16 = q.device, torch.bfloat16
+    qs, ks = q.shape, k.shape
+    nq, nk = len(qs), len(ks)
+    if q.dtype != bf16 or k.dtype != bf16 or v.dtype != bf16 or not 3 <= nq <= 4 or not 3 <= nk <= 4 or k.device != dev or v.device != dev:
+        for name, t in (("q", q), ("k", k), ("v", v)):
+            if t.dtype != bf16 or t.dim() not in (3, 4) or t.device != dev:
+                raise ValueError(f"attention: {name} must be bf16 [N, heads, columns] or [B, T, heads, columns] on {dev}, "
+                                 f"not {t.dtype} {tuple(t.shape)} on {t.device}")
+    H, D, G = qs[-2], qs[-1], ks[-2]
+    if ks != v.shape or ks[-1] != D:
+        raise ValueError(f"attention: keys {tuple(ks)} and values {tuple(v.shape)} must be alike, with the queries' {D} columns")
     if D % 8 or not 8 <= D <= 128:
         raise ValueError(f"attention: 8 to 128 columns, a multiple of 8, not {D}")
     if H < 1 or G < 1 or H % G:
         raise ValueError(f"attention: {H} query heads are no multiple of {G} key heads")
-    rows = []
-    for t, off, ln, what in ((q, offsets, lengths, ""), (k, kv_offsets, kv_lengths, "kv_")):
-        packed = t.dim() == 3
-        if packed and (off is None or ln is not None):
-            raise ValueError(f"attention: packed operands go with {what}offsets, not with {what}lengths")
-        if not packed and off is not None:
-            raise ValueError(f"attention: padded operands go with {what}lengths, not with {what}offsets")
-        r = off if packed else ln
-        if r is not None and (r.dtype != torch.int32 or r.dim() != 1 or r.device != q.device or (packed and r.numel() < 1)):
-            raise ValueError(f"attention: {what}{'offsets' if packed else 'lengths'} must be int32 [{'B + 1' if packed else 'B'}] on {q.device}")
-        rows.append(None if r is None else r.contiguous())
-    B = offsets.numel() - 1 if q.dim() == 3 else q.shape[0]
-    if B != (kv_offsets.numel() - 1 if k.dim() == 3 else k.shape[0]) or any(
-            t.dim() == 4 and r is not None and r.numel() != B for t, r in zip((q, k), rows)):
+    q_rows = _sequence_rows("", nq == 3, offsets, lengths, dev)
+    k_rows = _sequence_rows("kv_", nk == 3, kv_offsets, kv_lengths, dev)
+    B = q_rows.shape[0] - 1 if nq == 3 else qs[0]
+    if (B != (k_rows.shape[0] - 1 if nk == 3 else ks[0]) or (nq == 4 and q_rows is not None and q_rows.shape[0] != B)
+            or (nk == 4 and k_rows is not None and k_rows.shape[0] != B)):
         raise ValueError("attention: queries, keys and their lengths or offsets have different numbers of sequences")
     if prefix is not None:
         if not causal:
@@ -744,11 +743,25 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, lengths: Opt
         slopes = slopes.contiguous()
     cap = 0.0 if cap is None else float(cap)
     scale = D ** -0.5 if scale is None else float(scale)
-    if not cap >= 0.0 or not all(1e-30 < f < 1e30 for f in ((scale, cap, scale / cap) if cap else (scale,))):
+    if not cap >= 0.0 or not 1e-30 < scale < 1e30 or (cap and not (1e-30 < cap < 1e30 and 1e-30 < scale / cap < 1e30)):
         raise ValueError(f"attention: scale ({scale}) must be above zero, and so must cap ({cap or None}); they and their ratio are fp32")
     if q.is_cuda:
-        return _ext().attention(q, k, v, rows[0], rows[1], prefix, slopes, bool(causal), cap, scale, _status())
-    return _attention_cpu(q, k, v, rows, B, bool(causal), prefix, cap, slopes, scale)
+        return _ext().attention(q, k, v, q_rows, k_rows, prefix, slopes, bool(causal), cap, scale, _status())
+    return _attention_cpu(q, k, v, (q_rows, k_rows), B, bool(causal), prefix, cap, slopes, scale)
+
+
+def _sequence_rows(what, packed, offsets, lengths, dev):
+    """Where an operand's sequences are: the offsets of a packed one, the lengths of a padded one (None: all there)."""
+    if packed and (offsets is None or lengths is not None):
+        raise ValueError(f"attention: packed operands go with {what}offsets, not with {what}lengths")
+    if not packed and offsets is not None:
+        raise ValueError(f"attention: padded operands go with {what}lengths, not with {what}offsets")
+    r = offsets if packed else lengths
+    if r is None:
+        return None
+    if r.dtype != torch.int32 or r.dim() != 1 or r.device != dev or (packed and not r.shape[0]):
+        raise ValueError(f"attention: {what}{'offsets' if packed else 'lengths'} must be int32 [{'B + 1' if packed else 'B'}] on {dev}")
+    return r if r.is_contiguous() else r.contiguous()
 
 
 def _attention_cpu(q, k, v, rows, B, causal, prefix, cap, slopes, scale):

@@ -324,3 +324,18 @@ def test_bits_do_not_depend_on_what_lies_behind_a_sequence(tn_gpu, status_ok, D,
         x = big.requires_grad_()
         F.attention(x, x, x, cap=cap).sum().backward()
         assert all(torch.equal(a, b) for a, b in zip(once(fill), want)), fill
+
+
+def test_forward_mode_derivatives_are_refused(tn_gpu, status_ok):
+    import torch.autograd.forward_ad as fwd
+
+    from tensornet_b200.ops import functional as F
+
+    dev = tn_gpu.core.runtime().device
+    q, rows = normal(dev, 1, 20, 2, 16), normal(dev, 5, 16)
+    with fwd.dual_level():
+        for call in (lambda: F.attention(fwd.make_dual(q, q), q, q), lambda: F.layer_norm(fwd.make_dual(rows, rows))):
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                call()
+            with torch.no_grad(), pytest.raises((RuntimeError, NotImplementedError)):
+                call()
