@@ -11,8 +11,8 @@
 //     columns 8 spread(g) + i.
 // spread() puts neighbouring groups four rows (or four pieces) apart, where the swizzle has the other half of the banks.
 // Rows of 16 or 32 columns take pieces of 4 or 8 bytes of values in the same way.
-// Measured: 512 histories of 20 to 2000 x 8 heads x 64 columns 93 us (4.9 TB/s), 4 of 131072 x 2 key heads x 128 113 us (4.8 TB/s with
-// the kernel that joins the splits).
+// Measured: 512 histories of 20 to 2000 x 8 heads x 64 columns 94 us (4.8 TB/s), 2048 of 500 6.8 TB/s, 4 of 131072 x 2 key heads x 128
+// 95 us with the kernel that joins the splits (5.6 TB/s; a sum over as many bytes takes 100 us).
 // A sequence's keys are split over warps, blocks or both; what the blocks have of a row is brought to one reference and added by a
 // second kernel, in a fixed order.
 #include <cuda_bf16.h>
@@ -309,55 +309,85 @@ attention_few_kernel(const __grid_constant__ FewMaps maps, const __grid_constant
   }
 }
 
-// Adds a row's splits where the first had not all of it: a block per row, the threads of a column pair take splits in turn and their
-// sums are added in order.
-constexpr int kJoin = 256;
+// Adds a row's splits where the first had not all of it: a block per row, a thread per four columns and turn, up to 16 of them, which
+// take splits in turn.  What it costs is waiting for memory, so that a thread has eight loads on the way before it knows their weights;
+// the turns' sums are added in order.  74 splits of 8 rows x 8 pairs of a sequence and a key head, cold: 5.6 us (two columns per thread,
+// one load after another, 20 us).
+constexpr int kMaxTurns = 16, kAhead = 8, kMaxSplits = 1024;
 template <int kD>
-__global__ void __launch_bounds__(kJoin) attention_few_join_kernel(const __grid_constant__ AttnArgs a, const FewPlan plan,
-                                                                   const float* __restrict__ part, const float* __restrict__ part_ml) {
+__global__ void __launch_bounds__(kMaxTurns * kD / 4) attention_few_join_kernel(const __grid_constant__ AttnArgs a, const FewPlan plan,
+                                                                             const float* __restrict__ part, const float* __restrict__ part_ml) {
   pdl_sync();
-  constexpr int kPairs = kD / 2, kTurns = kJoin / kPairs;
-  __shared__ float s_x[kTurns][kPairs], s_y[kTurns][kPairs], s_sum[kTurns];
+  constexpr int kQuads = kD / 4;
+  const int threads = blockDim.x, turns = threads / kQuads;
+  __shared__ float4 s_sum[kMaxTurns][kQuads];
+  __shared__ float2 s_ml[kMaxSplits];                  // of a split: its largest score, then its weight; its sum of weights
+  __shared__ float s_max[kMaxTurns * kQuads / 32], s_l[kMaxTurns];
   const int R = a.H / a.G, rows = a.rq.T * R;
-  const int r = blockIdx.y, row0 = (int)(blockIdx.x % plan.row_blocks) * kRowsM, row = row0 + r;
-  const long long unit = blockIdx.x;
+  const unsigned unit = blockIdx.x, rest_of_unit = unit / plan.row_blocks;
+  const int r = blockIdx.y, row0 = (int)(unit - rest_of_unit * plan.row_blocks) * kRowsM, row = row0 + r;
   if (row >= rows) return;
-  const int kh = (int)(unit / plan.row_blocks % a.G), seq = (int)(unit / plan.row_blocks / a.G);
+  const int seq = (int)(rest_of_unit / a.G), kh = (int)(rest_of_unit - (unsigned)seq * a.G);
   const Span qs = span_of(a.rq, seq), ks = span_of(a.rk, seq);
   const int last = min((min(rows, row0 + kRowsM) - 1) / R, qs.n - 1);
   const int vis = row0 / R <= last ? keys_seen(a, seq, last, qs.n, ks.n) : 0;
   if (vis <= plan.chunk) return;
   const int n = (vis + plan.chunk - 1) / plan.chunk;
-  const int pair = threadIdx.x % kPairs, turn = threadIdx.x / kPairs;
-  const long long first = unit * plan.splits * kRowsM + r;
-  float all = kNone, sum = 0.f, x = 0.f, y = 0.f;
-  for (int s = 0; s < n; ++s) all = fmaxf(all, part_ml[2 * (first + (long long)s * kRowsM)]);
-  for (int s = turn; s < n; s += kTurns) {
-    const long long at_part = first + (long long)s * kRowsM;
-    const float2 ml = *reinterpret_cast<const float2*>(part_ml + 2 * at_part);
-    const float by = ml.x == kNone ? 0.f : ex2(ml.x - all);
-    const float2 v = pair * 2 < a.D ? *reinterpret_cast<const float2*>(part + at_part * kD + pair * 2) : make_float2(0.f, 0.f);
-    sum += ml.y * by;
-    x += v.x * by;
-    y += v.y * by;
+  const int quad = threadIdx.x % kQuads, turn = threadIdx.x / kQuads;
+  const long long first = (long long)unit * plan.splits * kRowsM + r;
+  const bool there = quad * 4 < a.D;
+  float4 v[kAhead];
+  auto fetch = [&](int s0) {
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int s = s0 + k * turns;
+      v[k] = there && s < n ? *reinterpret_cast<const float4*>(part + (first + (long long)s * kRowsM) * kD + quad * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  };
+  fetch(turn);
+  float all = kNone, sum = 0.f;
+  for (int s = threadIdx.x; s < n; s += threads) {
+    s_ml[s] = *reinterpret_cast<const float2*>(part_ml + 2 * (first + (long long)s * kRowsM));
+    all = fmaxf(all, s_ml[s].x);
   }
-  s_x[turn][pair] = x;
-  s_y[turn][pair] = y;
-  if (pair == 0) s_sum[turn] = sum;
+  for (int o = 16; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, o));
+  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = all;
   __syncthreads();
-  if (turn != 0 || pair * 2 >= a.D) return;
-  for (int k = 1; k < kTurns; ++k) {
-    x += s_x[k][pair];
-    y += s_y[k][pair];
+  for (int w = 0; w < threads / 32; ++w) all = fmaxf(all, s_max[w]);
+  for (int s = threadIdx.x; s < n; s += threads) s_ml[s].x = s_ml[s].x == kNone ? 0.f : ex2(s_ml[s].x - all);
+  __syncthreads();
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s0 = turn; s0 < n; s0 += kAhead * turns) {
+    if (s0 != turn) fetch(s0);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int s = s0 + k * turns;
+      if (s >= n) break;
+      const float2 by = s_ml[s];
+      sum = fmaf(by.y, by.x, sum);
+      x = make_float4(fmaf(v[k].x, by.x, x.x), fmaf(v[k].y, by.x, x.y), fmaf(v[k].z, by.x, x.z), fmaf(v[k].w, by.x, x.w));
+    }
   }
+  s_sum[turn][quad] = x;
+  if (quad == 0) s_l[turn] = sum;
+  __syncthreads();
+  if (turn != 0 || !there) return;
   sum = 0.f;
-  for (int k = 0; k < kTurns; ++k) sum += s_sum[k];
+  x = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k = 0; k < turns; ++k) {
+    const float4 y = s_sum[k][quad];
+    x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
+    sum += s_l[k];
+  }
   const int i = row / R, h = kh * R + row % R;
   const float w = sum > 0.f ? 1.f / sum : 0.f;
-  const uint32_t v = pack_bf16(x * w, y * w);
-  *reinterpret_cast<uint32_t*>(at_out(a.o, seq, i, h) + pair * 2) = v;
-  if (a.rest.p != nullptr) *reinterpret_cast<uint32_t*>(at_out(a.rest, seq, i, h) + pair * 2) = rest_of(x * w, y * w, v);
-  if (a.lse != nullptr && pair == 0) a.lse[h * ((long long)a.B * a.rq.T) + (long long)seq * a.rq.T + i] = sum > 0.f ? all + log2f(sum) : CUDART_INF_F;
+  const uint2 o = make_uint2(pack_bf16(x.x * w, x.y * w), pack_bf16(x.z * w, x.w * w));
+  *reinterpret_cast<uint2*>(at_out(a.o, seq, i, h) + quad * 4) = o;
+  if (a.rest.p != nullptr)
+    *reinterpret_cast<uint2*>(at_out(a.rest, seq, i, h) + quad * 4) =
+        make_uint2(rest_of(x.x * w, x.y * w, o.x), rest_of(x.z * w, x.w * w, o.y));
+  if (a.lse != nullptr && quad == 0)
+    a.lse[h * ((long long)a.B * a.rq.T) + (long long)seq * a.rq.T + i] = sum > 0.f ? all + log2f(sum) : CUDART_INF_F;
 }
 
 int few_columns(const AttnArgs& a) { return a.D <= 16 ? 16 : a.D <= 32 ? 32 : a.D <= 64 ? 64 : 128; }
@@ -375,8 +405,10 @@ FewPlan plan_of(const AttnArgs& a) {
     const long long want = (148 * 2 + units - 1) / units;           // blocks that fill the GPU
     const long long most = (keys + 255) / 256;
     long long s = want < most ? want : most;
-    if (s < (keys + 1023) / 1024 && a.rk.len != nullptr) s = (keys + 1023) / 1024;      // lengths may be anything: long ones are shared
-    if (s > 1024) s = 1024;
+    // Lengths may be anything: long ones are shared, 1024 keys to a block, or a 64th (4 of 131072: 95 us, with 128 splits 101).
+    const long long shares = keys > 64 * 1024 ? 64 : (keys + 1023) / 1024;
+    if (s < shares && a.rk.len != nullptr) s = shares;
+    if (s > kMaxSplits) s = kMaxSplits;
     p.chunk = (int)((keys + s - 1) / s + 63) / 64 * 64;
     p.splits = (keys + p.chunk - 1) / p.chunk;
   }
@@ -397,7 +429,9 @@ cudaError_t launch(const FewMaps& maps, const AttnArgs& a, const FewPlan& p, flo
   e = launch_pdl(k, dim3((unsigned)blocks, p.splits), dim3(32 * kWarps), S::smem, st, maps, a, p, work, ml);
   if (e != cudaSuccess || p.splits == 1) return e;
   const int rows = a.rq.T * (a.H / a.G);
-  return launch_pdl(attention_few_join_kernel<kD>, dim3((unsigned)units, rows < kRowsM ? rows : kRowsM), dim3(kJoin), 0, st, a, p, (const float*)work,
+  int turns = kD < 128 ? 128 / kD : 1;      // a warp at least
+  while (turns < kMaxTurns && turns * kAhead < p.splits) turns *= 2;
+  return launch_pdl(attention_few_join_kernel<kD>, dim3((unsigned)units, rows < kRowsM ? rows : kRowsM), dim3(turns * kD / 4), 0, st, a, p, (const float*)work,
                     (const float*)ml);
 }
 

@@ -339,3 +339,12 @@ def test_forward_mode_derivatives_are_refused(tn_gpu, status_ok):
                 call()
             with torch.no_grad(), pytest.raises((RuntimeError, NotImplementedError)):
                 call()
+
+
+@pytest.mark.parametrize("D", [16, 32, 56, 128])
+@pytest.mark.parametrize("G, lens", [(1, [40001]), (2, [70000, 1]), (1, [0, 38000, 40, 70000])])
+def test_one_query_and_keys_in_many_splits(tn_gpu, status_ok, D, G, lens):
+    dev = tn_gpu.core.runtime().device
+    B, T = len(lens), max(lens)
+    q, k, v = normal(dev, B, 1, 2 * G, D), normal(dev, B, T, G, D, seed=1), normal(dev, B, T, G, D, seed=2)
+    check(q, k, v, kv_lengths=ints(dev, *lens), slopes=slopes_of(dev, 2 * G) * 1e-3)
