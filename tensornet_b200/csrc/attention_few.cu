@@ -11,7 +11,7 @@
 //     columns 8 spread(g) + i.
 // spread() puts neighbouring groups four rows (or four pieces) apart, where the swizzle has the other half of the banks.
 // Rows of 16 or 32 columns take pieces of 4 or 8 bytes of values in the same way.
-// Measured: 512 histories of 20 to 2000 x 8 heads x 64 columns 94 us (4.8 TB/s), 2048 of 500 6.8 TB/s, 4 of 131072 x 2 key heads x 128
+// Measured: 512 histories of 20 to 2000 x 8 heads x 64 columns 89 us (5.1 TB/s), 2048 of 500 6.8 TB/s, 4 of 131072 x 2 key heads x 128
 // 95 us with the kernel that joins the splits (5.6 TB/s; a sum over as many bytes takes 100 us).
 // A sequence's keys are split over warps, blocks or both; what the blocks have of a row is brought to one reference and added by a
 // second kernel, in a fixed order.
@@ -239,6 +239,18 @@ attention_few_kernel(const __grid_constant__ FewMaps maps, const __grid_constant
     for (int r = 0; r < 2; ++r) {
       const int row = row0 + g + 8 * r;
       if (row >= rows) continue;
+      if (!whole) {
+        const long long at_part = (unit * plan.splits + blockIdx.y) * kRowsM + g + 8 * r;
+#pragma unroll
+        for (int p = 0; p < S::v_pieces; ++p)
+#pragma unroll
+          for (int f = 0; f < 2; ++f)
+#pragma unroll
+            for (int k = 0; k < S::v_cols; k += 2)
+              *reinterpret_cast<float2*>(part + at_part * kD + column(p, f) + k) = make_float2(o[p * S::v_cols + k][2 * r + f], o[p * S::v_cols + k + 1][2 * r + f]);
+        if (t == 0) *reinterpret_cast<float2*>(part_ml + 2 * at_part) = make_float2(m[r], l[r]);
+        continue;
+      }
       const int i = row / R, h = kh * R + row % R;
       const float w = l[r] > 0.f ? 1.f / l[r] : 0.f;
       __nv_bfloat16* out = at_out(a.o, seq, i, h);
@@ -401,7 +413,14 @@ FewPlan plan_of(const AttnArgs& a) {
   p.per_unit = keys <= 2048 && units >= 148 * 8 ? 1 : kWarps;
   p.splits = 1;
   p.chunk = keys;
-  if (p.per_unit > 1) {
+  if (p.per_unit == 1) {
+    // and 512 keys of long ones: a warp with 2000 that starts last ends alone.  512 histories of 20 to 2000 x 8 heads x 64 columns 94 -> 87
+    // us, 300 x 4 heads 53 -> 34, 300 x 4 x 128 columns 92 -> 63; 1000 of 500 to 1100 x 4 x 64 131 -> 134, 2000 of 10 to 600 would lose 61 -> 71.
+    if (keys > 1024) {
+      p.chunk = 512;
+      p.splits = (keys + p.chunk - 1) / p.chunk;
+    }
+  } else {
     const long long want = (148 * 2 + units - 1) / units;           // blocks that fill the GPU
     const long long most = (keys + 255) / 256;
     long long s = want < most ? want : most;

@@ -348,3 +348,16 @@ def test_one_query_and_keys_in_many_splits(tn_gpu, status_ok, D, G, lens):
     B, T = len(lens), max(lens)
     q, k, v = normal(dev, B, 1, 2 * G, D), normal(dev, B, T, G, D, seed=1), normal(dev, B, T, G, D, seed=2)
     check(q, k, v, kv_lengths=ints(dev, *lens), slopes=slopes_of(dev, 2 * G) * 1e-3)
+
+
+@pytest.mark.parametrize("D, H, G", [(16, 4, 4), (64, 8, 4), (128, 4, 4)])
+def test_many_histories_some_of_them_long(tn_gpu, status_ok, D, H, G):
+    """A warp per history and key head, or per 512 keys of it."""
+    dev = tn_gpu.core.runtime().device
+    lens = [(b * 37) % 1200 for b in range(300)]
+    lens[:6] = [0, 1, 512, 513, 1024, 1200]
+    q = normal(dev, 300, 2, H, D)
+    k, v = normal(dev, 300, 1200, G, D, seed=1), normal(dev, 300, 1200, G, D, seed=2)
+    check(q, k, v, kv_lengths=ints(dev, *lens), causal=True, slopes=slopes_of(dev, H) * 0.01)
+    go = normal(dev, 300, 2, H, D, seed=3)
+    check(q[:, :1], k, v, go[:, :1], kv_lengths=ints(dev, *lens))
