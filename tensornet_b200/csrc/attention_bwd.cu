@@ -86,7 +86,7 @@ __device__ __forceinline__ void store_acc(uint32_t tm, int from, int to, int D, 
 }
 
 // kKeys: the block owns keys; kSplit: ds in two terms
-template <int kD, bool kKeys, bool kCap, bool kBias, bool kSplit>
+template <int kD, bool kKeys, Cap kCap, bool kBias, bool kSplit>
 __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a, BwdShared<kD>& sh, uint8_t* smem_raw, int tile_at, int head) {
   using Shape = BwdShape<kD>;
   constexpr int kSlots = Shape::slots, kY = Shape::y, kParts = Shape::parts;
@@ -351,7 +351,7 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
           const float2 ls = !kKeys ? both(lse) : i % 2 == 0 ? make_float2(y4.x, y4.y) : make_float2(y4.z, y4.w);
           float2 arg, slope;
           if (kCap) {
-            const float2 th = near ? tanh_small(s[i]) : make_float2(tanh_any(s[i].x), tanh_any(s[i].y));
+            const float2 th = near ? tanh_small(s[i]) : tanh_any<kCap>(s[i]);
             arg = fma2(th, both(cap2), ls);
             slope = fma2(mul2(th, both(-1.f)), th, both(1.f));
           } else {
@@ -445,7 +445,7 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
 
 // The first key_tiles * G blocks own keys, the others queries.  Early keys are seen by the most queries and late queries see the most
 // keys: those go first.
-template <int kD, bool kCap, bool kBias, bool kSplit>
+template <int kD, Cap kCap, bool kBias, bool kSplit>
 __global__ void __launch_bounds__(BwdShape<kD>::threads, kD == 128 ? 1 : 2)
 attention_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, const __grid_constant__ AttnArgs a, int key_tiles, int query_tiles) {
   extern __shared__ uint8_t smem_raw[];
@@ -481,7 +481,7 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(const AttnArgs a, 
   if (row < rows && lane == 0) a.delta[h * rows + row] = v;
 }
 
-template <int kD, bool kCap, bool kBias, bool kSplit>
+template <int kD, Cap kCap, bool kBias, bool kSplit>
 cudaError_t launch(const BwdMaps& maps, const AttnArgs& a, cudaStream_t st) {
   auto* k = attention_bwd_tc_kernel<kD, kCap, kBias, kSplit>;
   cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, BwdShape<kD>::smem);      // of the current device
@@ -492,8 +492,9 @@ cudaError_t launch(const BwdMaps& maps, const AttnArgs& a, cudaStream_t st) {
 }
 template <int kD, bool kSplit>
 cudaError_t launch(const BwdMaps& maps, const AttnArgs& a, cudaStream_t st) {
-  if (a.cap > 0.f) return a.slopes ? launch<kD, true, true, kSplit>(maps, a, st) : launch<kD, true, false, kSplit>(maps, a, st);
-  return a.slopes ? launch<kD, false, true, kSplit>(maps, a, st) : launch<kD, false, false, kSplit>(maps, a, st);
+  return with_cap(a, [&](auto cap) {
+    return a.slopes ? launch<kD, decltype(cap)::value, true, kSplit>(maps, a, st) : launch<kD, decltype(cap)::value, false, kSplit>(maps, a, st);
+  });
 }
 
 }  // namespace

@@ -51,7 +51,8 @@ struct FewMaps {
 };
 
 // part: [unit][split][16][kD] sums and [unit][split][16][2] references and sums of weights, where there are several splits
-template <int kD>
+// kFar: the cap is above kCoarseCap
+template <int kD, bool kFar>
 __global__ void __launch_bounds__(32 * kWarps, kD == 128 ? 2 : 3)
 attention_few_kernel(const __grid_constant__ FewMaps maps, const __grid_constant__ AttnArgs a, const FewPlan plan, float* __restrict__ part,
                      float* __restrict__ part_ml) {
@@ -133,7 +134,7 @@ attention_few_kernel(const __grid_constant__ FewMaps maps, const __grid_constant
 #pragma unroll
   for (int i = 0; i < S::v_pieces * S::v_cols; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
   float m[2] = {kNone, kNone}, l[2] = {0.f, 0.f};
-  const float cs = a.cap > 0.f ? 2.f * kLog2e * a.scale / a.cap : a.scale * kLog2e;
+  const float cs = kFar ? a.scale / a.cap : a.cap > 0.f ? 2.f * kLog2e * a.scale / a.cap : a.scale * kLog2e;
   const float cap2 = a.cap * kLog2e;
   // where a lane reads: row spread(g) of eight for keys, rows t and t + 4 for values; the swizzle takes the row's number off the piece's
   const int k_row = spread(g), v_piece = kD >= 64 ? spread(g) : g;
@@ -161,14 +162,23 @@ attention_few_kernel(const __grid_constant__ FewMaps maps, const __grid_constant
       }
     }
     // score e of product c: key j0 + 8 c + spread(2 t + (e & 1)) = j0 + 8 c + t + 4 (e & 1), row g + 8 (e >> 1)
+    if (kFar)
+#pragma unroll
+      for (int c = 0; c < kTilesN; ++c)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float2 x = mul2(tanh_any<kCappedFar>(mul2(make_float2(s[c][2 * r], s[c][2 * r + 1]), both(cs))), both(cap2));
+          s[c][2 * r] = x.x;
+          s[c][2 * r + 1] = x.y;
+        }
     float top[2] = {kNone, kNone};
 #pragma unroll
     for (int c = 0; c < kTilesN; ++c)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int j = j0 + c * 8 + t + 4 * (e & 1), r = e >> 1;
-        float x = s[c][e] * cs;
-        if (a.cap > 0.f) x = cap2 - __fdividef(2.f * cap2, 1.f + ex2(x));
+        float x = kFar ? s[c][e] : s[c][e] * cs;
+        if (!kFar && a.cap > 0.f) x = cap2 - __fdividef(2.f * cap2, 1.f + ex2(x));
         if (a.slopes != nullptr) x -= slope2[r] * fabsf((float)(place[r] - j));
         if (masked) x = j < min(lim[r], to) ? x : kNone;
         s[c][e] = x;
@@ -438,7 +448,7 @@ template <int kD>
 cudaError_t launch(const FewMaps& maps, const AttnArgs& a, const FewPlan& p, float* work, cudaStream_t st) {
   using S = FewShape<kD>;
   static_assert(kWarps * kRowsM * (kD + 4) * 4 <= S::smem, "the warps' results take the place of the rings");
-  auto* k = attention_few_kernel<kD>;
+  auto* k = a.cap > kCoarseCap ? attention_few_kernel<kD, true> : attention_few_kernel<kD, false>;
   cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::smem);      // of the current device
   if (e != cudaSuccess) return e;
   const long long units = (long long)a.B * a.G * p.row_blocks;

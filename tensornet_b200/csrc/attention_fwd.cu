@@ -72,7 +72,7 @@ struct FwdMaps {
   CUtensorMap q, k, v;
 };
 
-template <int kD, int kTiles, bool kCap, bool kBias>
+template <int kD, int kTiles, Cap kCap, bool kBias>
 __global__ void __launch_bounds__(FwdShape<kD, kTiles, kCap ? 2 : 1>::threads, FwdShape<kD, kTiles, kCap ? 2 : 1>::blocks)
 attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_constant__ AttnArgs a, int tiles, int heads_first) {
   constexpr int kHalves = kCap ? 2 : 1;      // threads per query
@@ -297,7 +297,7 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
             for (int e = 0; e < 16; ++e) x[e] = mul2(tanh_small(x[e]), both(cap2));
           } else {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) x[e] = make_float2(cap2 * tanh_any(x[e].x), cap2 * tanh_any(x[e].y));
+            for (int e = 0; e < 16; ++e) x[e] = mul2(tanh_any<kCap>(x[e]), both(cap2));
           }
         }
         if (kBias) {
@@ -430,7 +430,7 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
   if (warp == 0) tmem_dealloc<Shape::tmem_cols>(tmem);
 }
 
-template <int kD, int kTiles, bool kCap, bool kBias>
+template <int kD, int kTiles, Cap kCap, bool kBias>
 cudaError_t launch(const FwdMaps& maps, const AttnArgs& a, cudaStream_t st) {
   using Shape = FwdShape<kD, kTiles, kCap ? 2 : 1>;
   auto* k = attention_fwd_tc_kernel<kD, kTiles, kCap, kBias>;
@@ -442,8 +442,9 @@ cudaError_t launch(const FwdMaps& maps, const AttnArgs& a, cudaStream_t st) {
 }
 template <int kD, int kTiles>
 cudaError_t launch(const FwdMaps& maps, const AttnArgs& a, cudaStream_t st) {
-  if (a.cap > 0.f) return a.slopes ? launch<kD, kTiles, true, true>(maps, a, st) : launch<kD, kTiles, true, false>(maps, a, st);
-  return a.slopes ? launch<kD, kTiles, false, true>(maps, a, st) : launch<kD, kTiles, false, false>(maps, a, st);
+  return with_cap(a, [&](auto cap) {
+    return a.slopes ? launch<kD, kTiles, decltype(cap)::value, true>(maps, a, st) : launch<kD, kTiles, decltype(cap)::value, false>(maps, a, st);
+  });
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,

@@ -2,8 +2,7 @@
 //
 // Queries stand at the end of their keys: query i of a sequence with nq queries and nk keys stands at place i + nk - nq.  Key j is
 // visible if j < nk and, where causal, j <= place or j < prefix: every mask is a limit per query, the number of keys it sees.
-// Scores are kept in units of log2:  s = c q.k,  or cap tanh(scale q.k / cap) with a cap, less slope |place - j|.  The tanh is
-// 1 - 2 / (1 + e^2x), one exponential: off by 2^-23 of its range, not of its value, which is what a score needs.
+// Scores are kept in units of log2:  s = c q.k,  or cap tanh(scale q.k / cap) with a cap, less slope |place - j|.
 #pragma once
 #include <cuda_bf16.h>
 #include <math_constants.h>

@@ -128,7 +128,7 @@ __device__ __forceinline__ void store_rows(const AttnOperand& to, int b, long lo
 }
 
 // A warp takes `heads` heads of its tile, one after another.
-template <int kD, bool kCap, bool kBias>
+template <int kD, Cap kCap, bool kBias>
 __global__ void __launch_bounds__(32 * kWarps, kD == 16 ? 6 : kD == 32 ? 4 : 3) attention_short_fwd_kernel(const __grid_constant__ AttnArgs a, unsigned tiles, unsigned heads) {
   using P = Pieces<kD>;
   pdl_sync();
@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(32 * kWarps, kD == 16 ? 6 : kD == 32 ? 4 : 3) 
           float2 x = s[c][r];
           if (kCap) {
             x = mul2(x, both(cs));
-            x = make_float2(cap2 * tanh_any(x.x), cap2 * tanh_any(x.y));
+            x = mul2(tanh_any<kCap>(x), both(cap2));
           }
           if (kBias) {
             const float away = row[r] - (float)(j0 + 8 * c);
@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(32 * kWarps, kD == 16 ? 6 : kD == 32 ? 4 : 3) 
 }
 
 // kKeys: the warp owns keys; see attention_bwd.cu for X and Y
-template <int kD, bool kCap, bool kBias, bool kKeys>
+template <int kD, Cap kCap, bool kBias, bool kKeys>
 __device__ __forceinline__ void short_bwd(const AttnArgs& a, int tile_at, int head0, int head1) {
   using P = Pieces<kD>;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -345,7 +345,7 @@ __device__ __forceinline__ void short_bwd(const AttnArgs& a, int tile_at, int he
             float2 arg, slope;
             if (kCap) {
               const float2 y = mul2(s[c][r], both(cs));
-              const float2 th = make_float2(tanh_any(y.x), tanh_any(y.y));
+              const float2 th = tanh_any<kCap>(y);
               arg = fma2(th, both(cap2), lg);
               slope = fma2(mul2(th, both(-1.f)), th, both(1.f));
             } else {
@@ -386,7 +386,7 @@ __device__ __forceinline__ void short_bwd(const AttnArgs& a, int tile_at, int he
 }
 
 // The first key_units warps own keys, the others queries.
-template <int kD, bool kCap, bool kBias>
+template <int kD, Cap kCap, bool kBias>
 __global__ void __launch_bounds__(32 * kWarps, kD == 16 ? 4 : kD == 32 ? 3 : 2)
 attention_short_bwd_kernel(const __grid_constant__ AttnArgs a, unsigned key_units, unsigned units, unsigned key_heads, unsigned heads) {
   pdl_sync();
@@ -409,7 +409,7 @@ unsigned heads_of(long long tiles, int H) {
   return n;
 }
 
-template <int kD, bool kCap, bool kBias>
+template <int kD, Cap kCap, bool kBias>
 cudaError_t launch_fwd(const AttnArgs& a, cudaStream_t st) {
   const long long tiles = tile_count(a.rq, a.B, kM);
   const unsigned heads = heads_of(tiles, a.H);
@@ -418,7 +418,7 @@ cudaError_t launch_fwd(const AttnArgs& a, cudaStream_t st) {
   return launch_pdl(attention_short_fwd_kernel<kD, kCap, kBias>, dim3((unsigned)((units + kWarps - 1) / kWarps)), dim3(32 * kWarps), 0, st, a,
                     (unsigned)tiles, heads);
 }
-template <int kD, bool kCap, bool kBias>
+template <int kD, Cap kCap, bool kBias>
 cudaError_t launch_bwd(const AttnArgs& a, cudaStream_t st) {
   const long long key_tiles = tile_count(a.rk, a.B, kM), tiles = tile_count(a.rq, a.B, kM);
   const unsigned key_heads = heads_of(key_tiles, a.G), heads = heads_of(tiles, a.H);
@@ -429,10 +429,11 @@ cudaError_t launch_bwd(const AttnArgs& a, cudaStream_t st) {
 }
 template <int kD>
 cudaError_t launch(bool fwd, const AttnArgs& a, cudaStream_t st) {
-  if (a.cap > 0.f && a.slopes) return fwd ? launch_fwd<kD, true, true>(a, st) : launch_bwd<kD, true, true>(a, st);
-  if (a.cap > 0.f) return fwd ? launch_fwd<kD, true, false>(a, st) : launch_bwd<kD, true, false>(a, st);
-  if (a.slopes) return fwd ? launch_fwd<kD, false, true>(a, st) : launch_bwd<kD, false, true>(a, st);
-  return fwd ? launch_fwd<kD, false, false>(a, st) : launch_bwd<kD, false, false>(a, st);
+  return with_cap(a, [&](auto cap) {
+    constexpr Cap kCap = decltype(cap)::value;
+    if (a.slopes) return fwd ? launch_fwd<kD, kCap, true>(a, st) : launch_bwd<kD, kCap, true>(a, st);
+    return fwd ? launch_fwd<kD, kCap, false>(a, st) : launch_bwd<kD, kCap, false>(a, st);
+  });
 }
 const char* told(cudaError_t e) {
   if (e == cudaSuccess) e = cudaGetLastError();

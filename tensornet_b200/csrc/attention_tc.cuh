@@ -4,6 +4,7 @@
 // serves as either side of a product: along its columns (K-major) for q k^T, along its rows (MN-major) for p v.
 #pragma once
 #include <cuda.h>
+#include <type_traits>
 #include "attention_rows.cuh"
 #include "tc_primitives.cuh"
 
@@ -60,19 +61,37 @@ __device__ __forceinline__ float2 ex2_poly(float2 x) {
   return add2(p, both(-c0 * 2.3509887016445750e-38f));           // 2^-125
 }
 
-// tanh for |y| <= 1: y times a polynomial in y^2, least squares reweighted towards the smallest largest error of tanh itself
-// (2.4e-7, 3.2e-7 in fp32).  No exponential, and two at a time.
+// tanh for |y| <= 1: y times a polynomial in y^2, least squares reweighted towards the smallest largest relative error (5.9e-7, 7.0e-7 in
+// fp32): with a cap far above it, a score has to be off by little of its own size.  No exponential, and two at a time.
 __device__ __forceinline__ float2 tanh_small(float2 y) {
   const float2 z = mul2(y, y);
-  float2 p = fma2(z, both(-0.002839465159922838f), both(0.01611418090760708f));
-  p = fma2(z, p, both(-0.05097286403179169f));
-  p = fma2(z, p, both(0.13253524899482727f));
-  p = fma2(z, p, both(-0.3332400321960449f));
-  p = fma2(z, p, both(0.9999968409538269f));
+  float2 p = fma2(z, both(-0.0030670601408928633f), both(0.016743114218115807f));
+  p = fma2(z, p, both(-0.051605671644210815f));
+  p = fma2(z, p, both(0.13281433284282684f));
+  p = fma2(z, p, both(-0.3332904279232025f));
+  p = fma2(z, p, both(0.9999994039535522f));
   return mul2(y, p);
 }
-// and for any y
-__device__ __forceinline__ float tanh_any(float y) { return 1.f - __fdividef(2.f, 1.f + ex2(2.f * kLog2e * y)); }
+// and for any y.  1 - 2 / (1 + e^2y), one exponential, is off by some 2^-22 of 1, which may be all of a small tanh: a score is off by that
+// much of its cap.  Up to kCoarseCap that is 2^-14, little beside the 2^-8 that rounding to bf16 moves its weight by; above, small values come
+// of the polynomial, each by itself, in instances of their own: 8192 causal tokens x 16 heads x 128 columns 487 + 1074 us in place of 404 +
+// 1050, 4096 sequences of 1 to 200 x 4 heads x 16 columns 127 + 300 in place of 119 + 288.
+constexpr float kCoarseCap = 256.f;
+enum Cap { kUncapped, kCapped, kCappedFar };
+template <Cap kCap>
+__device__ __forceinline__ float2 tanh_any(float2 y) {
+  const float2 far = make_float2(1.f - __fdividef(2.f, 1.f + ex2(2.f * kLog2e * y.x)), 1.f - __fdividef(2.f, 1.f + ex2(2.f * kLog2e * y.y)));
+  if (kCap != kCappedFar) return far;
+  const float2 near = tanh_small(y);
+  return make_float2(fabsf(y.x) <= 1.f ? near.x : far.x, fabsf(y.y) <= 1.f ? near.y : far.y);
+}
+// launch(...) of the instance that a call wants
+template <typename F>
+cudaError_t with_cap(const AttnArgs& a, F&& launch) {
+  if (!(a.cap > 0.f)) return launch(std::integral_constant<Cap, kUncapped>{});
+  if (a.cap <= kCoarseCap) return launch(std::integral_constant<Cap, kCapped>{});
+  return launch(std::integral_constant<Cap, kCappedFar>{});
+}
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int t, int h, int b, uint32_t bar) {
   asm volatile(
