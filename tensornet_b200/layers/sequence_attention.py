@@ -59,7 +59,7 @@ class SequenceAttention(nn.Module):
         if target is not None and (target.dim() not in (2, 3) or target.shape[0] != x.shape[0] or target.shape[-1] != self.dim):
             raise ValueError(f"{self.layer_name}: targets [{x.shape[0]}, (n,) {self.dim}], not {tuple(target.shape)}")
         lead, D = x.shape[:2], self.head_dim
-        asks = x if target is None else target.view(x.shape[0], -1, self.dim)
+        asks = x if target is None else target.unsqueeze(1) if target.dim() == 2 else target
         if asks.numel() == 0 or (target is None and x.numel() == 0):
             return x if target is None else target
         if lengths is not None:
