@@ -29,6 +29,8 @@ struct AttnArgs {
   const float* slopes;         // [H] or null
   const int* prefix;           // [B] or null
   int causal;
+  int newest;                  // every query stands at the last key (not with causal)
+  float step;                  // of a query's place to the next one's: 0 where newest, else 1
   // backward
   AttnOperand go, gq, gk, gv;
   float* delta;                // [H][rows of q] workspace

@@ -293,6 +293,7 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
     // keys: the queries [meet, qs.n) see this one; queries: keys [0, meet) are seen
     const int meet = x < xs.n ? (kKeys ? first_query(a, tile.seq, x, qs.n, ks.n) : keys_seen(a, tile.seq, x, qs.n, ks.n)) : (kKeys ? lo : hi);
     const int shift = ks.n - qs.n;
+    const int place = place_of(a, x, qs.n, ks.n), place0 = place_of(a, tile.first, qs.n, ks.n), places = a.newest ? 1 : kX;      // of queries' owners
     float lse = 0.f, delta = 0.f;      // negative
     if (!kKeys && x < xs.n) {
       lse = -a.lse[head * q_rows + q_flat + x];
@@ -341,9 +342,9 @@ __device__ __forceinline__ void bwd_block(const BwdMaps& maps, const AttnArgs& a
           near = __all_sync(0xffffffffu, x >= xs.n || fmaxf(far[0], far[1]) <= 1.f);
         }
         // the distance of columns from a row is linear where all lie on one side
-        const float from = (float)(kKeys ? y0 + c0 + shift - x : x + shift - y0 - c0), per = kKeys ? 1.f : -1.f;
-        const bool one_side = kBias && (kKeys ? y0 + c0 + shift >= tile.first + kX || y0 + c0 + kPart + shift <= tile.first
-                                              : tile.first + shift >= y0 + c0 + kPart || tile.first + kX + shift <= y0 + c0);
+        const float from = (float)(!kKeys ? place - y0 - c0 : a.newest ? ks.n - 1 - x : y0 + c0 + shift - x), per = !kKeys ? -1.f : a.newest ? 0.f : 1.f;
+        const bool one_side = kBias && (kKeys ? a.newest || y0 + c0 + shift >= tile.first + kX || y0 + c0 + kPart + shift <= tile.first
+                                              : place0 >= y0 + c0 + kPart || place0 + places <= y0 + c0);
         const float2 tilt = both(from + per > 0.f ? -slope2 : slope2);
 #pragma unroll
         for (int i = 0; i < kPart / 2; ++i) {

@@ -117,7 +117,7 @@ attention_few_kernel(const __grid_constant__ FewMaps maps, const __grid_constant
     const bool there = r < rows && i < qs.n;
     lim[e] = there ? keys_seen(a, seq, i, qs.n, ks.n) : 0;
     if (there) least = min(least, lim[e]);
-    place[e] = i + ks.n - qs.n;
+    place[e] = place_of(a, i, qs.n, ks.n);
     slope2[e] = there && a.slopes ? a.slopes[h] * kLog2e : 0.f;
 #pragma unroll
     for (int p = 0; p < S::k_pieces; ++p) {

@@ -256,8 +256,8 @@ attention_fwd_tc_kernel(const __grid_constant__ FwdMaps maps, const __grid_const
     const float c = kCap ? a.scale / a.cap : a.scale * kLog2e;
     const float cap2 = a.cap * kLog2e;
     const float slope2 = kBias ? a.slopes[h] * kLog2e : 0.f;
-    const int place0 = tile.first + t * kRows + ks.n - qs.n;          // of the tile's first query
-    const int place = i + ks.n - qs.n;
+    const int place0 = place_of(a, tile.first + t * kRows, qs.n, ks.n);          // of the tile's first query
+    const int place = place_of(a, i, qs.n, ks.n);
     float m = kNone, l = 0.f;
     const int d_half = kHalves == 2 ? round16(d16 / 2) : d16;
     bool ok = true;

@@ -1,7 +1,7 @@
 // Sequences, masks and scores as every attention kernel of this library sees them.
 //
-// Queries stand at the end of their keys: query i of a sequence with nq queries and nk keys stands at place i + nk - nq.  Key j is
-// visible if j < nk and, where causal, j <= place or j < prefix: every mask is a limit per query, the number of keys it sees.
+// Queries stand at the end of their keys: query i of a sequence with nq queries and nk keys stands at place i + nk - nq, or all of them,
+// where they are newest, at nk - 1.  Key j is visible if j < nk and, where causal, j <= place or j < prefix: every mask is a limit per query, the number of keys it sees.
 // Scores are kept in units of log2:  s = c q.k,  or cap tanh(scale q.k / cap) with a cap, less slope |place - j|.
 #pragma once
 #include <cuda_bf16.h>
@@ -64,6 +64,9 @@ __device__ __forceinline__ int keys_seen(const AttnArgs& a, int seq, int i, int 
   if (a.prefix != nullptr) lim = max(lim, a.prefix[seq]);
   return cut(lim, 0, nk);
 }
+
+// the place of query i among the keys
+__device__ __forceinline__ int place_of(const AttnArgs& a, int i, int nq, int nk) { return a.newest ? nk - 1 : i + nk - nq; }
 
 // the first query of a sequence that sees key j
 __device__ __forceinline__ int first_query(const AttnArgs& a, int seq, int j, int nq, int nk) {

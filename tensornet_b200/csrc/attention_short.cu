@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(32 * kWarps, kD == 16 ? 6 : kD == 32 ? 4 : 3) 
     qs = span_of(a.rq, tile.seq);
     ks = span_of(a.rk, tile.seq);
   }
-  const int x0 = tile.first, shift = ks.n - qs.n;
+  const int x0 = tile.first;
   // keys_seen grows with the query
   const int vis = x0 < qs.n ? keys_seen(a, tile.seq, min(x0 + kM, qs.n) - 1, qs.n, ks.n) : 0;
   const int least = x0 + kM <= qs.n ? keys_seen(a, tile.seq, x0, qs.n, ks.n) : 0;
@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(32 * kWarps, kD == 16 ? 6 : kD == 32 ? 4 : 3) 
   for (int e = 0; e < 2; ++e) {
     const int x = x0 + g + 8 * e;
     lim[e] = (x < qs.n ? keys_seen(a, tile.seq, x, qs.n, ks.n) : 0) - 2 * t;
-    row[e] = (float)(x + shift - 2 * t);
+    row[e] = (float)(place_of(a, x, qs.n, ks.n) - 2 * t);
   }
   const float cs = kCap ? a.scale / a.cap : a.scale * kLog2e, cap2 = a.cap * kLog2e;
   const long long q_rows = flat_rows(a.rq, a.B), flat = (a.rq.off ? 0 : (long long)qs.b * a.rq.T) + qs.first + x0 + g;
@@ -282,7 +282,7 @@ __device__ __forceinline__ void short_bwd(const AttnArgs& a, int tile_at, int he
   for (int e = 0; e < 2; ++e) {
     const int x = x0 + g + 8 * e;
     meet[e] = (x >= xs.n ? 0 : kKeys ? first_query(a, tile.seq, x, qs.n, ks.n) : keys_seen(a, tile.seq, x, qs.n, ks.n)) - 2 * t;
-    row[e] = (float)((kKeys ? x - shift : x + shift) - 2 * t);
+    row[e] = (float)(!kKeys ? place_of(a, x, qs.n, ks.n) - 2 * t : a.newest ? x - (ks.n - 1) : x - shift - 2 * t);
   }
   const float cs = kCap ? a.scale / a.cap : a.scale * kLog2e, cap2 = a.cap * kLog2e;
   const AttnOperand &o1 = kKeys ? a.q : a.k, &o2 = kKeys ? a.go : a.v;
@@ -352,8 +352,8 @@ __device__ __forceinline__ void short_bwd(const AttnArgs& a, int tile_at, int he
               arg = fma2(s[c][r], both(cs), lg);
             }
             if (kBias) {
-              const float away = row[r] - (float)(y0 + 8 * c);
-              arg = add2(arg, make_float2(slope2 * fabsf(away), slope2 * fabsf(away - 1.f)));
+              const float at_y = (float)(y0 + 8 * c), away = kKeys ? fmaf(-a.step, at_y, row[r]) : row[r] - at_y;
+              arg = add2(arg, make_float2(slope2 * fabsf(away), slope2 * fabsf(away - (kKeys ? a.step : 1.f))));
             }
             float2 p = make_float2(ex2(arg.x), ex2(arg.y));
             float2 ds = mul2(p, add2(d[c][r], dl));

@@ -148,7 +148,7 @@ const int* ints_of(const OptTensor& t, const at::Tensor& q, int64_t n, const cha
 
 struct Attention : torch::autograd::Function<Attention> {
   static tn::AttnArgs args_of(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const OptTensor& q_rows, const OptTensor& k_rows,
-                              const OptTensor& prefix, const OptTensor& slopes, bool causal, double cap, double scale, const at::Tensor& status) {
+                              const OptTensor& prefix, const OptTensor& slopes, bool causal, bool newest, double cap, double scale, const at::Tensor& status) {
     for (const at::Tensor* t : {&q, &k, &v})
       TORCH_CHECK(t->is_cuda() && t->device() == q.device() && t->scalar_type() == at::kBFloat16 && (t->dim() == 3 || t->dim() == 4) &&
                       t->size(-1) == q.size(-1), "attention: bf16 operands [N, heads, columns] or [B, T, heads, columns] on one GPU");
@@ -175,16 +175,17 @@ struct Attention : torch::autograd::Function<Attention> {
                   "attention: slopes must be fp32, one per query head");
       a.slopes = slopes->data_ptr<float>();
     }
-    a.causal = causal; a.cap = (float)cap; a.scale = (float)scale; a.status = status_of(status, q);
+    TORCH_CHECK(!(causal && newest), "attention: newest queries see all keys, causal ones do not");
+    a.causal = causal; a.newest = newest; a.step = newest ? 0.f : 1.f; a.cap = (float)cap; a.scale = (float)scale; a.status = status_of(status, q);
     return a;
   }
 
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in, const OptTensor& q_rows,
-                            const OptTensor& k_rows, const OptTensor& prefix, const OptTensor& slopes, bool causal, double cap, double scale,
+                            const OptTensor& k_rows, const OptTensor& prefix, const OptTensor& slopes, bool causal, bool newest, double cap, double scale,
                             const at::Tensor& status, bool keep) {
     c10::cuda::CUDAGuard guard(q_in.device());
     const at::Tensor q = operand(q_in), k = operand(k_in), v = operand(v_in);
-    tn::AttnArgs a = args_of(q, k, v, q_rows, k_rows, prefix, slopes, causal, cap, scale, status);
+    tn::AttnArgs a = args_of(q, k, v, q_rows, k_rows, prefix, slopes, causal, newest, cap, scale, status);
     at::Tensor out = at::empty(q.sizes(), q.options()), lse, rest;
     a.o = view_of(out);
     if (out.numel() > 0 && k.numel() == 0) out.zero_();
@@ -212,6 +213,7 @@ struct Attention : torch::autograd::Function<Attention> {
       auto opt = [](const OptTensor& t) { return t ? *t : at::Tensor(); };
       ctx->save_for_backward({q, k, v, out, lse, rest, opt(q_rows), opt(k_rows), opt(prefix), opt(slopes)});
       ctx->saved_data["causal"] = causal;
+      ctx->saved_data["newest"] = newest;
       ctx->saved_data["cap"] = cap;
       ctx->saved_data["scale"] = scale;
       ctx->saved_data["status"] = status;
@@ -226,7 +228,8 @@ struct Attention : torch::autograd::Function<Attention> {
     c10::cuda::CUDAGuard guard(q.device());
     const at::Tensor go = operand(grads[0]);
     tn::AttnArgs a = args_of(q, k, v, some(s[6]), some(s[7]), some(s[8]), some(s[9]), ctx->saved_data["causal"].toBool(),
-                             ctx->saved_data["cap"].toDouble(), ctx->saved_data["scale"].toDouble(), ctx->saved_data["status"].toTensor());
+                             ctx->saved_data["newest"].toBool(), ctx->saved_data["cap"].toDouble(), ctx->saved_data["scale"].toDouble(),
+                             ctx->saved_data["status"].toTensor());
     TORCH_CHECK(go.scalar_type() == at::kBFloat16 && go.sizes() == q.sizes(), "attention: the output's gradient must be like the output");
     at::Tensor gq = at::empty(q.sizes(), q.options()), gk = at::empty(k.sizes(), k.options()), gv = at::empty(v.sizes(), v.options());
     if (q.numel() > 0 && k.numel() > 0) {
@@ -238,7 +241,7 @@ struct Attention : torch::autograd::Function<Attention> {
     } else {
       for (at::Tensor* t : {&gq, &gk, &gv}) t->zero_();
     }
-    variable_list r(12);
+    variable_list r(13);
     if (ctx->needs_input_grad(0)) r[0] = gq;
     if (ctx->needs_input_grad(1)) r[1] = gk;
     if (ctx->needs_input_grad(2)) r[2] = gv;
@@ -247,11 +250,11 @@ struct Attention : torch::autograd::Function<Attention> {
 };
 
 at::Tensor attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const OptTensor& q_rows, const OptTensor& k_rows,
-                     const OptTensor& prefix, const OptTensor& slopes, bool causal, double cap, double scale, const at::Tensor& status) {
+                     const OptTensor& prefix, const OptTensor& slopes, bool causal, bool newest, double cap, double scale, const at::Tensor& status) {
   const bool keep = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad());
   if (!keep && !dual(q) && !dual(k) && !dual(v))
-    return Attention::forward(nullptr, q, k, v, q_rows, k_rows, prefix, slopes, causal, cap, scale, status, false);
-  return Attention::apply(q, k, v, q_rows, k_rows, prefix, slopes, causal, cap, scale, status, keep);
+    return Attention::forward(nullptr, q, k, v, q_rows, k_rows, prefix, slopes, causal, newest, cap, scale, status, false);
+  return Attention::apply(q, k, v, q_rows, k_rows, prefix, slopes, causal, newest, cap, scale, status, keep);
 }
 
 }  // namespace

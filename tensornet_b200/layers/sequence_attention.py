@@ -18,7 +18,7 @@ class SequenceAttention(nn.Module):
     * ``layer(x, lengths)``: ``x + attention(norm(x)) W_o`` of ``[B, T, dim]`` sequences, ``lengths[b]`` rows each (None: all).  Rows
       behind a length, which have to be finite, come back as they were.
     * ``layer(x, lengths, target)``: what targets ``[B, dim]`` or ``[B, n, dim]`` (candidate items, say) gather from the
-      sequence, ``target + attention(norm(target), norm(x)) W_o``.
+      sequence, ``target + attention(norm(target), norm(x)) W_o``, each by itself: all stand at the sequence's last row.
 
     Projections are bf16 products with biases, attention is :func:`tensornet_b200.ops.functional.attention`: ``heads`` of
     ``head_dim`` columns (``dim // heads``, a multiple of 8), ``kv_heads`` of them for keys and values.  ``causal``: a row sees
@@ -77,7 +77,7 @@ class SequenceAttention(nn.Module):
             kv = projected(rows, self.key_value)
             k, v = [self._heads_of(kv, lead, self.kv_heads, D, i * self.kv_heads) for i in range(2)]
         out = F.attention(q, k, v, lengths=lengths if target is None else None, kv_lengths=lengths, causal=self.causal and target is None,
-                          prefix=prefix, cap=self.cap, slopes=self.slopes)
+                          prefix=prefix, cap=self.cap, slopes=self.slopes, newest=target is not None)
         y = F.mlp(F.concat_cast([out.reshape(-1, self.heads * D)]), [self.output], self.heads * D, relu_last=False)
         y = y[:, :self.dim].float().view(asks.shape)
         if target is None and lengths is not None:

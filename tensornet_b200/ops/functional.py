@@ -691,7 +691,7 @@ def layer_norm(x: torch.Tensor, gamma: Optional[torch.Tensor] = None, beta: Opti
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, lengths: Optional[torch.Tensor] = None,
               kv_lengths: Optional[torch.Tensor] = None, offsets: Optional[torch.Tensor] = None, kv_offsets: Optional[torch.Tensor] = None,
               causal: bool = False, prefix: Optional[torch.Tensor] = None, cap: Optional[float] = None,
-              slopes: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> torch.Tensor:
+              slopes: Optional[torch.Tensor] = None, scale: Optional[float] = None, newest: bool = False) -> torch.Tensor:
     """Scaled dot-product attention of each sequence's queries over its own keys; the result has ``q``'s shape.
 
     Operands are bf16, 8 to 128 columns (a multiple of 8), with sums and softmax in fp32.  Padded ones are ``[B, T, heads,
@@ -702,7 +702,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, lengths: Opt
     do not start on 16 bytes are copied first.
 
     A sequence's queries stand at the end of its keys: query ``i`` of ``nq`` is at place ``i + nk - nq`` of ``nk`` keys, so that one
-    query is the newest token.  Its score with key ``j`` is ``scale * q.k``, with ``cap`` (0 and None: none) as ``cap * tanh(scale * q.k / cap)``, less
+    query is the newest token; with ``newest`` (not with ``causal``) each of them is, at place ``nk - 1``, as candidates are that are
+    scored beside one another.  Its score with key ``j`` is ``scale * q.k``, with ``cap`` (0 and None: none) as ``cap * tanh(scale * q.k / cap)``, less
     ``slopes[h] * |place - j|`` (fp32 ``[heads]``, constants).  ``causal`` hides the keys behind a query's place, but for the first
     ``prefix[b]`` (int32 ``[B]``) keys of the sequence, which all its queries see.  ``scale`` defaults to ``columns ** -0.5``.
 
@@ -735,6 +736,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, lengths: Opt
         if prefix.dtype != torch.int32 or prefix.shape != (B,) or prefix.device != q.device:
             raise ValueError(f"attention: prefix must be int32 [{B}] on {q.device}")
         prefix = prefix.contiguous()
+    if newest and causal:
+        raise ValueError("attention: newest queries see all keys, causal ones do not")
     if slopes is not None:
         if slopes.dtype != torch.float32 or slopes.shape != (H,) or slopes.device != q.device:
             raise ValueError(f"attention: slopes must be fp32 [{H}] on {q.device}")
@@ -746,8 +749,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, lengths: Opt
     if not cap >= 0.0 or not 1e-30 < scale < 1e30 or (cap and not (1e-30 < cap < 1e30 and 1e-30 < scale / cap < 1e30)):
         raise ValueError(f"attention: scale ({scale}) must be above zero, and so must cap ({cap or None}); they and their ratio are fp32")
     if q.is_cuda:
-        return _ext().attention(q, k, v, q_rows, k_rows, prefix, slopes, bool(causal), cap, scale, _status())
-    return _attention_cpu(q, k, v, (q_rows, k_rows), B, bool(causal), prefix, cap, slopes, scale)
+        return _ext().attention(q, k, v, q_rows, k_rows, prefix, slopes, bool(causal), bool(newest), cap, scale, _status())
+    return _attention_cpu(q, k, v, (q_rows, k_rows), B, bool(causal), bool(newest), prefix, cap, slopes, scale)
 
 
 def _sequence_rows(what, packed, offsets, lengths, dev):
@@ -764,7 +767,7 @@ def _sequence_rows(what, packed, offsets, lengths, dev):
     return r if r.is_contiguous() else r.contiguous()
 
 
-def _attention_cpu(q, k, v, rows, B, causal, prefix, cap, slopes, scale):
+def _attention_cpu(q, k, v, rows, B, causal, newest, prefix, cap, slopes, scale):
     R = q.shape[-2] // k.shape[-2]
     out = torch.zeros(q.shape, dtype=torch.float32)
 
@@ -784,7 +787,7 @@ def _attention_cpu(q, k, v, rows, B, causal, prefix, cap, slopes, scale):
         s = qb @ kb.transpose(1, 2) * scale
         if cap:
             s = cap * torch.tanh(s / cap)
-        place = torch.arange(nq).unsqueeze(1) + (nk - nq)
+        place = torch.full((nq, 1), nk - 1) if newest else torch.arange(nq).unsqueeze(1) + (nk - nq)
         j = torch.arange(nk)
         if slopes is not None:
             s = s - slopes.view(-1, 1, 1) * (place - j).abs()

@@ -11,7 +11,7 @@ import torch
 pytestmark = pytest.mark.gpu
 
 
-def _definition(q, k, v, go, lengths, kv_lengths, causal, cap, slopes):
+def definition(q, k, v, go, lengths, kv_lengths, causal, cap, slopes, newest=False):
     """``[out, gq, gk, gv]`` in 64 bits and how far each may be off, ``[B, T, heads, columns]``."""
     u, f, g18 = 2.0 ** -8, 2.0 ** -12, 2.0 ** -18
     q64, k64, v64, g64 = [t.detach().cpu().double() for t in (q, k, v, go)]
@@ -26,11 +26,11 @@ def _definition(q, k, v, go, lengths, kv_lengths, causal, cap, slopes):
         kb, vb = [t[b, :nk].transpose(0, 1).repeat_interleave(R, dim=0) for t in (k64, v64)]
         x = qb @ kb.transpose(1, 2) * scale
         size = qb.abs() @ kb.abs().transpose(1, 2) * scale
-        th = torch.tanh(x / cap)
-        place = torch.arange(nq).view(-1, 1) + nk - nq
+        th = torch.tanh(x / cap) if cap else torch.zeros_like(x)
+        place = torch.full((nq, 1), nk - 1) if newest else torch.arange(nq).view(-1, 1) + nk - nq
         j = torch.arange(nk).view(1, -1)
         bias = slopes.cpu().double().view(-1, 1, 1) * (place - j).abs()
-        x, size = cap * th - bias, size + bias
+        x, size = (cap * th if cap else x) - bias, size + bias
         if causal:
             x = x.masked_fill(j > place, -torch.inf)
         p = torch.softmax(x, dim=-1).nan_to_num()          # rows that see nothing
@@ -85,7 +85,7 @@ def _check(dev, shape, cap, cut):
     out = F.attention(*leaves, lengths=torch.tensor(lengths, dtype=torch.int32, device=dev), causal=causal, cap=cap, slopes=slopes,
                       kv_lengths=torch.tensor(kv_lengths, dtype=torch.int32, device=dev))
     got = [out.detach(), *(torch.autograd.grad(out, leaves, go) if train else ())]
-    want, tol = _definition(q, k, v, go, lengths, kv_lengths, causal, cap, slopes)
+    want, tol = definition(q, k, v, go, lengths, kv_lengths, causal, cap, slopes)
     for name, a, b, t in zip(("out", "gq", "gk", "gv"), got, want, tol):
         off = (a.cpu().double() - b).abs() - t
         assert bool((off <= 1e-30).all()), (name, float(off.max()), float(b.abs().max()), int((off > 0).sum()))
