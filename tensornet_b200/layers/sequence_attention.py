@@ -22,7 +22,7 @@ class SequenceAttention(nn.Module):
 
     Projections are bf16 products with biases, attention is :func:`tensornet_b200.ops.functional.attention`: ``heads`` of
     ``head_dim`` columns (``dim // heads``, a multiple of 8), ``kv_heads`` of them for keys and values.  ``causal``: a row sees
-    itself and the rows before it; ``prefix`` (int32 ``[B]``, call) rows are seen by all the same.  ``cap`` bounds the scores,
+    itself and the rows before it; ``prefix`` (int32 ``[B]``, call without targets) rows are seen by all the same.  ``cap`` bounds the scores,
     ``distance_bias`` lets them fall with the distance, by ``2^(-8 (h + 1) / heads)`` per row in head ``h``."""
 
     def __init__(self, dim: int, heads: int = 4, kv_heads: Optional[int] = None, head_dim: Optional[int] = None, causal: bool = False,
@@ -58,6 +58,8 @@ class SequenceAttention(nn.Module):
             raise ValueError(f"{self.layer_name}: sequences [B, T, {self.dim}], not {tuple(x.shape)}")
         if target is not None and (target.dim() not in (2, 3) or target.shape[0] != x.shape[0] or target.shape[-1] != self.dim):
             raise ValueError(f"{self.layer_name}: targets [{x.shape[0]}, (n,) {self.dim}], not {tuple(target.shape)}")
+        if target is not None and prefix is not None:
+            raise ValueError(f"{self.layer_name}: targets see all of their sequence, a prefix goes with the sequence's own rows")
         lead, D = x.shape[:2], self.head_dim
         asks = x if target is None else target.unsqueeze(1) if target.dim() == 2 else target
         if asks.numel() == 0 or (target is None and x.numel() == 0):

@@ -66,3 +66,13 @@ def test_newest_queries_stand_at_the_last_key(nq, nk):
     assert bool(((got.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -18 * v.double().abs().max()).all())      # fp32, rounded once
     with pytest.raises(ValueError, match="newest"):
         F.attention(q, k, v, causal=True, newest=True)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_a_prefix_does_not_go_with_targets(causal):
+    layer = tn.layers.SequenceAttention(16, heads=2, causal=causal)
+    prefix = torch.ones(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="targets see all"):
+        layer(torch.zeros(2, 5, 16), None, torch.zeros(2, 16), prefix=prefix)
+    if causal:
+        assert layer(torch.zeros(2, 5, 16), prefix=prefix).shape == (2, 5, 16)
