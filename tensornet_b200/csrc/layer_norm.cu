@@ -797,7 +797,7 @@ const char* bwd(const LayerNormArgs& a, int* part_rows, cudaStream_t st) {
       if (const char* err = told(launch_pdl(layer_norm_wide_sums_kernel<T>, dim3((a.C + 127) / 128, kWideSumRows), dim3(128), 0, st,
                                             (const T*)a.dy, (const T*)a.x, a.stats, a.rows, a.C, a.part)))
         return err;
-      return told(launch_pdl(layer_norm_add_kernel, dim3((2 * a.C + 31) / 32), dim3(32 * kAddRows), 0, st, a.part, kWideSumRows, a.C, a.dgamma,
+      return told(launch_pdl(layer_norm_add_kernel, dim3((unsigned)((2LL * a.C + 31) / 32)), dim3(32 * kAddRows), 0, st, a.part, kWideSumRows, a.C, a.dgamma,
                              a.dbeta));
     }
     return nullptr;
@@ -825,7 +825,7 @@ const char* bwd(const LayerNormArgs& a, int* part_rows, cudaStream_t st) {
     }
     if (part_rows) { *part_rows = grid; return nullptr; }
     if (err || !sums) return err;
-    return told(launch_pdl(layer_norm_add_kernel, dim3((2 * a.C + 31) / 32), dim3(32 * kAddRows), 0, st, a.part, grid, a.C, a.dgamma, a.dbeta));
+    return told(launch_pdl(layer_norm_add_kernel, dim3((unsigned)((2LL * a.C + 31) / 32)), dim3(32 * kAddRows), 0, st, a.part, grid, a.C, a.dgamma, a.dbeta));
   });
 }
 

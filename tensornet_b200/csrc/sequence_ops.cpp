@@ -55,7 +55,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
   static tn::LayerNormArgs args_of(const at::Tensor& x) {
     TORCH_CHECK(x.is_cuda() && (x.scalar_type() == at::kFloat || x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf),
                 "layer_norm: fp32, bf16 or fp16 rows on the GPU");
-    TORCH_CHECK(x.size(1) >= 1 && x.size(1) < (1LL << 31) - 64, "layer_norm: too many columns");
+    TORCH_CHECK(x.size(1) >= 1 && x.size(1) <= (1LL << 30), "layer_norm: too many columns");
     tn::LayerNormArgs a{};
     a.kind = x.scalar_type() == at::kFloat ? 0 : x.scalar_type() == at::kBFloat16 ? 1 : 2;
     a.rows = x.size(0); a.C = (int)x.size(1); a.x = x.data_ptr();

@@ -119,7 +119,7 @@ const char* launch_head_score(HeadArgs a, cudaStream_t st);
 struct LayerNormArgs {
   int kind;                             // of x, y, dy and dx: 0 fp32, 1 bf16, 2 fp16; rows behind one another, from 16-byte boundaries
   long long rows;                       // at least one
-  int C;
+  int C;                                // up to 2^30
   const void* x;
   const void* dy;
   const float* gamma;                   // [C]; null: ones

@@ -655,15 +655,18 @@ def embed_input(anchor, link, ids, offsets, B, S, D, combiner, labels=None, labe
 # layer normalisation
 # =========================================================================================
 _NORM_TYPES = (torch.float32, torch.bfloat16, torch.float16)
+_NORM_COLUMNS = 1 << 30
 _FP32_TINY = torch.finfo(torch.float32).tiny
 
 
 def layer_norm(x: torch.Tensor, gamma: Optional[torch.Tensor] = None, beta: Optional[torch.Tensor] = None, eps: float = 1e-5) -> torch.Tensor:
     """``(x - mean) / sqrt(var + eps) * gamma + beta`` with the moments of each row, the last dimension of ``x`` (fp32, bf16 or
-    fp16); the result has ``x``'s shape and type.  ``gamma`` and ``beta``: fp32 ``[columns]``, either may be left out.  Moments
+    fp16, up to 2^30 columns); the result has ``x``'s shape and type.  ``gamma`` and ``beta``: fp32 ``[columns]``, either may be left out.  Moments
     and sums are fp32, and the gradients of ``gamma`` and ``beta`` are summed in a fixed order.  Differentiable once."""
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"layer_norm: rows of one column or more, not {tuple(x.shape)}")
+    if x.shape[-1] > _NORM_COLUMNS:
+        raise ValueError(f"layer_norm: up to {_NORM_COLUMNS} columns, not {x.shape[-1]}")
     if x.dtype not in _NORM_TYPES:
         raise ValueError(f"layer_norm: fp32, bf16 or fp16, not {x.dtype}")
     columns, dev = x.shape[-1:], x.device
