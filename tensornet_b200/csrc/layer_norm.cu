@@ -126,11 +126,11 @@ __device__ __forceinline__ void warp_sum(float (&v)[kN], int tpr) {
     for (int o = tpr / 2; o > 0; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
 }
 
-// Sum over the block.  `s`: two rows of 32 values that take turns, so that one barrier per sum is enough.
+// Sum over the block.  `s`: two rows of 32 times kN values that take turns, so that one barrier per sum is enough.
 template <int kN>
-__device__ __forceinline__ void block_sum(float (&v)[kN], int threads, float* s, int& turn) {
+__device__ __forceinline__ void block_sum(float (&v)[kN], int threads, float2* s, int& turn) {
   warp_sum<kN>(v, 32);
-  float* row = s + turn * 32 * kN;
+  float* row = reinterpret_cast<float*>(s) + turn * 32 * kN;
   turn ^= 1;
   const int warp = threadIdx.x >> 5, warps = threads >> 5;      // an even number
   if ((threadIdx.x & 31) == 0)
@@ -387,7 +387,7 @@ layer_norm_row_fwd_kernel(const T* __restrict__ x, const float* __restrict__ gam
   using namespace attn;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ __align__(8) uint64_t s_full[kRing];
-  __shared__ float s_sum[64];
+  __shared__ float2 s_sum[32];
   __shared__ int s_abort_i;
   const int t = threadIdx.x, tpr = blockDim.x;
   if (t == 0) {
@@ -491,7 +491,7 @@ layer_norm_row_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, con
   using namespace attn;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ __align__(8) uint64_t s_full[kRing];
-  __shared__ float s_sum[128];
+  __shared__ float2 s_sum[64];
   __shared__ int s_abort_i;
   const int t = threadIdx.x, tpr = blockDim.x;
   if (t == 0) {
@@ -626,7 +626,7 @@ __global__ void __launch_bounds__(1024) layer_norm_wide_fwd_kernel(const T* __re
                                                                    const float* __restrict__ beta, float eps, long long rows, int C,
                                                                    T* __restrict__ y, float* __restrict__ stats) {
   pdl_sync();
-  __shared__ float s_sum[64];
+  __shared__ float2 s_sum[32];
   int turn = 0;
   for (long long r = blockIdx.x; r < rows; r += gridDim.x) {
     const T* row = x + r * C;
@@ -657,7 +657,7 @@ __global__ void __launch_bounds__(1024) layer_norm_wide_bwd_kernel(const T* __re
                                                                    const float* __restrict__ stats, const float* __restrict__ gamma,
                                                                    long long rows, int C, T* __restrict__ dx) {
   pdl_sync();
-  __shared__ float s_sum[128];
+  __shared__ float2 s_sum[64];
   int turn = 0;
   for (long long r = blockIdx.x; r < rows; r += gridDim.x) {
     const float mean = stats[r], rstd = stats[rows + r];

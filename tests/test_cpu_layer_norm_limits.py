@@ -13,3 +13,18 @@ def test_wider_rows_are_refused(columns):
 
 def test_the_widest_are_taken():
     assert F.layer_norm(torch.empty((1, 2 ** 30), device="meta")).shape == (1, 2 ** 30)
+
+
+def test_sums_over_a_block_lie_where_two_are_read_at_a_time():
+    """``block_sum`` reads its shared memory in pairs: what is handed to it has to be declared in pairs, which is what aligns it."""
+    import os
+    import re
+
+    import tensornet_b200
+
+    with open(os.path.join(os.path.dirname(tensornet_b200.__file__), "csrc", "layer_norm.cu")) as f:
+        text = f.read()
+    assert re.search(r"void block_sum\(.*float2\* s,", text)
+    assert len(re.findall(r"block_sum<\d>\(", text)) == 6
+    assert set(re.findall(r"block_sum<\d>\(\w+, \w+, (\w+),", text)) == {"s_sum"}
+    assert set(re.findall(r"__shared__ (\w+) s_sum\[", text)) == {"float2"}
