@@ -58,7 +58,7 @@ attention_few_kernel(const __grid_constant__ FewMaps maps, const __grid_constant
                      float* __restrict__ part_ml) {
   using S = FewShape<kD>;
   constexpr int kTilesN = S::keys / 8;
-  extern __shared__ uint8_t smem_raw[];
+  extern __shared__ __align__(16) uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t s_full[kWarps][S::stages];
   __shared__ float s_m[kWarps][kRowsM], s_l[kWarps][kRowsM];
   __shared__ int s_abort_i;
