@@ -756,7 +756,8 @@ const char* told(cudaError_t e) {
   return e == cudaSuccess ? nullptr : cudaGetErrorString(e);
 }
 
-constexpr int kWideSumRows = 64;      // rows of the workspace where a row is too wide for a block's registers
+// Rows of the workspace where a row is too wide for a block's registers
+int wide_sum_rows(long long rows) { return rows < 64 ? (int)rows : 64; }
 
 template <typename T>
 const char* fwd(const LayerNormArgs& a, cudaStream_t st) {
@@ -787,17 +788,18 @@ const char* bwd(const LayerNormArgs& a, int* part_rows, cudaStream_t st) {
   const Plan p = plan_of<T>(a.rows, a.C);
   const bool sums = a.dgamma != nullptr || a.dbeta != nullptr;
   if (p.wide) {
-    if (part_rows) { *part_rows = kWideSumRows; return nullptr; }
+    const int shares = wide_sum_rows(a.rows);
+    if (part_rows) { *part_rows = shares; return nullptr; }
     const int grid = (int)(a.rows < 592 ? a.rows : 592);
     if (a.dx != nullptr)
       if (const char* err = told(launch_pdl(layer_norm_wide_bwd_kernel<T>, dim3(grid), dim3(1024), 0, st, (const T*)a.dy, (const T*)a.x, a.stats,
                                             a.gamma, a.rows, a.C, (T*)a.dx)))
         return err;
     if (sums) {
-      if (const char* err = told(launch_pdl(layer_norm_wide_sums_kernel<T>, dim3((a.C + 127) / 128, kWideSumRows), dim3(128), 0, st,
+      if (const char* err = told(launch_pdl(layer_norm_wide_sums_kernel<T>, dim3((a.C + 127) / 128, shares), dim3(128), 0, st,
                                             (const T*)a.dy, (const T*)a.x, a.stats, a.rows, a.C, a.part)))
         return err;
-      return told(launch_pdl(layer_norm_add_kernel, dim3((unsigned)((2LL * a.C + 31) / 32)), dim3(32 * kAddRows), 0, st, a.part, kWideSumRows, a.C, a.dgamma,
+      return told(launch_pdl(layer_norm_add_kernel, dim3((unsigned)((2LL * a.C + 31) / 32)), dim3(32 * kAddRows), 0, st, a.part, shares, a.C, a.dgamma,
                              a.dbeta));
     }
     return nullptr;
