@@ -6,7 +6,7 @@
 //
 // One pass over the data each way: a row lies in the registers of a group of threads (a power of two of them, up to a block of 512),
 // so the variance is summed around the mean that was just found, without reading x again.  Sums are fp32.  Rows of more than 8192
-// elements are read again for each sum, by a block of 1024 and out of L2.
+// elements (of some widths from 8186 on, as they start anywhere in 16 bytes) are read again for each sum, by a block of 1024 and out of L2.
 // What bounds it is memory where rows are within a warp: x once and y once forward, x and dy once and dx once backward.  Measured, fp32
 // 409600 x 64: 39 us forward (5.4 TB/s), 62 us backward (5.0 TB/s), its sums over rows included.  Rows that a block shares wait twice
 // for its sum of two numbers, and with 16 elements per thread the instructions between the waits take longer than the loads: bf16
@@ -379,11 +379,11 @@ struct RowSpan {
   }
 };
 
-template <typename T, int kNV>
+template <typename T>
 __global__ void __launch_bounds__(kWideBlock, 2)
 layer_norm_row_fwd_kernel(const T* __restrict__ x, const float* __restrict__ gamma, const float* __restrict__ beta, float eps, long long rows, int C,
                           int slot_bytes, T* __restrict__ y, float* __restrict__ stats, int* status) {
-  constexpr int n = Piece<T>::n;
+  constexpr int n = Piece<T>::n, kNV = kPerThread / n;      // (with half as many per thread, half the threads would hold the row)
   using namespace attn;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ __align__(8) uint64_t s_full[kRing];
@@ -483,11 +483,11 @@ layer_norm_row_fwd_kernel(const T* __restrict__ x, const float* __restrict__ gam
   }
 }
 
-template <typename T, int kNV>
+template <typename T>
 __global__ void __launch_bounds__(kWideBlock)
 layer_norm_row_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, const float* __restrict__ stats, const float* __restrict__ gamma,
                           long long rows, int C, int slot_bytes, T* __restrict__ dx, float* __restrict__ part, int* status) {
-  constexpr int n = Piece<T>::n;
+  constexpr int n = Piece<T>::n, kNV = kPerThread / n;      // (with half as many per thread, half the threads would hold the row)
   using namespace attn;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ __align__(8) uint64_t s_full[kRing];
@@ -774,7 +774,7 @@ const char* fwd(const LayerNormArgs& a, cudaStream_t st) {
       return told(launch_pdl(k, dim3(resident_grid(k, p.block, 0, p.blocks)), dim3(p.block), 0, st, (const T*)a.x, a.gamma, a.beta, a.eps, a.rows,
                              a.C, p.tpr, (T*)a.y, a.stats));
     }
-    auto* k = layer_norm_row_fwd_kernel<T, kNV>;
+    auto* k = layer_norm_row_fwd_kernel<T>;
     const int slot = slot_bytes<T>(a.C);
     const size_t smem = kRing * slot + 2 * slot / sizeof(T) * sizeof(float);
     cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);      // of the current device
@@ -816,7 +816,7 @@ const char* bwd(const LayerNormArgs& a, int* part_rows, cudaStream_t st) {
         err = told(launch_pdl(k, dim3(grid), dim3(p.block), smem, st, (const T*)a.dy, (const T*)a.x, a.stats, a.gamma, a.rows, a.C, p.tpr, (T*)a.dx,
                               sums ? a.part : nullptr));
     } else {
-      auto* k = layer_norm_row_bwd_kernel<T, kNV>;
+      auto* k = layer_norm_row_bwd_kernel<T>;
       const int slot = slot_bytes<T>(a.C);
       const size_t smem = 2 * kRing * slot + slot / sizeof(T) * sizeof(float);
       cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);      // of the current device
