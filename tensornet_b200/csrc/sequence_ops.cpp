@@ -65,7 +65,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const OptTensor& gamma, const OptTensor& beta, double eps, const at::Tensor& status, bool keep) {
     c10::cuda::CUDAGuard guard(x.device());
     const int64_t C = x.size(-1);
-    at::Tensor x2 = rows16(x, C), y = at::empty_like(x2), stats, kg, kb;
+    at::Tensor x2 = rows16(x, C), y = at::empty(x.sizes(), x.options()), stats, kg, kb;      // (y is no view: it may be changed in place)
     tn::LayerNormArgs a = args_of(x2);
     a.gamma = column_vec(gamma, x, "gamma", kg); a.beta = column_vec(beta, x, "beta", kb);
     a.eps = (float)eps; a.y = y.data_ptr(); a.status = status_of(status, x);
@@ -81,7 +81,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
       ctx->saved_data["status"] = status;
       ctx->saved_data["beta"] = has_beta ? (has_gamma ? 2 : 1) : -1;
     }
-    return y.view(x.sizes());
+    return y;
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
